@@ -319,6 +319,64 @@ int stbpe_rows_count_pairs_noalloc(const int32_t *tokens, const uint8_t *valid, 
                                    int32_t *pair_keys, int64_t *pair_counts, int64_t cap,
                                    int64_t *length_dev, void *stream, char *err, size_t err_len);
 
+/* Losses over a large vocabulary at the output layer of a language model, without its logits: for a row h of hidden
+ * and the rows w_j of weight, z_j = h . w_j,
+ *   k == 0 : cross entropy, loss = log sum_j exp(z_j) - z_id
+ *   k > 0  : distillation from a teacher's top k logits, softened by the temperature T: with p = softmax(logits / T) over the
+ *            entries of the row, loss = T^2 sum_e p_e (log p_e - log softmax(z / T)_id_e)
+ * They have no counterpart in the reference, whose padded batches (tokens, valid) they take.  Rows are outer x inner,
+ * every array is reached by its strides (in elements, the last dimension contiguous).  A row does not count where valid is 0, its
+ * id is negative (k == 0), or it has no entry with an id of 0 or more and a logit above -inf (k > 0): its loss and its row of
+ * grad_hidden are 0 and what it holds is not multiplied.  An id of vocab or more, or a logit of NaN or +inf, gives NaN.
+ *   STBPE_WANT_LOSS  : loss[rows] (no reduction) or loss[1] (sum, or mean over the rows that count; 0 if none does), and
+ *                      lse2[rows], log2 of the sum, which a later call for the gradients takes
+ *   STBPE_WANT_GRADS : grad_hidden[rows][dim] and grad_weight[vocab][dim] in the inputs' type (NULL: not wanted), times
+ *                      grad_loss (one value, or one per row without a reduction; NULL: 1).  Alone, lse2 comes from a
+ *                      call with the same inputs.
+ * The call reads nothing back and does not synchronise: it can be captured.  workspace: device memory on a 1024-byte
+ * boundary, of the size that stbpe_vocab_loss_workspace gives for the same arguments; nothing in it outlasts the call.
+ * err may be NULL. */
+#define STBPE_REAL_BF16 0
+#define STBPE_REAL_FP16 1
+#define STBPE_REAL_FP32 2
+#define STBPE_REDUCE_NONE 0
+#define STBPE_REDUCE_SUM 1
+#define STBPE_REDUCE_MEAN 2
+#define STBPE_WANT_LOSS 1
+#define STBPE_WANT_GRADS 2
+#define STBPE_VOCAB_LOSS_MAX_K 256
+
+typedef struct stbpe_vocab_loss {
+    int64_t outer, inner, vocab, dim;
+    int32_t type;                /* of hidden, weight and the gradients: STBPE_REAL_BF16 or _FP16 */
+    int32_t k;                   /* teacher's entries per row, 0: cross entropy */
+    int32_t ids_bytes;           /* 4 or 8 */
+    int32_t logits_type;         /* STBPE_REAL_* */
+    int32_t reduction;           /* STBPE_REDUCE_* */
+    int32_t want;                /* STBPE_WANT_* */
+    float temperature;           /* 1 where k is 0 */
+    int32_t reserved;
+    const void *hidden;          /* [outer][inner][dim] */
+    int64_t hidden_outer, hidden_inner;
+    const void *weight;          /* [vocab][dim] */
+    int64_t weight_stride;
+    const void *ids;             /* [outer][inner], or [outer][inner][k] */
+    int64_t ids_outer, ids_inner;
+    const void *logits;          /* [outer][inner][k] */
+    int64_t logits_outer, logits_inner;
+    const uint8_t *valid;        /* [outer][inner], NULL: all rows */
+    int64_t valid_outer, valid_inner;
+    const float *grad_loss;
+    int64_t grad_outer, grad_inner;
+    float *loss, *lse2;
+    void *grad_hidden, *grad_weight;
+    void *workspace;
+    int64_t workspace_bytes;
+} stbpe_vocab_loss;
+
+int stbpe_vocab_loss_workspace(const stbpe_vocab_loss *args, int64_t *bytes, char *err, size_t err_len);
+int stbpe_vocab_loss_run(const stbpe_vocab_loss *args, void *stream, char *err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

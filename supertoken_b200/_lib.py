@@ -31,6 +31,22 @@ class State(ctypes.Structure):
                 ("tile_bytes_in", ctypes.c_int64), ("tile_bytes_out", ctypes.c_int64)]
 
 
+class VocabLoss(ctypes.Structure):
+    _fields_ = [("outer", ctypes.c_int64), ("inner", ctypes.c_int64), ("vocab", ctypes.c_int64), ("dim", ctypes.c_int64),
+                ("type", ctypes.c_int32), ("k", ctypes.c_int32), ("ids_bytes", ctypes.c_int32),
+                ("logits_type", ctypes.c_int32), ("reduction", ctypes.c_int32), ("want", ctypes.c_int32),
+                ("temperature", ctypes.c_float), ("reserved", ctypes.c_int32),
+                ("hidden", ctypes.c_void_p), ("hidden_outer", ctypes.c_int64), ("hidden_inner", ctypes.c_int64),
+                ("weight", ctypes.c_void_p), ("weight_stride", ctypes.c_int64),
+                ("ids", ctypes.c_void_p), ("ids_outer", ctypes.c_int64), ("ids_inner", ctypes.c_int64),
+                ("logits", ctypes.c_void_p), ("logits_outer", ctypes.c_int64), ("logits_inner", ctypes.c_int64),
+                ("valid", ctypes.c_void_p), ("valid_outer", ctypes.c_int64), ("valid_inner", ctypes.c_int64),
+                ("grad_loss", ctypes.c_void_p), ("grad_outer", ctypes.c_int64), ("grad_inner", ctypes.c_int64),
+                ("loss", ctypes.c_void_p), ("lse2", ctypes.c_void_p),
+                ("grad_hidden", ctypes.c_void_p), ("grad_weight", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+
 # every symbol include/stbpe.h declares: name -> (restype, argtypes)
 _vp, _i64, _i32, _int = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int
 _P = ctypes.POINTER
@@ -86,6 +102,8 @@ SIGNATURES = {
     "stbpe_rows_count_pairs": (_int, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp]),
     "stbpe_rows_count_pairs_noalloc": (_int, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp,
                                               ctypes.c_char_p, ctypes.c_size_t]),
+    "stbpe_vocab_loss_workspace": (_int, [_P(VocabLoss), _P(_i64), ctypes.c_char_p, ctypes.c_size_t]),
+    "stbpe_vocab_loss_run": (_int, [_P(VocabLoss), _vp, ctypes.c_char_p, ctypes.c_size_t]),
     "stbpe_rows_apply_merge": (_int, [_vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp]),
 }
 

@@ -8,7 +8,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libstbpe.so")
-SOURCES = ["engine.cu", "rows_ops.cu"]
+SOURCES = ["engine.cu", "rows_ops.cu", "vocab_loss.cu"]
 INCLUDE = os.path.join(HERE, "..", "include")
 
 

@@ -1,0 +1,541 @@
+// Losses over a large vocabulary, straight from the output layer's input: cross entropy, and distillation from a
+// teacher's top logits.  With h_i a row of `hidden`, w_j a row of `weight`, s = 1 / temperature and entries
+// (t_ik, p_ik) of row i (cross entropy: one, p = 1; s = 1):
+//   z_ij = h_i . w_j              lse_i = log sum_j exp(s z_ij)
+//   loss_i = T^2 (lse_i + sum_k p_ik (log p_ik - s z_i,t_ik))
+//   G_ij = g_i T (exp(s z_ij - lse_i) - sum_k p_ik [j = t_ik])       dH = G W        dW = G^T H
+// z is never stored: the forward product keeps (maximum, sum, sum_k p z) of each row and piece of columns, the
+// backward one makes G for a piece of the vocabulary at a time, from which both gradients take their share.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdio>
+
+#include "../../include/stbpe.h"
+#include "vocab_loss.cuh"
+
+#define STBPE_VISIBLE __attribute__((visibility("default")))
+
+namespace {
+using namespace vloss;
+
+// ---------------------------------------------------------------------------------------------- rows and entries
+__device__ __forceinline__ i64 load_id(const void *p, int bytes, i64 at) {
+    return bytes == 8 ? ((const i64 *)p)[at] : (i64)((const int32_t *)p)[at];
+}
+
+__device__ __forceinline__ float load_real(const void *p, int type, i64 at) {
+    if (type == STBPE_REAL_BF16) return __bfloat162float(((const __nv_bfloat16 *)p)[at]);
+    if (type == STBPE_REAL_FP16) return __half2float(((const __half *)p)[at]);
+    return ((const float *)p)[at];
+}
+
+// One warp per row: softmax of the teacher's entries in 32 bits, entries in ascending order of their ids (the order in
+// which the products meet them), and for each piece of columns the first entry that lies in it or behind.  The ids
+// come in the order of the logits; 64-bit words (id, share) are ordered by a bitonic network in shared memory.
+// Floor: 8 to 12 bytes per entry.
+__global__ void __launch_bounds__(128) teacher_kernel(Plan p) {
+    extern __shared__ u64 sorted[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    u64 *e = sorted + (size_t)warp * p.k_sorted;
+    for (i64 row = (i64)blockIdx.x * 4 + warp; row < p.rows; row += (i64)gridDim.x * 4) {
+        const i64 o = row / p.inner, i = row - o * p.inner;
+        const i64 id_at = o * p.ids_outer + i * p.ids_inner, real_at = o * p.logits_outer + i * p.logits_inner;
+        // rounded before anything is taken from it: the maximum less itself has to be 0 at the type's lowest value, too
+        auto softened = [&](i64 at) { return __fmul_rn(load_real(p.logits, p.logits_type, at), p.inv_temperature); };
+        float top = -INFINITY;
+        bool outside = false, nan = false;
+        for (int k = lane; k < p.k; k += 32) {
+            const i64 id = load_id(p.ids, p.ids_bytes, id_at + k);
+            if (id < 0) continue;
+            const float t = softened(real_at + k);
+            outside |= id >= p.vocab;
+            nan |= isnan(t) || t == INFINITY;
+            top = fmaxf(top, t);
+        }
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+        outside = __any_sync(~0u, outside), nan = __any_sync(~0u, nan);
+        const bool counted = top > -INFINITY || nan;
+        float sum = 0.f;
+        for (int k = lane; k < p.k; k += 32) {
+            const i64 id = load_id(p.ids, p.ids_bytes, id_at + k);
+            if (id >= 0 && counted) sum += expf(softened(real_at + k) - top);
+        }
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        const float inv = 1.f / sum, log_sum = logf(sum);
+        float plogp = 0.f;
+        for (int k = lane; k < p.k_sorted; k += 32) {
+            u64 word = ~0ull;  // no entry: behind all others
+            if (k < p.k && counted && !outside && !nan) {
+                const i64 id = load_id(p.ids, p.ids_bytes, id_at + k);
+                if (id >= 0) {
+                    const float x = softened(real_at + k) - top;
+                    const float share = expf(x) * inv;
+                    if (share > 0.f) {
+                        plogp += share * (x - log_sum);
+                        word = ((u64)id << 32) | __float_as_uint(share);
+                    }
+                }
+            }
+            e[k] = word;
+        }
+        for (int d = 16; d; d >>= 1) plogp += __shfl_xor_sync(~0u, plogp, d);
+        __syncwarp();
+        for (int size = 2; size <= p.k_sorted; size <<= 1)
+            for (int step = size >> 1; step; step >>= 1) {
+                for (int k = lane; k < p.k_sorted / 2; k += 32) {
+                    const int a = 2 * k - (k & (step - 1)), b = a + step;
+                    const u64 x = e[a], y = e[b];
+                    if ((x > y) == !(a & size)) e[a] = y, e[b] = x;
+                }
+                __syncwarp();
+            }
+        for (int k = lane; k < p.k; k += 32) {
+            const u64 word = e[k];
+            p.entries[row * p.k + k] = word == ~0ull ? make_int2(INT_MAX, 0) : make_int2((int)(word >> 32), (int)word);
+        }
+        for (int t = lane; t < p.pieces; t += 32) {  // first entry at or behind the piece's first column
+            const u64 from = (u64)t * PIECE << 32;
+            int lo = 0, hi = p.k;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (e[mid] < from) lo = mid + 1;
+                else hi = mid;
+            }
+            p.first[row * p.pieces + t] = (unsigned short)lo;
+        }
+        if (lane == 0) {
+            p.plogp[row] = outside || nan ? NAN : plogp;
+            p.has_entries[row] = counted;
+        }
+        __syncwarp();
+    }
+}
+
+// One CTA: which rows count, in their order (row_of, slot_of); the entry of a cross entropy row.
+__global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
+    __shared__ int in_warp[32];
+    __shared__ int base;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) base = 0;
+    __syncthreads();
+    for (i64 r0 = 0; r0 < p.rows; r0 += 1024) {
+        const i64 row = r0 + threadIdx.x;
+        bool counted = false;
+        if (row < p.rows) {
+            const i64 o = row / p.inner, i = row - o * p.inner;
+            counted = !p.valid || p.valid[o * p.valid_outer + i * p.valid_inner];
+            if (p.k) {
+                counted = counted && p.has_entries[row];
+            } else {
+                const i64 id = load_id(p.ids, p.ids_bytes, o * p.ids_outer + i * p.ids_inner);
+                counted = counted && id >= 0;
+                const bool outside = id >= p.vocab;
+                p.entries[row] = make_int2(outside || id < 0 ? INT_MAX : (int)id, __float_as_int(1.f));
+                p.plogp[row] = outside ? NAN : 0.f;
+            }
+        }
+        const unsigned votes = __ballot_sync(~0u, counted);
+        if (lane == 0) in_warp[warp] = __popc(votes);
+        __syncthreads();
+        int before = base, all = 0;
+        for (int w = 0; w < 32; ++w) {
+            before += w < warp ? in_warp[w] : 0;
+            all += in_warp[w];
+        }
+        const int slot = before + __popc(votes & ((1u << lane) - 1));
+        if (row < p.rows) p.slot_of[row] = counted ? slot : -1;
+        if (counted) p.row_of[slot] = (int)row;
+        __syncthreads();
+        if (threadIdx.x == 0) base += all;
+        __syncthreads();
+    }
+    const int n = base;
+    for (i64 c = n + threadIdx.x; c < p.rows_padded; c += 1024) p.row_of[c] = -1;
+    if (threadIdx.x == 0) p.meta->counted = n, p.meta->error = 0;
+}
+
+// Counted rows of `hidden` one behind another, zeros up to the end of the last tile: products then do no work for
+// padding, never multiply what a masked row holds (it may be NaN), and may read rows of any stride or alignment.
+template <class T>
+__global__ void __launch_bounds__(256) gather_kernel(Plan p) {
+    const int lane = threadIdx.x & 31;
+    const i64 n = p.meta->counted, until = (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS;
+    for (i64 c = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); c < until; c += (i64)gridDim.x * 8) {
+        T *to = (T *)p.packed + c * p.dim_padded;
+        if (c >= n) {
+            for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)(to + d) = make_uint4(0, 0, 0, 0);
+            continue;
+        }
+        const i64 row = p.row_of[c], o = row / p.inner, i = row - o * p.inner;
+        const T *from = (const T *)p.hidden + o * p.hidden_outer + i * p.hidden_inner;
+        if (p.hidden_aligned) {
+            for (int d = lane * 8; d < p.dim; d += 256) *(uint4 *)(to + d) = *(const uint4 *)(from + d);
+        } else {
+            for (int d = lane; d < p.dim_padded; d += 32) to[d] = d < p.dim ? from[d] : T(0.f);
+        }
+    }
+}
+
+// A weight whose rows do not start on 16-byte boundaries, copied so that they do.
+template <class T>
+__global__ void __launch_bounds__(256) align_weight_kernel(Plan p, T *to) {
+    const int lane = threadIdx.x & 31;
+    for (i64 j = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); j < p.vocab; j += (i64)gridDim.x * 8) {
+        const T *from = (const T *)p.weight + j * p.weight_stride;
+        for (int d = lane; d < p.dim_padded; d += 32) to[j * p.dim_padded + d] = d < p.dim ? from[d] : T(0.f);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- after the products
+// One warp per row: joins what the pieces of columns left, in a fixed order.
+__global__ void __launch_bounds__(256) join_kernel(Plan p) {
+    const int lane = threadIdx.x & 31;
+    for (i64 row = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); row < p.rows; row += (i64)gridDim.x * 8) {
+        const int c = p.slot_of[row];
+        float loss = 0.f, lse2 = 0.f;
+        if (c >= 0) {
+            float top = LOWEST, sum = 0.f, pz = 0.f;
+            for (int t = lane; t < p.pieces; t += 32) {
+                const i64 at = (i64)t * p.rows_padded + c;
+                const float m = p.part_max[at], x = p.part_sum[at];
+                pz += p.part_pz[at];
+                const float both = fmaxf(top, m);
+                sum = sum * exp2f(top - both) + x * exp2f(m - both);
+                top = both;
+            }
+            for (int d = 16; d; d >>= 1) {
+                const float m = __shfl_xor_sync(~0u, top, d), x = __shfl_xor_sync(~0u, sum, d);
+                const float both = fmaxf(top, m);
+                sum = sum * exp2f(top - both) + x * exp2f(m - both);
+                top = both;
+                pz += __shfl_xor_sync(~0u, pz, d);
+            }
+            lse2 = top + log2f(sum);
+            const float tau = p.temperature;
+            loss = tau * tau * (lse2 * 0.69314718055994531f + p.plogp[row] - pz * p.inv_temperature);
+        }
+        if (lane == 0) {
+            if (p.meta->error) loss = NAN;
+            p.lse2[row] = lse2;
+            p.row_loss[row] = loss;
+        }
+    }
+}
+
+// One CTA: the reduced loss, and what each counted row's G is multiplied by.  G is held in the inputs' 16-bit type, so it is
+// brought into that type's range: the largest |g_i T| becomes 2^14 (a power of two, so bf16 loses nothing; fp16 keeps
+// shares down to 2^-28 at full precision and its entries stay below 2^15), and both gradients are scaled back in 32 bits.
+__global__ void __launch_bounds__(1024) finish_kernel(Plan p) {
+    __shared__ float part[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const i64 n = p.meta->counted;
+    if (p.want_loss && p.reduction != STBPE_REDUCE_NONE) {
+        float sum = 0.f;
+        for (i64 r = threadIdx.x; r < p.rows; r += 1024) sum += p.row_loss[r];
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        if (lane == 0) part[warp] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            float all = 0.f;
+            for (int w = 0; w < 32; ++w) all += part[w];
+            p.loss[0] = p.reduction == STBPE_REDUCE_MEAN ? all / (float)(n > 0 ? n : 1) : all;
+        }
+        __syncthreads();
+    }
+    if (!p.want_grads) return;
+    const float factor = p.temperature / (p.reduction == STBPE_REDUCE_MEAN ? (float)(n > 0 ? n : 1) : 1.f);
+    auto g = [&](i64 c) {
+        const i64 row = p.row_of[c], o = row / p.inner, i = row - o * p.inner;
+        const float up = !p.grad_loss ? 1.f : p.grad_loss[p.reduction == STBPE_REDUCE_NONE ? o * p.grad_outer + i * p.grad_inner : 0];
+        return isnan(p.plogp[row]) ? NAN : up * factor;
+    };
+    float most = 0.f;
+    for (i64 c = threadIdx.x; c < n; c += 1024) {
+        const float x = fabsf(g(c));
+        if (x <= 3.4e38f) most = fmaxf(most, x);
+    }
+    for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+    if (lane == 0) part[warp] = most;
+    __syncthreads();
+    for (int w = 0; w < 32; ++w) most = fmaxf(most, part[w]);
+    // 2^14 over the next power of two, both sides kept within what 32 bits hold as normal numbers
+    int up = 0;
+    if (most > 0.f) frexpf(most, &up);
+    up = max(-100, min(100, up));
+    const float in = ldexpf(1.f, 14 - up);
+    if (threadIdx.x == 0) p.meta->out_scale = ldexpf(1.f, up - 14);
+    for (i64 c = threadIdx.x; c < p.rows_padded; c += 1024) p.coef[c] = c < n ? g(c) * in : 0.f;
+}
+
+// dH in the caller's rows and type: sums over the pieces and splits of the vocabulary, zeros where a row does not count.
+template <class T>
+__global__ void __launch_bounds__(256) scatter_kernel(Plan p) {
+    const float scale = p.meta->error ? NAN : p.meta->out_scale;
+    const i64 total = p.rows * p.dim;
+    for (i64 x = (i64)blockIdx.x * 256 + threadIdx.x; x < total; x += (i64)gridDim.x * 256) {
+        const i64 row = x / p.dim, d = x - row * p.dim;
+        const int c = p.slot_of[row];
+        float v = 0.f;
+        if (c >= 0) {
+            for (int s = 0; s < p.splits; ++s) v += p.acc[((i64)s * p.rows_padded + c) * p.dim + d];
+            v *= scale;
+        }
+        ((T *)p.grad_hidden)[x] = T(v);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- products
+// 64 x 64 results by 256 threads, 16 terms at a time through shared memory, all sums in 32 bits.
+enum { STATS, MAKE_G, GRAD_HIDDEN, GRAD_WEIGHT };
+
+template <class T, int KIND>
+__global__ void __launch_bounds__(256) product_kernel(Plan p, i64 v0, i64 width, int first) {
+    __shared__ float a[16][68], b[16][68], z[64][65];
+    const i64 n = p.meta->counted;
+    const T *packed = (const T *)p.packed, *w = (const T *)p.weight_rows;
+    T *g = (T *)p.g;
+    const i64 rows = KIND == GRAD_WEIGHT ? width : (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS;
+    const i64 cols = KIND == STATS || KIND == MAKE_G ? width : p.dim;
+    const i64 depth = KIND == STATS || KIND == MAKE_G ? p.dim : KIND == GRAD_HIDDEN ? width : n;
+    const i64 tiles_m = (rows + 63) / 64, tiles_n = (cols + 63) / 64;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    for (i64 tile = blockIdx.x; tile < tiles_m * tiles_n; tile += gridDim.x) {
+        const i64 m0 = tile % tiles_m * 64, n0 = tile / tiles_m * 64;
+        float c[4][4] = {};
+        for (i64 k0 = 0; k0 < depth; k0 += 16) {
+            for (int x = threadIdx.x; x < 1024; x += 256) {
+                i64 m, k, j;
+                float u = 0.f, v = 0.f;
+                if (KIND == STATS || KIND == MAKE_G) {
+                    k = k0 + (x & 15), m = m0 + (x >> 4), j = n0 + (x >> 4);
+                    if (k < depth && m < rows) u = (float)packed[m * p.dim_padded + k];
+                    if (k < depth && v0 + j < p.vocab) v = (float)w[(v0 + j) * p.weight_rows_stride + k];
+                    a[x & 15][x >> 4] = u, b[x & 15][x >> 4] = v;
+                } else {
+                    if (KIND == GRAD_HIDDEN) {
+                        k = k0 + (x & 15), m = m0 + (x >> 4);
+                        if (k < depth && m < rows) u = (float)g[m * p.g_stride + k];
+                        a[x & 15][x >> 4] = u;
+                    } else {
+                        k = k0 + (x >> 6), m = m0 + (x & 63);
+                        if (k < depth && m < rows) u = (float)g[k * p.g_stride + m];
+                        a[x >> 6][x & 63] = u;
+                    }
+                    k = k0 + (x >> 6), j = n0 + (x & 63);
+                    if (k < depth && j < cols) {
+                        if (KIND == GRAD_WEIGHT) v = (float)packed[k * p.dim_padded + j];
+                        else if (v0 + k < p.vocab) v = (float)w[(v0 + k) * p.weight_rows_stride + j];
+                    }
+                    b[x >> 6][x & 63] = v;
+                }
+            }
+            __syncthreads();
+            for (int k = 0; k < 16; ++k)
+                for (int y = 0; y < 4; ++y)
+                    for (int x = 0; x < 4; ++x) c[y][x] += a[k][ty * 4 + y] * b[k][tx * 4 + x];
+            __syncthreads();
+        }
+        if (KIND == GRAD_HIDDEN || KIND == GRAD_WEIGHT) {
+            for (int y = 0; y < 4; ++y)
+                for (int x = 0; x < 4; ++x) {
+                    const i64 m = m0 + ty * 4 + y, j = n0 + tx * 4 + x;
+                    if (m >= rows || j >= cols) continue;
+                    if (KIND == GRAD_HIDDEN) {
+                        float *to = p.acc + m * p.dim + j;
+                        *to = first ? c[y][x] : *to + c[y][x];
+                    } else if (v0 + m < p.vocab) {
+                        ((T *)p.grad_weight)[(v0 + m) * p.dim + j] = T(c[y][x] * p.meta->out_scale);
+                    }
+                }
+            continue;
+        }
+        for (int y = 0; y < 4; ++y)
+            for (int x = 0; x < 4; ++x) z[ty * 4 + y][tx * 4 + x] = c[y][x];
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            const int y = threadIdx.x;
+            const i64 m = m0 + y, row = p.row_of[m];
+            if (row < 0) {
+                if (KIND == MAKE_G)
+                    for (int x = 0; x < 64; ++x)
+                        if (n0 + x < p.g_stride) g[m * p.g_stride + n0 + x] = T(0.f);
+            } else {
+                const i64 k_all = p.k ? p.k : 1;
+                const int2 *e = p.entries + row * k_all;
+                i64 at = p.k ? p.first[row * p.pieces + (v0 + n0) / PIECE] : 0;
+                const float scale = p.inv_temperature * 1.4426950408889634f;
+                const float lse2 = KIND == MAKE_G ? p.lse2[row] : 0.f;
+                float top = LOWEST, sum = 0.f, pz = 0.f;
+                for (int x = 0; x < 64; ++x) {
+                    const i64 j = v0 + n0 + x;
+                    float v = z[y][x] * scale;
+                    float share = 0.f;
+                    while (at < k_all && e[at].x < j) ++at;
+                    while (at < k_all && e[at].x == j) share += __int_as_float(e[at].y), ++at;
+                    if (KIND == MAKE_G) {
+                        if (n0 + x < p.g_stride)
+                            g[m * p.g_stride + n0 + x] = T(j < p.vocab ? p.coef[m] * (exp2f(v - lse2) - share) : 0.f);
+                    } else if (j < p.vocab) {
+                        if (share != 0.f) pz += share * z[y][x];
+                        if (v > top) sum = sum * exp2f(top - v), top = v;
+                        sum += exp2f(v - top);
+                    }
+                }
+                if (KIND == STATS) {
+                    const i64 to = (v0 + n0) / PIECE * p.rows_padded + m;
+                    p.part_max[to] = top, p.part_sum[to] = sum, p.part_pz[to] = pz;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+#define VCK(call)                                                                              \
+    do {                                                                                       \
+        cudaError_t c_ = (call);                                                               \
+        if (c_ != cudaSuccess) return fail(err, err_len, STBPE_E_CUDA, #call, cudaGetErrorString(c_)); \
+    } while (0)
+
+int fail(char *err, size_t len, int status, const char *what, const char *why) {
+    if (err && len) snprintf(err, len, "%s: %s", what, why);
+    if (status == STBPE_E_CUDA) cudaGetLastError();
+    return status;
+}
+
+i64 up_to(i64 x, i64 unit) { return (x + unit - 1) / unit * unit; }
+
+// Checks the arguments and lays the workspace out; `bytes` gets its size.
+int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_len) {
+    auto bad = [&](const char *why) { return fail(err, err_len, STBPE_E_BADARG, "stbpe_vocab_loss", why); };
+    if (!a) return bad("no arguments");
+    if (a->outer < 0 || a->inner < 0 || a->vocab < 1 || a->dim < 1) return bad("negative or empty size");
+    if (a->vocab > INT_MAX - 65536 || a->dim > (1 << 20)) return bad("vocabulary or width too large");
+    if (a->inner && a->outer > (INT_MAX - 65536) / a->inner) return bad("too many rows");
+    if (a->type != STBPE_REAL_BF16 && a->type != STBPE_REAL_FP16) return bad("hidden and weight are bf16 or fp16");
+    if (a->k < 0 || a->k > STBPE_VOCAB_LOSS_MAX_K) return bad("number of teacher entries out of range");
+    if (a->ids_bytes != 4 && a->ids_bytes != 8) return bad("ids have 4 or 8 bytes");
+    if (a->k && (a->logits_type < STBPE_REAL_BF16 || a->logits_type > STBPE_REAL_FP32)) return bad("type of the teacher's logits");
+    if (!(a->temperature > 0.f) || !std::isfinite(a->temperature) || !std::isfinite(1.f / a->temperature)) return bad("temperature is positive and finite");
+    if (!a->k && a->temperature != 1.f) return bad("cross entropy has no temperature");
+    if (a->reduction < STBPE_REDUCE_NONE || a->reduction > STBPE_REDUCE_MEAN) return bad("reduction");
+    if (!(a->want & (STBPE_WANT_LOSS | STBPE_WANT_GRADS))) return bad("nothing is wanted");
+    p = Plan{};
+    p.rows = a->outer * a->inner, p.inner = a->inner > 0 ? a->inner : 1;
+    p.vocab = a->vocab, p.dim = a->dim, p.k = a->k;
+    p.dim_padded = up_to(a->dim, 8);
+    p.rows_padded = up_to(p.rows > 0 ? p.rows : 1, TILE_ROWS);
+    p.pieces = (int)((a->vocab + PIECE - 1) / PIECE);
+    p.k_sorted = 2;
+    while (p.k_sorted < a->k) p.k_sorted *= 2;
+    p.temperature = a->temperature, p.inv_temperature = 1.f / a->temperature;
+    p.reduction = a->reduction;
+    p.want_loss = (a->want & STBPE_WANT_LOSS) != 0, p.want_grads = (a->want & STBPE_WANT_GRADS) != 0;
+    p.hidden = a->hidden, p.hidden_outer = a->hidden_outer, p.hidden_inner = a->hidden_inner;
+    p.hidden_aligned = (uintptr_t)a->hidden % 16 == 0 && a->hidden_outer % 8 == 0 && a->hidden_inner % 8 == 0 && a->dim % 8 == 0;
+    p.weight = a->weight, p.weight_stride = a->weight_stride;
+    p.ids = a->ids, p.ids_bytes = a->ids_bytes, p.ids_outer = a->ids_outer, p.ids_inner = a->ids_inner;
+    p.logits = a->logits, p.logits_type = a->logits_type, p.logits_outer = a->logits_outer, p.logits_inner = a->logits_inner;
+    p.valid = a->valid, p.valid_outer = a->valid_outer, p.valid_inner = a->valid_inner;
+    p.grad_loss = a->grad_loss, p.grad_outer = a->grad_outer, p.grad_inner = a->grad_inner;
+    p.loss = a->loss, p.lse2 = a->lse2, p.grad_hidden = a->grad_hidden, p.grad_weight = a->grad_weight;
+    const bool aligned = (uintptr_t)a->weight % 16 == 0 && a->weight_stride % 8 == 0 && a->dim % 8 == 0;
+    p.weight_rows_stride = aligned ? a->weight_stride : p.dim_padded;
+    // as many columns of G at a time as 256 MiB hold
+    i64 width = up_to(a->vocab, PIECE);
+    const i64 most = (256ll << 20) / (2 * p.rows_padded) / PIECE * PIECE;
+    if (width > most) width = most > 2048 ? most : (width < 2048 ? width : 2048);
+    p.g_stride = width;
+    p.splits = 1;
+    bytes = 0;
+    char *base = (char *)a->workspace;
+    auto take = [&](i64 n) {
+        char *at = base + bytes;
+        bytes += up_to(n, 1024);
+        return (void *)at;
+    };
+    p.meta = (Meta *)take(sizeof(Meta));
+    p.row_of = (int *)take(p.rows_padded * 4);
+    p.slot_of = (int *)take(p.rows_padded * 4);
+    p.plogp = (float *)take(p.rows_padded * 4);
+    p.entries = (int2 *)take(p.rows_padded * 8 * (p.k ? p.k : 1));
+    if (p.k) {
+        p.first = (unsigned short *)take(p.rows_padded * 2 * p.pieces);
+        p.has_entries = (unsigned char *)take(p.rows_padded);
+    }
+    p.packed = take(p.rows_padded * p.dim_padded * 2);
+    p.weight_rows = aligned ? a->weight : take(p.vocab * p.dim_padded * 2);
+    if (p.want_loss) {
+        p.part_max = (float *)take(p.rows_padded * 4 * p.pieces);
+        p.part_sum = (float *)take(p.rows_padded * 4 * p.pieces);
+        p.part_pz = (float *)take(p.rows_padded * 4 * p.pieces);
+        p.row_loss = a->reduction == STBPE_REDUCE_NONE ? a->loss : (float *)take(p.rows_padded * 4);
+    }
+    if (p.want_grads) {
+        p.coef = (float *)take(p.rows_padded * 4);
+        p.g = take(p.rows_padded * p.g_stride * 2);
+        if (p.grad_hidden) p.acc = (float *)take((i64)p.splits * p.rows_padded * p.dim * 4);
+    }
+    return STBPE_OK;
+}
+
+template <class T>
+int run(const Plan &p, cudaStream_t s, char *err, size_t err_len) {
+    const int wide = 148 * 8;
+    auto blocks = [&](i64 n, i64 per) { return (unsigned)(n <= 0 ? 1 : (n + per - 1) / per < wide ? (n + per - 1) / per : wide); };
+    if (p.k) teacher_kernel<<<blocks(p.rows, 4), 128, 4 * p.k_sorted * sizeof(u64), s>>>(p);
+    rows_kernel<<<1, 1024, 0, s>>>(p);
+    gather_kernel<T><<<blocks(p.rows_padded, 8), 256, 0, s>>>(p);
+    if (p.weight_rows != p.weight) align_weight_kernel<T><<<blocks(p.vocab, 8), 256, 0, s>>>(p, (T *)p.weight_rows);
+    if (p.want_loss) {
+        product_kernel<T, STATS><<<wide, 256, 0, s>>>(p, 0, p.vocab, 0);
+        join_kernel<<<blocks(p.rows, 8), 256, 0, s>>>(p);
+    }
+    if (p.want_grads || p.reduction != STBPE_REDUCE_NONE) finish_kernel<<<1, 1024, 0, s>>>(p);
+    if (p.want_grads) {
+        for (i64 v0 = 0; v0 < p.vocab; v0 += p.g_stride) {
+            const i64 width = p.vocab - v0 < p.g_stride ? p.vocab - v0 : p.g_stride;
+            product_kernel<T, MAKE_G><<<wide, 256, 0, s>>>(p, v0, width, 0);
+            if (p.grad_hidden) product_kernel<T, GRAD_HIDDEN><<<wide, 256, 0, s>>>(p, v0, width, v0 == 0);
+            if (p.grad_weight) product_kernel<T, GRAD_WEIGHT><<<wide, 256, 0, s>>>(p, v0, width, 0);
+        }
+        if (p.grad_hidden) scatter_kernel<T><<<blocks(p.rows * p.dim, 256), 256, 0, s>>>(p);
+    }
+    VCK(cudaGetLastError());
+    return STBPE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+STBPE_VISIBLE int stbpe_vocab_loss_workspace(const stbpe_vocab_loss *args, int64_t *bytes, char *err, size_t err_len) {
+    Plan p;
+    i64 need = 0;
+    if (err && err_len) err[0] = 0;
+    const int st = plan(args, p, need, err, err_len);
+    if (st == STBPE_OK && bytes) *bytes = need;
+    return st;
+}
+
+STBPE_VISIBLE int stbpe_vocab_loss_run(const stbpe_vocab_loss *args, void *stream, char *err, size_t err_len) {
+    Plan p;
+    i64 need = 0;
+    if (err && err_len) err[0] = 0;
+    const int st = plan(args, p, need, err, err_len);
+    if (st != STBPE_OK) return st;
+    if (!args->workspace || (uintptr_t)args->workspace % 1024 || args->workspace_bytes < need)
+        return fail(err, err_len, STBPE_E_CAPACITY, "stbpe_vocab_loss", "workspace missing, not on a 1024-byte boundary or too small");
+    if (!args->lse2 || (p.want_loss && !args->loss) || (p.want_grads && !args->grad_hidden && !args->grad_weight))
+        return fail(err, err_len, STBPE_E_BADARG, "stbpe_vocab_loss", "an output is missing");
+    if (!args->weight || (p.rows && (!args->hidden || !args->ids || (p.k && !args->logits))))
+        return fail(err, err_len, STBPE_E_BADARG, "stbpe_vocab_loss", "an input is missing");
+    return args->type == STBPE_REAL_BF16 ? run<__nv_bfloat16>(p, (cudaStream_t)stream, err, err_len)
+                                         : run<__half>(p, (cudaStream_t)stream, err, err_len);
+}
+
+}  // extern "C"

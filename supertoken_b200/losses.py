@@ -1,0 +1,232 @@
+"""Losses over a large vocabulary at the output layer of a language model, on the padded batches that the other
+operators take: cross entropy with token ids, and distillation from a teacher's top logits.
+
+``hidden @ weight.T`` are the logits, which are never kept: the kernels go over the vocabulary in pieces.  Shapes:
+``hidden`` ``[N, D]`` or ``[B, L, D]``, ``weight`` ``[V, D]``, both bfloat16 or both float16; ``targets`` and ``valid``
+like ``hidden`` without its last dimension, ``teacher_ids`` and ``teacher_logits`` with the teacher's ``K`` entries as
+their last.  Any strides, but for the last dimension of ``hidden``, ``weight`` and the teacher's tensors, which is contiguous, so
+``hidden[:, :-1]`` with ``tokens[:, 1:]`` and ``valid[:, 1:]`` is the next-token loss of a batch.
+
+A row counts unless ``valid`` is 0 there or its target is negative (the padding of the batches); with a teacher, unless it has
+no entry with an id of 0 or more and a logit above ``-inf``.  Rows that do not count have a loss and a gradient of 0, and
+what ``hidden`` holds there is not looked at.  ``reduction="mean"`` divides by the rows that count (0 if none does).  Nothing is read back, so
+an id of ``V`` or more cannot raise: it makes the loss NaN, as a NaN among the inputs does.  Results are the same at every call with the same
+inputs; sums are held in 32 bits."""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib as L
+
+_REAL = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_WANT_LOSS, _WANT_GRADS = 1, 2
+MAX_TEACHER_ENTRIES = 256
+
+
+def _raise(status: int, msg: str) -> None:
+    if status == L.E_BADARG:
+        raise ValueError(msg)
+    raise RuntimeError(msg)
+
+
+def _rows(t: torch.Tensor, lead: int) -> Tuple[int, int]:
+    """Strides of the (outer, inner) row dimensions."""
+    return (t.stride(0), t.stride(1)) if lead == 2 else (0, t.stride(0))
+
+
+def _arguments(hidden, weight, ids, logits, valid, temperature, reduction) -> L.VocabLoss:
+    for t in (hidden, weight, ids) + ((logits,) if logits is not None else ()) + ((valid,) if valid is not None else ()):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("hidden, weight, ids, teacher_logits and valid must be tensors")
+        if not t.is_cuda:
+            raise RuntimeError("supertoken_b200 operators need CUDA tensors; there is no CPU fallback")
+        if t.device != hidden.device:
+            raise ValueError("tensors must be on one device")
+    if hidden.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != hidden.dtype:
+        raise TypeError("hidden and weight must both be bfloat16 or both be float16")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError("token ids must be int32 or int64")
+    if valid is not None and valid.dtype not in (torch.uint8, torch.bool):
+        raise TypeError("valid must be uint8 or bool")
+    if hidden.dim() not in (2, 3) or weight.dim() != 2 or weight.size(1) != hidden.size(-1):
+        raise ValueError("hidden must be [N, D] or [B, L, D] and weight [V, D]")
+    lead, shape = hidden.dim() - 1, hidden.shape[:-1]
+    if weight.size(0) < 1 or weight.size(1) < 1:
+        raise ValueError("weight must have at least one row and one column")
+    if reduction not in _REDUCTIONS:
+        raise ValueError("reduction must be 'none', 'sum' or 'mean'")
+    if valid is not None and valid.shape != shape:
+        raise ValueError("valid must have the shape of hidden without its last dimension")
+    if (hidden.stride(-1) != 1 and hidden.size(-1) > 1) or (weight.stride(-1) != 1 and weight.size(-1) > 1):
+        raise ValueError("the last dimension of hidden and weight must be contiguous")
+    a = L.VocabLoss()
+    a.k = 0
+    if logits is None:
+        if ids.shape != shape:
+            raise ValueError("targets must have the shape of hidden without its last dimension")
+    else:
+        if logits.dtype not in _REAL:
+            raise TypeError("teacher_logits must be bfloat16, float16 or float32")
+        if ids.dim() != lead + 1 or ids.shape[:-1] != shape or logits.shape != ids.shape:
+            raise ValueError("teacher_ids and teacher_logits must have the shape of hidden with K as last dimension")
+        a.k = ids.size(-1)
+        if not 1 <= a.k <= MAX_TEACHER_ENTRIES:
+            raise ValueError(f"a teacher gives 1 to {MAX_TEACHER_ENTRIES} entries per row")
+        if a.k > 1 and (ids.stride(-1) != 1 or logits.stride(-1) != 1):
+            raise ValueError("the last dimension of teacher_ids and teacher_logits must be contiguous")
+        if not (0.0 < temperature < float("inf")):
+            raise ValueError("temperature must be positive and finite")
+        a.logits, a.logits_type = logits.data_ptr(), _REAL[logits.dtype]
+        a.logits_outer, a.logits_inner = _rows(logits, lead)
+    a.outer, a.inner = (shape[0], shape[1]) if lead == 2 else (1, shape[0])
+    a.vocab, a.dim = weight.shape
+    a.type, a.ids_bytes = _REAL[hidden.dtype], ids.element_size()
+    a.reduction, a.temperature = _REDUCTIONS[reduction], temperature
+    a.hidden, a.weight, a.ids = hidden.data_ptr(), weight.data_ptr(), ids.data_ptr()
+    a.hidden_outer, a.hidden_inner = _rows(hidden, lead)
+    a.weight_stride = weight.stride(0)
+    a.ids_outer, a.ids_inner = _rows(ids, lead)
+    if valid is not None:
+        a.valid = valid.data_ptr()
+        a.valid_outer, a.valid_inner = _rows(valid, lead)
+    return a
+
+
+def _run(a: L.VocabLoss, device: torch.device) -> None:
+    lib, need, err = L.load(), ctypes.c_int64(0), ctypes.create_string_buffer(256)
+    with torch.cuda.device(device):
+        st = lib.stbpe_vocab_loss_workspace(ctypes.byref(a), ctypes.byref(need), err, 256)
+        if st == L.OK:
+            # torch's allocator knows streams and captures: a graph's workspace is in the graph's own pool
+            space = torch.empty(need.value + 1024, dtype=torch.uint8, device=device)
+            a.workspace, a.workspace_bytes = (space.data_ptr() + 1023) // 1024 * 1024, need.value
+            stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+            st = lib.stbpe_vocab_loss_run(ctypes.byref(a), stream, err, 256)
+    if st != L.OK:
+        _raise(st, err.value.decode())
+
+
+def _loss(hidden, weight, ids, logits, valid, temperature, reduction):
+    """The loss, and what the gradients need of it again."""
+    a = _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
+    shape = hidden.shape[:-1]
+    loss = torch.empty(shape if reduction == "none" else (), dtype=torch.float32, device=hidden.device)
+    lse2 = torch.empty(shape, dtype=torch.float32, device=hidden.device)
+    a.want, a.loss, a.lse2 = _WANT_LOSS, loss.data_ptr(), lse2.data_ptr()
+    if a.outer * a.inner == 0 and reduction == "none":
+        return loss, lse2
+    if lse2.numel() == 0:
+        lse2 = lse2.new_empty(1)  # no address without an element
+        a.lse2 = lse2.data_ptr()
+    _run(a, hidden.device)
+    return loss, lse2
+
+
+def _grads(hidden, weight, ids, logits, valid, temperature, reduction, grad_loss, lse2, want_hidden=True, want_weight=True):
+    """(loss or None, grad_hidden or None, grad_weight or None); without ``lse2`` the loss is made, too."""
+    a = _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
+    dev, shape, loss = hidden.device, hidden.shape[:-1], None
+    if grad_loss is not None:
+        if not isinstance(grad_loss, torch.Tensor):
+            grad_loss = torch.full((), float(grad_loss), dtype=torch.float32, device=dev)
+        if grad_loss.device != dev:
+            raise ValueError("tensors must be on one device")
+        if grad_loss.dtype != torch.float32:
+            raise TypeError("grad_loss must be float32")
+        if reduction == "none" and grad_loss.shape == shape:
+            a.grad_outer, a.grad_inner = _rows(grad_loss, len(shape))
+        elif grad_loss.numel() != 1:
+            raise ValueError("grad_loss must have one element, or the shape of the loss")
+        a.grad_loss = grad_loss.data_ptr()
+    a.want = _WANT_GRADS
+    if lse2 is None:
+        loss = torch.empty(shape if reduction == "none" else (), dtype=torch.float32, device=dev)
+        lse2 = torch.empty(max(1, a.outer * a.inner), dtype=torch.float32, device=dev)
+        # (a tensor without elements has no address)
+        a.want, a.loss = _WANT_LOSS | _WANT_GRADS, (loss if loss.numel() else lse2).data_ptr()
+    gh = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if want_hidden else None
+    gw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want_weight else None
+    a.lse2 = lse2.data_ptr()
+    a.grad_hidden = gh.data_ptr() if want_hidden and gh.numel() else None
+    a.grad_weight = gw.data_ptr() if want_weight else None
+    if a.grad_hidden or a.grad_weight:
+        _run(a, dev)
+    return loss, gh, gw
+
+
+class _VocabLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, ids, logits, valid, temperature, reduction):
+        loss, lse2 = _loss(hidden, weight, ids, logits, valid, temperature, reduction)
+        ctx.save_for_backward(hidden, weight, ids, logits, valid, lse2)
+        ctx.temperature, ctx.reduction = temperature, reduction
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss):
+        hidden, weight, ids, logits, valid, lse2 = ctx.saved_tensors
+        _refuse_capture(hidden.device)
+        _, gh, gw = _grads(hidden, weight, ids, logits, valid, ctx.temperature, ctx.reduction, grad_loss, lse2,
+                           ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return gh, gw, None, None, None, None, None
+
+
+def _refuse_capture(device: torch.device) -> None:
+    """torch adds a leaf's gradient on the stream that the leaf was first used on.  A captured backward pass reaches out
+    of its capture there when an eager graph of the same leaf is alive, which torch answers by ending the process."""
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a loss with autograd cannot be captured: capture the call that returns the gradients "
+                               "(vocab_cross_entropy_grads, vocab_distillation_grads)")
+
+
+def _differentiable(hidden, weight, ids, logits, valid, temperature, reduction):
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (hidden, weight)):
+        _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
+        _refuse_capture(hidden.device)
+        return _VocabLoss.apply(hidden, weight, ids, logits, valid, temperature, reduction)
+    return _loss(hidden, weight, ids, logits, valid, temperature, reduction)[0]
+
+
+def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                        valid: Optional[torch.Tensor] = None, *, reduction: str = "mean") -> torch.Tensor:
+    """``-log softmax(hidden @ weight.T)[targets]`` in float32: a scalar, or one per row with ``reduction="none"``.
+    Differentiable in ``hidden`` and ``weight``; without gradients wanted it can be captured into a graph."""
+    return _differentiable(hidden, weight, targets, None, valid, 1.0, reduction)
+
+
+def vocab_cross_entropy_grads(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                              valid: Optional[torch.Tensor] = None, grad_loss=None, *, reduction: str = "mean"
+                              ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(loss, grad_hidden, grad_weight)`` in one call without autograd, which can be captured into a graph.  The
+    gradients are contiguous, in the inputs' type, and times ``grad_loss``: a number, a float32 tensor of one element (a loss
+    scale), or with ``reduction="none"`` one of the loss's shape."""
+    with torch.no_grad():
+        return _grads(hidden, weight, targets, None, valid, 1.0, reduction, grad_loss, None)
+
+
+def vocab_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
+                       teacher_logits: torch.Tensor, valid: Optional[torch.Tensor] = None, *, temperature: float = 1.0,
+                       reduction: str = "mean") -> torch.Tensor:
+    """``T^2 KL(p || softmax(hidden @ weight.T / T))`` with ``p = softmax(teacher_logits / T)`` over the teacher's up to 256
+    entries of a row (in any order; an id below 0 is no entry, the same id twice counts twice).  Differentiable in
+    ``hidden`` and ``weight``; without gradients wanted it can be captured into a graph."""
+    if teacher_logits is None:
+        raise TypeError("teacher_logits must be a tensor")
+    return _differentiable(hidden, weight, teacher_ids, teacher_logits, valid, float(temperature), reduction)
+
+
+def vocab_distillation_grads(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
+                             teacher_logits: torch.Tensor, valid: Optional[torch.Tensor] = None, grad_loss=None, *,
+                             temperature: float = 1.0, reduction: str = "mean"
+                             ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(loss, grad_hidden, grad_weight)`` of ``vocab_distillation``, as ``vocab_cross_entropy_grads`` gives them."""
+    if teacher_logits is None:
+        raise TypeError("teacher_logits must be a tensor")
+    with torch.no_grad():
+        return _grads(hidden, weight, teacher_ids, teacher_logits, valid, float(temperature), reduction, grad_loss, None)

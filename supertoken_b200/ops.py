@@ -2,7 +2,10 @@
 ``select_best_pair`` with the reference's names, argument meaning and errors
 (``gpu_tokenizer/utils.py:691-706``, ``:413-555``; ``gpu_tokenizer/trainers/bpe_gpu.py:14-130``).
 Each call is one C-ABI call into ``libstbpe.so``; CPU tensors are rejected (the CPU path is
-the reference's own)."""
+the reference's own).
+
+On the same padded batches, the losses of a language model over the vocabulary that was trained:
+``vocab_cross_entropy``, ``vocab_distillation`` and their gradients (``losses.py``; no counterpart in the reference)."""
 from __future__ import annotations
 
 import ctypes
@@ -12,6 +15,8 @@ from typing import Callable, Optional, Sequence, Tuple
 import torch
 
 from . import _lib as L
+from .losses import (vocab_cross_entropy, vocab_cross_entropy_grads, vocab_distillation,  # noqa: F401
+                     vocab_distillation_grads)
 
 UINT32_MAX = (1 << 32) - 1
 

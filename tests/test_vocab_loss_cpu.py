@@ -1,0 +1,74 @@
+"""Arguments that the losses over a large vocabulary refuse before any GPU work, and the size of their workspace."""
+import ctypes
+
+import pytest
+import torch
+
+from supertoken_b200 import _lib as L
+from supertoken_b200 import losses, ops
+
+
+def _args(**more):
+    a = L.VocabLoss()
+    a.outer, a.inner, a.vocab, a.dim, a.type, a.k, a.ids_bytes = 4, 512, 32256, 1024, 0, 0, 4
+    a.reduction, a.want, a.temperature = 2, 3, 1.0
+    a.hidden, a.weight, a.weight_stride, a.hidden_outer, a.hidden_inner = 1 << 20, 2 << 20, 1024, 512 * 1024, 1024
+    a.grad_hidden, a.grad_weight = 3 << 20, 4 << 20
+    for name, value in more.items():
+        setattr(a, name, value)
+    return a
+
+
+def _need(a):
+    n, err = ctypes.c_int64(-1), ctypes.create_string_buffer(256)
+    st = L.load().stbpe_vocab_loss_workspace(ctypes.byref(a), ctypes.byref(n), err, 256)
+    return st, n.value, err.value.decode()
+
+
+@pytest.mark.parametrize("more", [
+    {"outer": -1}, {"inner": -1}, {"vocab": 0}, {"dim": 0}, {"vocab": 1 << 31}, {"dim": 1 << 21}, {"outer": 1 << 22, "inner": 1 << 10},
+    {"type": 2}, {"type": -1}, {"k": -1}, {"k": 257}, {"ids_bytes": 2}, {"k": 4, "logits_type": 3}, {"reduction": 3},
+    {"reduction": -1}, {"want": 0}, {"temperature": 2.0}, {"k": 4, "temperature": 0.0}, {"k": 4, "temperature": float("nan")},
+    {"k": 4, "temperature": float("inf")}, {"k": 4, "temperature": 1e-40}])
+def test_bad_arguments_are_refused(more):
+    st, n, text = _need(_args(**more))
+    assert st == L.E_BADARG and n == -1 and text.startswith("stbpe_vocab_loss: ")
+
+
+def test_nothing_runs_without_what_it_needs():
+    lib, err = L.load(), ctypes.create_string_buffer(256)
+    assert lib.stbpe_vocab_loss_run(None, None, err, 256) == L.E_BADARG
+    assert lib.stbpe_vocab_loss_workspace(None, None, None, 0) == L.E_BADARG
+    a = _args()
+    _, need, _ = _need(a)
+    for space, size in ((0, need), (1 << 30, need - 1), ((1 << 30) + 512, need)):
+        a.workspace, a.workspace_bytes = space, size
+        assert lib.stbpe_vocab_loss_run(ctypes.byref(a), None, err, 256) == L.E_CAPACITY
+    a.workspace, a.workspace_bytes = 1 << 30, need
+    assert lib.stbpe_vocab_loss_run(ctypes.byref(a), None, err, 256) == L.E_BADARG and b"output" in err.value
+    a.lse2 = a.loss = 5 << 20
+    assert lib.stbpe_vocab_loss_run(ctypes.byref(a), None, err, 256) == L.E_BADARG and b"input" in err.value
+
+
+def test_workspace_holds_no_logits():
+    """Its size follows the rows and a bounded piece of the vocabulary, not their product."""
+    logits = 32 * 2048 * 262144 * 2
+    for want in (1, 3):
+        st, n, _ = _need(_args(outer=32, inner=2048, vocab=262144, want=want))
+        assert st == L.OK and n < logits / 8
+    assert _need(_args(want=1))[1] < _need(_args(want=3))[1]
+    # a weight that starts anywhere is copied
+    assert _need(_args(weight=(2 << 20) + 2))[1] - _need(_args())[1] == 32256 * 1024 * 2
+    assert _need(_args(dim=1023))[1] > _need(_args())[1]
+    assert _need(_args(outer=0))[0] == L.OK
+
+
+def test_cpu_tensors_are_refused():
+    h, w, t = torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(5, 8, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: ops.vocab_cross_entropy(h, w, t), lambda: ops.vocab_cross_entropy_grads(h, w, t),
+                 lambda: ops.vocab_distillation(h, w, t[:, None], torch.zeros(2, 1)),
+                 lambda: ops.vocab_distillation_grads(h, w, t[:, None], torch.zeros(2, 1))):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+    with pytest.raises(TypeError):
+        losses.vocab_distillation(h, w, t[:, None], None)
