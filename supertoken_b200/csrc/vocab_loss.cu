@@ -14,9 +14,13 @@
 #include <cstdio>
 
 #include "../../include/stbpe.h"
-#include "vocab_loss.cuh"
+#include "vocab_products.cuh"
 
 #define STBPE_VISIBLE __attribute__((visibility("default")))
+
+#ifndef VL_GROUP
+#define VL_GROUP 2
+#endif
 
 namespace {
 using namespace vloss;
@@ -198,7 +202,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p) {
         float loss = 0.f, lse2 = 0.f;
         if (c >= 0) {
             float top = LOWEST, sum = 0.f, pz = 0.f;
-            for (int t = lane; t < p.pieces; t += 32) {
+            for (int t = lane; t < p.parts; t += 32) {
                 const i64 at = (i64)t * p.rows_padded + c;
                 const float m = p.part_max[at], x = p.part_sum[at];
                 pz += p.part_pz[at];
@@ -280,117 +284,10 @@ __global__ void __launch_bounds__(256) scatter_kernel(Plan p) {
         const int c = p.slot_of[row];
         float v = 0.f;
         if (c >= 0) {
-            for (int s = 0; s < p.splits; ++s) v += p.acc[((i64)s * p.rows_padded + c) * p.dim + d];
+            for (int s = 0; s < p.splits; ++s) v += p.acc[((i64)s * p.rows_padded + c) * p.acc_stride + d];
             v *= scale;
         }
         ((T *)p.grad_hidden)[x] = T(v);
-    }
-}
-
-// ---------------------------------------------------------------------------------------------- products
-// 64 x 64 results by 256 threads, 16 terms at a time through shared memory, all sums in 32 bits.
-enum { STATS, MAKE_G, GRAD_HIDDEN, GRAD_WEIGHT };
-
-template <class T, int KIND>
-__global__ void __launch_bounds__(256) product_kernel(Plan p, i64 v0, i64 width, int first) {
-    __shared__ float a[16][68], b[16][68], z[64][65];
-    const i64 n = p.meta->counted;
-    const T *packed = (const T *)p.packed, *w = (const T *)p.weight_rows;
-    T *g = (T *)p.g;
-    const i64 rows = KIND == GRAD_WEIGHT ? width : (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS;
-    const i64 cols = KIND == STATS || KIND == MAKE_G ? width : p.dim;
-    const i64 depth = KIND == STATS || KIND == MAKE_G ? p.dim : KIND == GRAD_HIDDEN ? width : n;
-    const i64 tiles_m = (rows + 63) / 64, tiles_n = (cols + 63) / 64;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for (i64 tile = blockIdx.x; tile < tiles_m * tiles_n; tile += gridDim.x) {
-        const i64 m0 = tile % tiles_m * 64, n0 = tile / tiles_m * 64;
-        float c[4][4] = {};
-        for (i64 k0 = 0; k0 < depth; k0 += 16) {
-            for (int x = threadIdx.x; x < 1024; x += 256) {
-                i64 m, k, j;
-                float u = 0.f, v = 0.f;
-                if (KIND == STATS || KIND == MAKE_G) {
-                    k = k0 + (x & 15), m = m0 + (x >> 4), j = n0 + (x >> 4);
-                    if (k < depth && m < rows) u = (float)packed[m * p.dim_padded + k];
-                    if (k < depth && v0 + j < p.vocab) v = (float)w[(v0 + j) * p.weight_rows_stride + k];
-                    a[x & 15][x >> 4] = u, b[x & 15][x >> 4] = v;
-                } else {
-                    if (KIND == GRAD_HIDDEN) {
-                        k = k0 + (x & 15), m = m0 + (x >> 4);
-                        if (k < depth && m < rows) u = (float)g[m * p.g_stride + k];
-                        a[x & 15][x >> 4] = u;
-                    } else {
-                        k = k0 + (x >> 6), m = m0 + (x & 63);
-                        if (k < depth && m < rows) u = (float)g[k * p.g_stride + m];
-                        a[x >> 6][x & 63] = u;
-                    }
-                    k = k0 + (x >> 6), j = n0 + (x & 63);
-                    if (k < depth && j < cols) {
-                        if (KIND == GRAD_WEIGHT) v = (float)packed[k * p.dim_padded + j];
-                        else if (v0 + k < p.vocab) v = (float)w[(v0 + k) * p.weight_rows_stride + j];
-                    }
-                    b[x >> 6][x & 63] = v;
-                }
-            }
-            __syncthreads();
-            for (int k = 0; k < 16; ++k)
-                for (int y = 0; y < 4; ++y)
-                    for (int x = 0; x < 4; ++x) c[y][x] += a[k][ty * 4 + y] * b[k][tx * 4 + x];
-            __syncthreads();
-        }
-        if (KIND == GRAD_HIDDEN || KIND == GRAD_WEIGHT) {
-            for (int y = 0; y < 4; ++y)
-                for (int x = 0; x < 4; ++x) {
-                    const i64 m = m0 + ty * 4 + y, j = n0 + tx * 4 + x;
-                    if (m >= rows || j >= cols) continue;
-                    if (KIND == GRAD_HIDDEN) {
-                        float *to = p.acc + m * p.dim + j;
-                        *to = first ? c[y][x] : *to + c[y][x];
-                    } else if (v0 + m < p.vocab) {
-                        ((T *)p.grad_weight)[(v0 + m) * p.dim + j] = T(c[y][x] * p.meta->out_scale);
-                    }
-                }
-            continue;
-        }
-        for (int y = 0; y < 4; ++y)
-            for (int x = 0; x < 4; ++x) z[ty * 4 + y][tx * 4 + x] = c[y][x];
-        __syncthreads();
-        if (threadIdx.x < 64) {
-            const int y = threadIdx.x;
-            const i64 m = m0 + y, row = p.row_of[m];
-            if (row < 0) {
-                if (KIND == MAKE_G)
-                    for (int x = 0; x < 64; ++x)
-                        if (n0 + x < p.g_stride) g[m * p.g_stride + n0 + x] = T(0.f);
-            } else {
-                const i64 k_all = p.k ? p.k : 1;
-                const int2 *e = p.entries + row * k_all;
-                i64 at = p.k ? p.first[row * p.pieces + (v0 + n0) / PIECE] : 0;
-                const float scale = p.inv_temperature * 1.4426950408889634f;
-                const float lse2 = KIND == MAKE_G ? p.lse2[row] : 0.f;
-                float top = LOWEST, sum = 0.f, pz = 0.f;
-                for (int x = 0; x < 64; ++x) {
-                    const i64 j = v0 + n0 + x;
-                    float v = z[y][x] * scale;
-                    float share = 0.f;
-                    while (at < k_all && e[at].x < j) ++at;
-                    while (at < k_all && e[at].x == j) share += __int_as_float(e[at].y), ++at;
-                    if (KIND == MAKE_G) {
-                        if (n0 + x < p.g_stride)
-                            g[m * p.g_stride + n0 + x] = T(j < p.vocab ? p.coef[m] * (exp2f(v - lse2) - share) : 0.f);
-                    } else if (j < p.vocab) {
-                        if (share != 0.f) pz += share * z[y][x];
-                        if (v > top) sum = sum * exp2f(top - v), top = v;
-                        sum += exp2f(v - top);
-                    }
-                }
-                if (KIND == STATS) {
-                    const i64 to = (v0 + n0) / PIECE * p.rows_padded + m;
-                    p.part_max[to] = top, p.part_sum[to] = sum, p.part_pz[to] = pz;
-                }
-            }
-        }
-        __syncthreads();
     }
 }
 
@@ -430,6 +327,7 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     p.dim_padded = up_to(a->dim, 8);
     p.rows_padded = up_to(p.rows > 0 ? p.rows : 1, TILE_ROWS);
     p.pieces = (int)((a->vocab + PIECE - 1) / PIECE);
+    p.parts = (int)((a->vocab + 64 * VL_GROUP - 1) / (64 * VL_GROUP));
     p.k_sorted = 2;
     while (p.k_sorted < a->k) p.k_sorted *= 2;
     p.temperature = a->temperature, p.inv_temperature = 1.f / a->temperature;
@@ -451,6 +349,8 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     if (width > most) width = most > 2048 ? most : (width < 2048 ? width : 2048);
     p.g_stride = width;
     p.splits = 1;
+    p.acc_stride = up_to(a->dim, 32);
+    p.grad_weight_aligned = (uintptr_t)a->grad_weight % 16 == 0 && a->dim % 8 == 0;
     bytes = 0;
     char *base = (char *)a->workspace;
     auto take = [&](i64 n) {
@@ -470,38 +370,96 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     p.packed = take(p.rows_padded * p.dim_padded * 2);
     p.weight_rows = aligned ? a->weight : take(p.vocab * p.dim_padded * 2);
     if (p.want_loss) {
-        p.part_max = (float *)take(p.rows_padded * 4 * p.pieces);
-        p.part_sum = (float *)take(p.rows_padded * 4 * p.pieces);
-        p.part_pz = (float *)take(p.rows_padded * 4 * p.pieces);
+        p.part_max = (float *)take(p.rows_padded * 4 * p.parts);
+        p.part_sum = (float *)take(p.rows_padded * 4 * p.parts);
+        p.part_pz = (float *)take(p.rows_padded * 4 * p.parts);
         p.row_loss = a->reduction == STBPE_REDUCE_NONE ? a->loss : (float *)take(p.rows_padded * 4);
     }
     if (p.want_grads) {
         p.coef = (float *)take(p.rows_padded * 4);
         p.g = take(p.rows_padded * p.g_stride * 2);
-        if (p.grad_hidden) p.acc = (float *)take((i64)p.splits * p.rows_padded * p.dim * 4);
+        if (p.grad_hidden) p.acc = (float *)take((i64)p.splits * p.rows_padded * p.acc_stride * 4);
     }
     return STBPE_OK;
 }
 
-template <class T>
-int run(const Plan &p, cudaStream_t s, char *err, size_t err_len) {
-    const int wide = 148 * 8;
+// A matrix of 16-bit numbers for TMA: boxes of 64 columns (128 bytes, swizzled) by `box` rows, zeros outside.
+int tensor_map(CUtensorMap *map, int type, const void *at, i64 rows, i64 cols, i64 stride, int box, char *err, size_t err_len) {
+    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                               const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static Encode encode = nullptr;
+    if (!encode) {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        VCK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q));
+        if (q != cudaDriverEntryPointSuccess || !f) return fail(err, err_len, STBPE_E_CUDA, "cuTensorMapEncodeTiled", "not found");
+        encode = (Encode)f;
+    }
+    const cuuint64_t size[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, pitch[1] = {(cuuint64_t)stride * 2};
+    const cuuint32_t tile[2] = {64, (cuuint32_t)box}, one[2] = {1, 1};
+    const CUresult r = encode(map, type == STBPE_REAL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                              const_cast<void *>(at), size, pitch, tile, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? STBPE_OK : fail(err, err_len, STBPE_E_CUDA, "cuTensorMapEncodeTiled", "refused");
+}
+
+constexpr int SMS = 148;
+
+template <class T, int KIND, int GROUP>
+int launch(const Plan &p, const Job &job, const CUtensorMap &a, const CUtensorMap &b, cudaStream_t s, char *err, size_t err_len) {
+    const i64 tile = 128 * GROUP;
+    const i64 rows = KIND == GRAD_WEIGHT ? job.width : p.rows, cols = KIND <= MAKE_G ? job.width : p.dim;
+    const i64 tiles = ((rows + tile - 1) / tile) * ((cols + tile - 1) / tile);
+    if (tiles == 0) return STBPE_OK;
+    auto *kernel = product_kernel<T, KIND, GROUP>;
+    VCK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PRODUCT_SMEM));
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((unsigned)(tiles < SMS / GROUP ? tiles : SMS / GROUP) * GROUP);
+    c.blockDim = dim3(PRODUCT_THREADS);
+    c.dynamicSmemBytes = PRODUCT_SMEM;
+    c.stream = s;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim = {GROUP, 1, 1};
+    c.attrs = &cluster, c.numAttrs = 1;
+    VCK(cudaLaunchKernelEx(&c, kernel, p, job, a, b));
+    return STBPE_OK;
+}
+
+#define VTRY(call)                        \
+    do {                                  \
+        const int st_ = (call);           \
+        if (st_ != STBPE_OK) return st_;  \
+    } while (0)
+
+template <class T, int GROUP>
+int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
+    const int wide = SMS * 8;
     auto blocks = [&](i64 n, i64 per) { return (unsigned)(n <= 0 ? 1 : (n + per - 1) / per < wide ? (n + per - 1) / per : wide); };
     if (p.k) teacher_kernel<<<blocks(p.rows, 4), 128, 4 * p.k_sorted * sizeof(u64), s>>>(p);
     rows_kernel<<<1, 1024, 0, s>>>(p);
     gather_kernel<T><<<blocks(p.rows_padded, 8), 256, 0, s>>>(p);
     if (p.weight_rows != p.weight) align_weight_kernel<T><<<blocks(p.vocab, 8), 256, 0, s>>>(p, (T *)p.weight_rows);
+    CUtensorMap h, w;
+    VTRY(tensor_map(&h, type, p.packed, p.rows_padded, p.dim, p.dim_padded, 128, err, err_len));
+    VTRY(tensor_map(&w, type, p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 128, err, err_len));
     if (p.want_loss) {
-        product_kernel<T, STATS><<<wide, 256, 0, s>>>(p, 0, p.vocab, 0);
+        VTRY((launch<T, STATS, GROUP>(p, Job{0, p.vocab, 0}, h, w, s, err, err_len)));
         join_kernel<<<blocks(p.rows, 8), 256, 0, s>>>(p);
     }
     if (p.want_grads || p.reduction != STBPE_REDUCE_NONE) finish_kernel<<<1, 1024, 0, s>>>(p);
     if (p.want_grads) {
+        CUtensorMap h_across, w_across, g, g_across;
+        VTRY(tensor_map(&h_across, type, p.packed, p.rows_padded, p.dim, p.dim_padded, 64, err, err_len));
+        VTRY(tensor_map(&w_across, type, p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 64, err, err_len));
+        VTRY(tensor_map(&g, type, p.g, p.rows_padded, p.g_stride, p.g_stride, 128, err, err_len));
+        VTRY(tensor_map(&g_across, type, p.g, p.rows_padded, p.g_stride, p.g_stride, 64, err, err_len));
         for (i64 v0 = 0; v0 < p.vocab; v0 += p.g_stride) {
-            const i64 width = p.vocab - v0 < p.g_stride ? p.vocab - v0 : p.g_stride;
-            product_kernel<T, MAKE_G><<<wide, 256, 0, s>>>(p, v0, width, 0);
-            if (p.grad_hidden) product_kernel<T, GRAD_HIDDEN><<<wide, 256, 0, s>>>(p, v0, width, v0 == 0);
-            if (p.grad_weight) product_kernel<T, GRAD_WEIGHT><<<wide, 256, 0, s>>>(p, v0, width, 0);
+            const Job job{v0, p.vocab - v0 < p.g_stride ? p.vocab - v0 : p.g_stride, v0 == 0};
+            VTRY((launch<T, MAKE_G, GROUP>(p, job, h, w, s, err, err_len)));
+            if (p.grad_hidden) VTRY((launch<T, GRAD_HIDDEN, GROUP>(p, job, g, w_across, s, err, err_len)));
+            if (p.grad_weight) VTRY((launch<T, GRAD_WEIGHT, GROUP>(p, job, g_across, h_across, s, err, err_len)));
         }
         if (p.grad_hidden) scatter_kernel<T><<<blocks(p.rows * p.dim, 256), 256, 0, s>>>(p);
     }
@@ -534,8 +492,8 @@ STBPE_VISIBLE int stbpe_vocab_loss_run(const stbpe_vocab_loss *args, void *strea
         return fail(err, err_len, STBPE_E_BADARG, "stbpe_vocab_loss", "an output is missing");
     if (!args->weight || (p.rows && (!args->hidden || !args->ids || (p.k && !args->logits))))
         return fail(err, err_len, STBPE_E_BADARG, "stbpe_vocab_loss", "an input is missing");
-    return args->type == STBPE_REAL_BF16 ? run<__nv_bfloat16>(p, (cudaStream_t)stream, err, err_len)
-                                         : run<__half>(p, (cudaStream_t)stream, err, err_len);
+    return args->type == STBPE_REAL_BF16 ? run<__nv_bfloat16, VL_GROUP>(p, args->type, (cudaStream_t)stream, err, err_len)
+                                         : run<__half, VL_GROUP>(p, args->type, (cudaStream_t)stream, err, err_len);
 }
 
 }  // extern "C"

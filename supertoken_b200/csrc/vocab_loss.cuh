@@ -8,7 +8,7 @@ namespace vloss {
 typedef unsigned long long u64;
 typedef long long i64;
 
-constexpr int PIECE = 64;       // columns whose statistics one thread keeps for its row
+constexpr int PIECE = 256;      // columns per step of the table that finds a row's entries
 constexpr int TILE_ROWS = 256;  // the packed rows end on this boundary
 
 // the running maximum starts at a finite value: a logit of -inf then adds 0 to the sum, and one of NaN or +inf makes it NaN
@@ -23,8 +23,8 @@ struct Meta {
 struct Plan {
     i64 rows, inner;  // row = outer * inner + inner index
     i64 vocab, dim, dim_padded, rows_padded;
-    int k, k_sorted, pieces, reduction, splits;
-    bool want_loss, want_grads, hidden_aligned;
+    int k, k_sorted, pieces, parts, reduction, splits;
+    bool want_loss, want_grads, hidden_aligned, grad_weight_aligned;
     float temperature, inv_temperature;
     const void *hidden, *weight, *ids, *logits;
     const unsigned char *valid;
@@ -45,11 +45,12 @@ struct Plan {
     void *packed;            // counted rows of hidden, one behind another
     const void *weight_rows; // weight, or its copy with rows on 16-byte boundaries
     i64 weight_rows_stride;
-    float *part_max, *part_sum, *part_pz, *row_loss;  // [piece][packed row]; per row
+    float *part_max, *part_sum, *part_pz, *row_loss;  // [part][packed row]; per row
     float *coef;             // what a packed row of G is multiplied by
     void *g;                 // G of one piece of the vocabulary, [packed row][g_stride]
     i64 g_stride;
-    float *acc;              // dH of packed rows in 32 bits, [split][packed row][dim]
+    float *acc;              // dH of packed rows in 32 bits, [split][packed row][acc_stride]
+    i64 acc_stride;
 };
 
 }  // namespace vloss

@@ -1,0 +1,457 @@
+// The products of the losses over a large vocabulary on the tensor cores: tcgen05 with its operands in shared memory, filled by
+// TMA, and its sums (32 bits) in TMEM.
+//
+//   STATS        Z = H W^T of the whole vocabulary; per row and piece of columns the maximum, the sum of exp and sum p z
+//   MAKE_G       Z again, of one piece of the vocabulary, and G from it in 16 bits
+//   GRAD_HIDDEN  dH += G W      (k over the piece's columns: W is read with the other dimension contiguous)
+//   GRAD_WEIGHT  dW = G^T H     (k over the rows: both are read with the other dimension contiguous)
+//
+// A group of GROUP CTAs makes a tile of 128 GROUP x 128 GROUP: with GROUP = 2 the two CTAs of a cluster share one
+// 256 x 256 tile (cta_group::2), each holding its half of both operands, so that a byte brought into shared memory serves twice as
+// many products.  A CTA loads 128 x 64 of each operand per step in either case.  Persistent: the tiles are dealt out
+// to the clusters in turn, and the sums of one tile are looked at while the next one is being made (two buffers in TMEM).
+// Warp 0 loads, warp 1 of the group's first CTA multiplies, warp 2 owns the TMEM, warps 4 to 11 take the sums.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "vocab_loss.cuh"
+
+namespace vloss {
+
+enum { STATS, MAKE_G, GRAD_HIDDEN, GRAD_WEIGHT };
+
+constexpr int STAGES = 6;
+constexpr int OPERAND_BYTES = 128 * 64 * 2;  // what a CTA loads of one operand per step of 64 terms
+constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
+constexpr int PRODUCT_THREADS = 384;
+constexpr int PRODUCT_SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+
+struct Job {
+    i64 v0, width;   // the piece of the vocabulary
+    int first;       // GRAD_HIDDEN: nothing to add to
+};
+
+// ---------------------------------------------------------------------------------------------- instructions
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+
+__device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void barrier_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Every wait ends: after two seconds the error is recorded, and all roles leave their loops as they meet it.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, unsigned int *error) {
+    uint32_t done;
+    u64 began = 0;
+    for (;;) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+        u64 now;
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+        if (!began) began = now;
+        if (now - began > 2000000000ull) {
+            atomicOr(error, 1u);
+            return false;
+        }
+    }
+}
+
+template <int GROUP>
+__device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    if (GROUP == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(map),
+            "r"(x), "r"(y), "r"(bar)
+            : "memory");
+}
+
+template <int GROUP>
+__device__ __forceinline__ void mma(uint32_t tmem, u64 a, u64 b, uint32_t what, uint32_t add) {
+    if (GROUP == 2)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+                     "l"(a), "l"(b), "r"(what), "r"(add)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+                     "l"(a), "l"(b), "r"(what), "r"(add)
+                     : "memory");
+}
+
+// arrives at the barrier (of both CTAs of a pair) when the products issued so far are done
+template <int GROUP>
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    if (GROUP == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                     "h"((unsigned short)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at)
+        : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// Descriptor of an operand in shared memory, 128-byte swizzle.  Contiguous along k: rows of 128 bytes, eight rows to the
+// next at 1024 (the other offset is unused).  Contiguous along the other dimension: slabs of 64 of them by 64 k, eight k to
+// the next at 1024, the next slab at 8192.
+template <bool ALONG_K>
+__device__ __forceinline__ u64 operand(uint32_t addr) {
+    const u64 leading = ALONG_K ? 1 : 8192 >> 4, stride = 1024 >> 4;
+    return (u64)((addr & 0x3FFFF) >> 4) | leading << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *(uint32_t *)&v;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    __half2 v = __floats2half2_rn(a, b);
+    return *(uint32_t *)&v;
+}
+
+// 32 values of one row, 16 bits each; `inside`: how many of them there are
+template <class T>
+__device__ __forceinline__ void store_row(T *to, const float (&v)[32], i64 inside, bool aligned) {
+    if (aligned && inside >= 32) {
+#pragma unroll
+        for (int x = 0; x < 32; x += 8)
+            *(uint4 *)(to + x) = make_uint4(pack2<T>(v[x], v[x + 1]), pack2<T>(v[x + 2], v[x + 3]), pack2<T>(v[x + 4], v[x + 5]),
+                                            pack2<T>(v[x + 6], v[x + 7]));
+    } else {
+#pragma unroll
+        for (int x = 0; x < 32; ++x)
+            if (x < inside) to[x] = T(v[x]);
+    }
+}
+
+// The entries of one row in ascending order: what falls into each 32 columns.
+struct Walk {
+    const int2 *entries;
+    int at, all;
+    int2 next;
+
+    __device__ __forceinline__ void start(const Plan &p, i64 row, i64 column) {
+        all = p.k ? p.k : 1;
+        entries = p.entries + row * all;
+        at = p.k ? p.first[row * p.pieces + column / PIECE] : 0;
+        next = at < all ? entries[at] : make_int2(INT_MAX, 0);
+        while (next.x < column) advance();
+    }
+    __device__ __forceinline__ void advance() {
+        ++at;
+        next = at < all ? entries[at] : make_int2(INT_MAX, 0);
+    }
+};
+
+// ---------------------------------------------------------------------------------------------- the kernel
+template <class T, int KIND, int GROUP>
+__global__ void __launch_bounds__(PRODUCT_THREADS, 1)
+    product_kernel(const __grid_constant__ Plan p, const __grid_constant__ Job job, const __grid_constant__ CUtensorMap map_a,
+                   const __grid_constant__ CUtensorMap map_b) {
+    constexpr bool LOGITS = KIND == STATS || KIND == MAKE_G;
+    constexpr bool A_ALONG_K = KIND != GRAD_WEIGHT, B_ALONG_K = LOGITS;
+    constexpr u64 A_NEXT = (A_ALONG_K ? 32 : 2048) >> 4, B_NEXT = (B_ALONG_K ? 32 : 2048) >> 4;  // 16 k further, for the descriptors
+    constexpr int TILE = 128 * GROUP, COLUMNS = TILE / 2;  // columns that one epilogue thread takes of its row
+    constexpr uint32_t WHAT = 1u << 4 | (std::is_same<T, __nv_bfloat16>::value ? 1u << 7 | 1u << 10 : 0u) |
+                              (A_ALONG_K ? 0u : 1u << 15) | (B_ALONG_K ? 0u : 1u << 16) | (uint32_t)(TILE >> 3) << 17 |
+                              (uint32_t)(TILE >> 4) << 24;
+    extern __shared__ char raw[];
+    const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
+    const uint32_t bars = base + STAGES * STAGE_BYTES;
+    const uint32_t full = bars, empty = bars + 8 * STAGES, sums_full = bars + 16 * STAGES, sums_empty = sums_full + 16,
+                   drained = sums_full + 32, tmem_at = sums_full + 40;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t rank = 0;
+    if (GROUP == 2) asm("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
+    unsigned int *error = &p.meta->error;
+
+    if (warp == 0 && lane == 0) {
+        for (int s = 0; s < STAGES; ++s) barrier_init(full + 8 * s, 1), barrier_init(empty + 8 * s, 1);
+        for (int b = 0; b < 2; ++b) barrier_init(sums_full + 8 * b, 1), barrier_init(sums_empty + 8 * b, 8 * GROUP);
+        barrier_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+    }
+    if (warp == 2) {
+        if (GROUP == 2)
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_at), "r"(2 * TILE) : "memory");
+        else
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_at), "r"(2 * TILE) : "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    __syncthreads();
+    if (GROUP == 2) cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    uint32_t tmem;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
+
+    // the tiles and their depth
+    const i64 n = p.meta->counted;
+    const i64 rows = KIND == GRAD_WEIGHT ? job.width : n, cols = LOGITS ? job.width : p.dim;
+    const i64 depth = LOGITS ? p.dim : KIND == GRAD_HIDDEN ? job.width : n;
+    const i64 tiles_m = (rows + TILE - 1) / TILE, tiles_n = (cols + TILE - 1) / TILE;
+    const int steps = (int)((depth + 63) / 64);
+    const i64 tiles = tiles_m * tiles_n;
+    const i64 cluster = blockIdx.x / GROUP, clusters = gridDim.x / GROUP;
+    // a band of BAND tiles of rows goes through all columns, its rows first: that much of A stays in L2
+    constexpr i64 BAND = 16;
+    auto place = [&](i64 tile, i64 &m0, i64 &n0) {
+        const i64 band = tile / (BAND * tiles_n), in = tile - band * BAND * tiles_n;
+        const i64 high = tiles_m - band * BAND < BAND ? tiles_m - band * BAND : BAND;
+        n0 = in / high * TILE;
+        m0 = (band * BAND + in % high) * TILE;
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t phase = 0;
+            i64 issued = 0;
+            bool alive = true;
+            for (i64 tile = cluster; tile < tiles && alive; tile += clusters) {
+                i64 m0, n0;
+                place(tile, m0, n0);
+                const int am = (int)(m0 + rank * 128), bn = (int)(n0 + rank * 128);
+                for (int k = 0; k < steps; ++k) {
+                    if (!barrier_wait(empty + 8 * s, phase ^ 1, error)) {
+                        alive = false;
+                        break;
+                    }
+                    const uint32_t a = base + s * STAGE_BYTES, b = a + OPERAND_BYTES;
+                    const uint32_t bar = GROUP == 2 ? in_cta(full + 8 * s, 0) : full + 8 * s;
+                    if (rank == 0) barrier_expect(full + 8 * s, GROUP * STAGE_BYTES);
+                    if (A_ALONG_K) {
+                        tma_load<GROUP>(a, &map_a, k * 64, am, bar);
+                    } else {
+                        tma_load<GROUP>(a, &map_a, am, k * 64, bar);
+                        tma_load<GROUP>(a + 8192, &map_a, am + 64, k * 64, bar);
+                    }
+                    if (LOGITS) {
+                        tma_load<GROUP>(b, &map_b, k * 64, (int)job.v0 + bn, bar);
+                    } else {
+                        const int row = (KIND == GRAD_HIDDEN ? (int)job.v0 : 0) + k * 64;
+                        tma_load<GROUP>(b, &map_b, bn, row, bar);
+                        tma_load<GROUP>(b + 8192, &map_b, bn + 64, row, bar);
+                    }
+                    ++issued;
+                    if (++s == STAGES) s = 0, phase ^= 1;
+                }
+            }
+            if (!alive && rank == 0) {  // copies in flight land before the memory is given up
+                const i64 pending = issued < STAGES ? issued : STAGES;
+                for (i64 x = issued - pending; x < issued; ++x)
+                    barrier_wait(full + 8 * (int)(x % STAGES), (uint32_t)(x / STAGES & 1), error);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            int s = 0, buffer = 0;
+            uint32_t phase = 0, sums_phase = 0;
+            bool alive = true;
+            for (i64 tile = cluster; tile < tiles && alive; tile += clusters) {
+                if (!barrier_wait(sums_empty + 8 * buffer, sums_phase ^ 1, error)) {
+                    alive = false;
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t d = tmem + buffer * TILE;
+                for (int k = 0; k < steps; ++k) {
+                    if (!barrier_wait(full + 8 * s, phase, error)) {
+                        alive = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const u64 a = operand<A_ALONG_K>(base + s * STAGE_BYTES), b = operand<B_ALONG_K>(base + s * STAGE_BYTES + OPERAND_BYTES);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        mma<GROUP>(d, a + x * A_NEXT, b + x * B_NEXT, WHAT, k > 0 || x > 0);
+                    mma_commit<GROUP>(empty + 8 * s);
+                    if (++s == STAGES) s = 0, phase ^= 1;
+                }
+                if (alive) mma_commit<GROUP>(sums_full + 8 * buffer);
+                buffer ^= 1;
+                if (buffer == 0) sums_phase ^= 1;
+            }
+            if (!alive) {  // products in flight end before the TMEM is given up
+                mma_commit<GROUP>(drained);
+                barrier_wait(drained, 0, error);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        int buffer = 0;
+        uint32_t sums_phase = 0;
+        for (i64 tile = cluster; tile < tiles; tile += clusters) {
+            i64 m0, n0;
+            place(tile, m0, n0);
+            const i64 m = m0 + rank * 128 + quarter * 32 + lane;  // this thread's row of the result
+            const i64 c0 = n0 + half * COLUMNS;                   // and its first column
+            i64 row = -1;
+            float lse2 = 0.f, coef = 0.f, top = LOWEST, sum = 0.f, pz = 0.f;
+            const float scale = p.inv_temperature * 1.4426950408889634f;
+            Walk walk;
+            if (LOGITS) {
+                row = m < p.rows_padded ? p.row_of[m] : -1;
+                if (row >= 0 && job.v0 + c0 < p.vocab) walk.start(p, row, job.v0 + c0);
+                else walk.next.x = INT_MAX, walk.at = walk.all = 0;
+                if (KIND == MAKE_G && row >= 0) lse2 = p.lse2[row], coef = p.coef[m];
+            }
+            const float out_scale = KIND == GRAD_WEIGHT ? p.meta->out_scale : 1.f;
+            if (!__all_sync(~0u, barrier_wait(sums_full + 8 * buffer, sums_phase, error))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t from = tmem + buffer * TILE + half * COLUMNS + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+            for (int c = 0; c < COLUMNS; c += 32) {
+                uint32_t bits[32];
+                __syncwarp();
+                tmem_load(from + c, bits);
+                if (c + 32 == COLUMNS) {  // the buffer is free
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) barrier_arrive_cluster(GROUP == 2 ? in_cta(sums_empty + 8 * buffer, 0) : sums_empty + 8 * buffer);
+                }
+                float v[32];
+#pragma unroll
+                for (int x = 0; x < 32; ++x) v[x] = steps ? __uint_as_float(bits[x]) : 0.f;  // (no rows: nothing was summed)
+                const i64 j = job.v0 + c0 + c;  // first column, as a token id (LOGITS)
+                if (KIND == STATS) {
+                    while (walk.next.x < j + 32) {
+                        const int x0 = walk.next.x - (int)j;
+                        float z = 0.f;
+#pragma unroll
+                        for (int x = 0; x < 32; ++x)
+                            if (x == x0) z = v[x];
+                        pz += __int_as_float(walk.next.y) * z;
+                        walk.advance();
+                    }
+                    if (j + 32 > p.vocab) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x)
+                            if (j + x >= p.vocab) v[x] = -INFINITY;
+                    }
+                    float most = v[0];
+#pragma unroll
+                    for (int x = 1; x < 32; ++x) most = fmaxf(most, v[x]);
+                    const float now = fmaxf(top, most * scale);
+                    sum *= exp2_fast(top - now);
+                    top = now;
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) sum += exp2_fast(fmaf(v[x], scale, -now));
+                }
+                if (KIND == MAKE_G) {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) v[x] = exp2_fast(fmaf(v[x], scale, -lse2));
+                    while (walk.next.x < j + 32) {
+                        const int x0 = walk.next.x - (int)j;
+#pragma unroll
+                        for (int x = 0; x < 32; ++x)
+                            if (x == x0) v[x] -= __int_as_float(walk.next.y);
+                        walk.advance();
+                    }
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) v[x] = row >= 0 && j + x < p.vocab ? v[x] * coef : 0.f;
+                    if (m < p.rows_padded && c0 + c < p.g_stride) store_row((T *)p.g + m * p.g_stride + c0 + c, v, 32, true);
+                }
+                if (KIND == GRAD_HIDDEN) {
+                    if (m < n && c0 + c < p.acc_stride) {
+                        float4 *to = (float4 *)(p.acc + m * p.acc_stride + c0 + c);
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            float4 y = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+                            if (!job.first) {
+                                const float4 z = to[x];
+                                y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+                            }
+                            to[x] = y;
+                        }
+                    }
+                }
+                if (KIND == GRAD_WEIGHT) {
+                    const i64 id = job.v0 + m;
+                    if (m < job.width && c0 + c < p.dim) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) v[x] *= out_scale;
+                        store_row((T *)p.grad_weight + id * p.dim + c0 + c, v, p.dim - c0 - c, p.grad_weight_aligned);
+                    }
+                }
+            }
+            if (KIND == STATS && row >= 0 && job.v0 + c0 < p.vocab) {
+                const i64 to = (job.v0 + c0) / COLUMNS * p.rows_padded + m;
+                p.part_max[to] = top, p.part_sum[to] = sum, p.part_pz[to] = pz;
+            }
+            buffer ^= 1;
+            if (buffer == 0) sums_phase ^= 1;
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (GROUP == 2) cluster_sync();  // the other CTA may still arrive at this one's barriers
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 2) {
+        if (GROUP == 2) {
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TILE));
+        } else {
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TILE));
+        }
+    }
+}
+
+}  // namespace vloss
