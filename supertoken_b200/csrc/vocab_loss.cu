@@ -4,8 +4,14 @@
 //   z_ij = h_i . w_j              lse_i = log sum_j exp(s z_ij)
 //   loss_i = T^2 (lse_i + sum_k p_ik (log p_ik - s z_i,t_ik))
 //   G_ij = g_i T (exp(s z_ij - lse_i) - sum_k p_ik [j = t_ik])       dH = G W        dW = G^T H
-// z is never stored: the forward product keeps (maximum, sum, sum_k p z) of each row and piece of columns, the
-// backward one makes G for a piece of the vocabulary at a time, from which both gradients take their share.
+// The N x V logits are never stored.  Two ways to the gradients:
+//   keep    (loss and gradients at once, bf16): E_ij = exp2(s' z_ij - c_i) goes to memory in 16 bits for at most 1 GiB of rows at a time, with
+//           a reference c_i known before the product, and the sums that make lse_i of it beside it.  Then with
+//           a_i = g_i T exp2(c_i - lse2_i): E - p / exp2(c_i - lse2_i) at the entries, from z in 32 bits, dH = a (E W), dW = E^T (a H).
+//           Three products.  c_i is 0; a row whose largest logit lies further than 2^96 from it gets that as its reference and its
+//           tile is made again, which no model's logits below 66 in size ever need.  fp16 has not the range for it.
+//   anew    (fp16, or gradients after the loss): z is made a second time, and G from it for up to 1 GiB of the vocabulary
+//           at a time.  Four products, or three behind a loss.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -17,10 +23,6 @@
 #include "vocab_products.cuh"
 
 #define STBPE_VISIBLE __attribute__((visibility("default")))
-
-#ifndef VL_GROUP
-#define VL_GROUP 2
-#endif
 
 namespace {
 using namespace vloss;
@@ -118,67 +120,141 @@ __global__ void __launch_bounds__(128) teacher_kernel(Plan p) {
     }
 }
 
-// One CTA: which rows count, in their order (row_of, slot_of); the entry of a cross entropy row.
+// One CTA: which rows count, in their order (row_of, slot_of); the entry of a cross entropy row; what each counted row's dlogits are
+// multiplied by.  dlogits are held in the inputs' 16-bit type, so they are brought into that type's range: the largest |g_i T|
+// becomes up to 2^14 (by a power of two, so bf16 loses nothing; fp16 keeps shares down to 2^-28 at full precision and its
+// entries stay below 2^15), and both gradients are scaled back in 32 bits.
 __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
-    __shared__ int in_warp[32];
+    constexpr int EACH = 8;  // rows of a thread, 1024 apart: their loads are in flight together
+    __shared__ int in_warp[EACH * 32];
     __shared__ int base;
+    __shared__ float part[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) base = 0;
-    __syncthreads();
-    for (i64 r0 = 0; r0 < p.rows; r0 += 1024) {
-        const i64 row = r0 + threadIdx.x;
-        bool counted = false;
-        if (row < p.rows) {
-            const i64 o = row / p.inner, i = row - o * p.inner;
-            counted = !p.valid || p.valid[o * p.valid_outer + i * p.valid_inner];
-            if (p.k) {
-                counted = counted && p.has_entries[row];
-            } else {
-                const i64 id = load_id(p.ids, p.ids_bytes, o * p.ids_outer + i * p.ids_inner);
-                counted = counted && id >= 0;
-                const bool outside = id >= p.vocab;
-                p.entries[row] = make_int2(outside || id < 0 ? INT_MAX : (int)id, __float_as_int(1.f));
-                p.plogp[row] = outside ? NAN : 0.f;
+    if (p.split_done)
+        for (int x = threadIdx.x; x < SMS * 8; x += 1024) p.split_done[x] = 0;
+    for (i64 r0 = 0; r0 < p.rows; r0 += EACH * 1024) {
+        bool counted[EACH];
+        unsigned votes[EACH];
+#pragma unroll
+        for (int x = 0; x < EACH; ++x) {
+            const i64 row = r0 + x * 1024 + threadIdx.x;
+            counted[x] = false;
+            if (row < p.rows) {
+                const i64 o = row / p.inner, i = row - o * p.inner;
+                counted[x] = !p.valid || p.valid[o * p.valid_outer + i * p.valid_inner];
+                if (p.k) {
+                    counted[x] = counted[x] && p.has_entries[row];
+                } else {
+                    const i64 id = load_id(p.ids, p.ids_bytes, o * p.ids_outer + i * p.ids_inner);
+                    counted[x] = counted[x] && id >= 0;
+                    const bool outside = id >= p.vocab;
+                    p.entries[row] = make_int2(outside || id < 0 ? INT_MAX : (int)id, __float_as_int(1.f));
+                    p.plogp[row] = outside ? NAN : 0.f;
+                }
             }
         }
-        const unsigned votes = __ballot_sync(~0u, counted);
-        if (lane == 0) in_warp[warp] = __popc(votes);
         __syncthreads();
-        int before = base, all = 0;
-        for (int w = 0; w < 32; ++w) {
-            before += w < warp ? in_warp[w] : 0;
-            all += in_warp[w];
+#pragma unroll
+        for (int x = 0; x < EACH; ++x) {
+            votes[x] = __ballot_sync(~0u, counted[x]);
+            if (lane == 0) in_warp[x * 32 + warp] = __popc(votes[x]);
         }
-        const int slot = before + __popc(votes & ((1u << lane) - 1));
-        if (row < p.rows) p.slot_of[row] = counted ? slot : -1;
-        if (counted) p.row_of[slot] = (int)row;
         __syncthreads();
-        if (threadIdx.x == 0) base += all;
+        if (warp == 0) {  // counts to places
+            int mine = 0;
+#pragma unroll
+            for (int x = 0; x < EACH; ++x) mine += in_warp[lane * EACH + x];
+            int upto = mine;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int y = __shfl_up_sync(~0u, upto, d);
+                if (lane >= d) upto += y;
+            }
+            int at = base + upto - mine;
+            __syncwarp();
+#pragma unroll
+            for (int x = 0; x < EACH; ++x) {
+                const int y = in_warp[lane * EACH + x];
+                in_warp[lane * EACH + x] = at;
+                at += y;
+            }
+            if (lane == 31) base = at;
+        }
         __syncthreads();
+#pragma unroll
+        for (int x = 0; x < EACH; ++x) {
+            const i64 row = r0 + x * 1024 + threadIdx.x;
+            const int slot = in_warp[x * 32 + warp] + __popc(votes[x] & ((1u << lane) - 1));
+            if (row < p.rows) {
+                p.slot_of[row] = counted[x] ? slot : -1;
+                if (counted[x]) p.row_of[slot] = (int)row;
+                else if (p.want_loss) p.row_loss[row] = p.lse2[row] = 0.f;
+            }
+        }
     }
+    __syncthreads();
     const int n = base;
     for (i64 c = n + threadIdx.x; c < p.rows_padded; c += 1024) p.row_of[c] = -1;
-    if (threadIdx.x == 0) p.meta->counted = n, p.meta->error = 0;
+    if (p.keep) {
+        for (i64 c = threadIdx.x; c < p.rows_padded; c += 1024) p.reference[c] = 0.f;
+        for (i64 c = threadIdx.x; c < p.rows_padded / TILE_ROWS; c += 1024) p.again[c] = 0;
+    }
+    if (threadIdx.x == 0) p.meta->counted = n, p.meta->tickets = 0;
+    if (!p.want_grads) return;
+    const float factor = p.temperature / (p.reduction == STBPE_REDUCE_MEAN ? (float)(n > 0 ? n : 1) : 1.f);
+    const bool each = p.reduction == STBPE_REDUCE_NONE && p.grad_loss;
+    auto g = [&](i64 row) {
+        const i64 o = row / p.inner, i = row - o * p.inner;
+        return (!p.grad_loss ? 1.f : p.grad_loss[each ? o * p.grad_outer + i * p.grad_inner : 0]) * factor;
+    };
+    float most = fabsf(g(0) * (p.rows > 0));
+    if (each) {
+        most = 0.f;
+        for (i64 c = threadIdx.x; c < n; c += 1024) most = fmaxf(most, fabsf(g(p.row_of[c])));
+        for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+        if (lane == 0) part[warp] = most;
+        __syncthreads();
+        for (int w = 0; w < 32; ++w) most = fmaxf(most, part[w]);
+    }
+    int up = 0;  // the next power of two, both sides kept within what 32 bits hold as normal numbers
+    if (most > 0.f && most < INFINITY) frexpf(most, &up);
+    up = max(-100, min(100, up));
+    const float in = ldexpf(1.f, 14 - up);
+    if (threadIdx.x == 0) p.meta->out_scale = ldexpf(1.f, up - 14);
+    for (i64 c = threadIdx.x; c < n; c += 1024) {
+        const int row = p.row_of[c];
+        p.coef[c] = isnan(p.plogp[row]) ? NAN : g(row) * in;
+    }
 }
 
 // Counted rows of `hidden` one behind another, zeros up to the end of the last tile: products then do no work for
-// padding, never multiply what a masked row holds (it may be NaN), and may read rows of any stride or alignment.
+// padding, never multiply what a masked row holds (it may be NaN), and may read rows of any stride or alignment.  The rows of dH that do
+// not count get their zeros here.
 template <class T>
 __global__ void __launch_bounds__(256) gather_kernel(Plan p) {
     const int lane = threadIdx.x & 31;
     const i64 n = p.meta->counted, until = (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS;
-    for (i64 c = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); c < until; c += (i64)gridDim.x * 8) {
-        T *to = (T *)p.packed + c * p.dim_padded;
-        if (c >= n) {
+    for (i64 x = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); x < p.rows + until - n; x += (i64)gridDim.x * 8) {
+        const i64 slot = x < p.rows ? p.slot_of[x] : n + x - p.rows;
+        T *to = (T *)p.packed + slot * p.dim_padded;
+        if (x >= p.rows) {
             for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)(to + d) = make_uint4(0, 0, 0, 0);
-            continue;
-        }
-        const i64 row = p.row_of[c], o = row / p.inner, i = row - o * p.inner;
-        const T *from = (const T *)p.hidden + o * p.hidden_outer + i * p.hidden_inner;
-        if (p.hidden_aligned) {
-            for (int d = lane * 8; d < p.dim; d += 256) *(uint4 *)(to + d) = *(const uint4 *)(from + d);
+        } else if (slot < 0) {
+            if (!p.grad_hidden) continue;
+            to = (T *)p.grad_hidden + x * p.dim;
+            if (p.dim % 8 == 0)
+                for (int d = lane * 8; d < p.dim; d += 256) *(uint4 *)(to + d) = make_uint4(0, 0, 0, 0);
+            else
+                for (int d = lane; d < p.dim; d += 32) to[d] = T(0.f);
         } else {
-            for (int d = lane; d < p.dim_padded; d += 32) to[d] = d < p.dim ? from[d] : T(0.f);
+            const i64 o = x / p.inner, i = x - o * p.inner;
+            const T *from = (const T *)p.hidden + o * p.hidden_outer + i * p.hidden_inner;
+            if (p.hidden_aligned)
+#pragma unroll 4
+                for (int d = lane * 8; d < p.dim; d += 256) *(uint4 *)(to + d) = *(const uint4 *)(from + d);
+            else
+#pragma unroll 4
+                for (int d = lane; d < p.dim_padded; d += 32) to[d] = d < p.dim ? from[d] : T(0.f);
         }
     }
 }
@@ -193,101 +269,145 @@ __global__ void __launch_bounds__(256) align_weight_kernel(Plan p, T *to) {
     }
 }
 
-// ---------------------------------------------------------------------------------------------- after the products
-// One warp per row: joins what the pieces of columns left, in a fixed order.
-__global__ void __launch_bounds__(256) join_kernel(Plan p) {
+// dW's rows on 16-byte boundaries to where the caller wants them.
+template <class T>
+__global__ void __launch_bounds__(256) unalign_weight_kernel(Plan p) {
     const int lane = threadIdx.x & 31;
-    for (i64 row = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); row < p.rows; row += (i64)gridDim.x * 8) {
-        const int c = p.slot_of[row];
-        float loss = 0.f, lse2 = 0.f;
-        if (c >= 0) {
-            float top = LOWEST, sum = 0.f, pz = 0.f;
-            for (int t = lane; t < p.parts; t += 32) {
-                const i64 at = (i64)t * p.rows_padded + c;
-                const float m = p.part_max[at], x = p.part_sum[at];
-                pz += p.part_pz[at];
-                const float both = fmaxf(top, m);
-                sum = sum * exp2f(top - both) + x * exp2f(m - both);
-                top = both;
-            }
-            for (int d = 16; d; d >>= 1) {
-                const float m = __shfl_xor_sync(~0u, top, d), x = __shfl_xor_sync(~0u, sum, d);
-                const float both = fmaxf(top, m);
-                sum = sum * exp2f(top - both) + x * exp2f(m - both);
-                top = both;
-                pz += __shfl_xor_sync(~0u, pz, d);
-            }
-            lse2 = top + log2f(sum);
-            const float tau = p.temperature;
-            loss = tau * tau * (lse2 * 0.69314718055994531f + p.plogp[row] - pz * p.inv_temperature);
-        }
-        if (lane == 0) {
-            if (p.meta->error) loss = NAN;
-            p.lse2[row] = lse2;
-            p.row_loss[row] = loss;
-        }
+    for (i64 j = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); j < p.vocab; j += (i64)gridDim.x * 8) {
+        const T *from = (const T *)p.weight_out + j * p.weight_out_stride;
+#pragma unroll 4
+        for (int d = lane; d < p.dim; d += 32) ((T *)p.grad_weight)[j * p.dim + d] = from[d];
     }
 }
 
-// One CTA: the reduced loss, and what each counted row's G is multiplied by.  G is held in the inputs' 16-bit type, so it is
-// brought into that type's range: the largest |g_i T| becomes 2^14 (a power of two, so bf16 loses nothing; fp16 keeps
-// shares down to 2^-28 at full precision and its entries stay below 2^15), and both gradients are scaled back in 32 bits.
-__global__ void __launch_bounds__(1024) finish_kernel(Plan p) {
-    __shared__ float part[32];
+// ---------------------------------------------------------------------------------------------- after the products
+// 32 rows of a chunk to a block: joins what the parts of the columns left, in a fixed order, to lse and the loss of a row.  Where E is
+// kept, the row's E gets its entries and the packed row its factor.  `again`: the tiles that were made a second time.
+template <class T>
+__global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, bool again, unsigned int all_tickets) {
+    __shared__ float tops[8][32], sums[8][32], lse2s[32], refs[32];
+    __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const i64 n = p.meta->counted;
-    if (p.want_loss && p.reduction != STBPE_REDUCE_NONE) {
-        float sum = 0.f;
-        for (i64 r = threadIdx.x; r < p.rows; r += 1024) sum += p.row_loss[r];
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-        if (lane == 0) part[warp] = sum;
+    const i64 counted = p.meta->counted;
+    const i64 n = counted - r0 < 0 ? 0 : counted - r0 < rows ? counted - r0 : rows;
+    const i64 until = p.keep ? (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS : n;
+    const int entries_of_row = p.k ? p.k : 1;
+    const float scale = p.inv_temperature * 1.4426950408889634f;
+    for (i64 m0 = (i64)blockIdx.x * 32; m0 < until; m0 += (i64)gridDim.x * 32) {
+        if (again && !p.again[(r0 + m0) / TILE_ROWS]) continue;
+        float top = LOWEST, sum = 0.f;
+        if (m0 + lane < n) {
+            const float *from_max = p.part_max + m0 + lane, *from_sum = p.part_sum + m0 + lane;
+            if (p.keep) {  // all parts have the row's reference
+#pragma unroll 4
+                for (int t = warp; t < p.parts; t += 8) {
+                    top = fmaxf(top, from_max[t * p.part_stride]);
+                    sum += from_sum[t * p.part_stride];
+                }
+            } else {
+#pragma unroll 4
+                for (int t = warp; t < p.parts; t += 8) {
+                    const float m = from_max[t * p.part_stride], x = from_sum[t * p.part_stride], both = fmaxf(top, m);
+                    sum = sum * exp2f(top - both) + x * exp2f(m - both);
+                    top = both;
+                }
+            }
+        }
+        tops[warp][lane] = top, sums[warp][lane] = sum;
         __syncthreads();
-        if (threadIdx.x == 0) {
-            float all = 0.f;
-            for (int w = 0; w < 32; ++w) all += part[w];
-            p.loss[0] = p.reduction == STBPE_REDUCE_MEAN ? all / (float)(n > 0 ? n : 1) : all;
+        if (warp == 0) {
+            for (int w = 1; w < 8; ++w) {
+                const float m = tops[w][lane], x = sums[w][lane], both = fmaxf(top, m);
+                sum = p.keep ? sum + x : sum * exp2f(top - both) + x * exp2f(m - both);
+                top = both;
+            }
+            float ref = top;
+            if (p.keep && m0 + lane < n) {
+                ref = p.reference[r0 + m0 + lane];
+                if (!again && fabsf(top - ref) > 96.f && fabsf(top) < INFINITY) {
+                    p.reference[r0 + m0 + lane] = top;
+                    p.again[(r0 + m0) / TILE_ROWS] = 1;
+                }
+            }
+            refs[lane] = ref, lse2s[lane] = ref + log2f(sum);
+        }
+        __syncthreads();
+        for (int y = warp; y < 32; y += 8) {
+            const i64 m = m0 + y, slot = r0 + m;
+            if (m >= until) break;
+            T *scaled = (T *)p.scaled + m * p.dim_padded;
+            if (m >= n) {  // (keep) zeros behind the last row
+                for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)(scaled + d) = make_uint4(0, 0, 0, 0);
+                continue;
+            }
+            const int row = p.row_of[slot];
+            const float lse2 = lse2s[y], ref = refs[y];
+            const float less = exp2f(lse2 - ref);  // keep: a share in the units of E
+            const int2 *e = p.entries + (i64)row * entries_of_row;
+            const float *z = p.entry_z + slot * entries_of_row;
+            float pz = 0.f;
+            for (int k = lane; k < entries_of_row; k += 32) {
+                const int2 it = e[k];
+                if (it.x == INT_MAX) break;
+                pz += __int_as_float(it.y) * z[k];
+                if (p.keep && (k == 0 || e[k - 1].x != it.x)) {  // (the same id again: its first entry takes them all)
+                    float share = __int_as_float(it.y);
+                    for (int l = k + 1; l < entries_of_row && e[l].x == it.x; ++l) share += __int_as_float(e[l].y);
+                    ((T *)p.g)[m * p.g_stride + it.x] = T(exp2f(fmaf(z[k], scale, -ref)) - share * less);
+                }
+            }
+            for (int d = 16; d; d >>= 1) pz += __shfl_xor_sync(~0u, pz, d);
+            if (lane == 0) {
+                const float tau = p.temperature;
+                p.lse2[row] = lse2;
+                p.row_loss[row] = tau * tau * (lse2 * 0.69314718055994531f + p.plogp[row] - pz * p.inv_temperature);
+            }
+            if (p.keep) {
+                const float a = p.coef[slot] * exp2f(ref - lse2);
+                if (lane == 0) p.out_row[slot] = a * p.meta->out_scale;
+                const T *from = (const T *)p.packed + slot * p.dim_padded;
+#pragma unroll 4
+                for (int d = lane * 8; d < p.dim_padded; d += 256) {
+                    uint4 x = *(const uint4 *)(from + d);
+                    T *v = (T *)&x;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = T((float)v[i] * a);
+                    *(uint4 *)(scaled + d) = x;
+                }
+            }
         }
         __syncthreads();
     }
-    if (!p.want_grads) return;
-    const float factor = p.temperature / (p.reduction == STBPE_REDUCE_MEAN ? (float)(n > 0 ? n : 1) : 1.f);
-    auto g = [&](i64 c) {
-        const i64 row = p.row_of[c], o = row / p.inner, i = row - o * p.inner;
-        const float up = !p.grad_loss ? 1.f : p.grad_loss[p.reduction == STBPE_REDUCE_NONE ? o * p.grad_outer + i * p.grad_inner : 0];
-        return isnan(p.plogp[row]) ? NAN : up * factor;
-    };
-    float most = 0.f;
-    for (i64 c = threadIdx.x; c < n; c += 1024) {
-        const float x = fabsf(g(c));
-        if (x <= 3.4e38f) most = fmaxf(most, x);
-    }
-    for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
-    if (lane == 0) part[warp] = most;
+    if (p.reduction == STBPE_REDUCE_NONE || !all_tickets) return;
+    // the block that is through last adds the losses up, in the order of the rows
+    __threadfence();
     __syncthreads();
-    for (int w = 0; w < 32; ++w) most = fmaxf(most, part[w]);
-    // 2^14 over the next power of two, both sides kept within what 32 bits hold as normal numbers
-    int up = 0;
-    if (most > 0.f) frexpf(most, &up);
-    up = max(-100, min(100, up));
-    const float in = ldexpf(1.f, 14 - up);
-    if (threadIdx.x == 0) p.meta->out_scale = ldexpf(1.f, up - 14);
-    for (i64 c = threadIdx.x; c < p.rows_padded; c += 1024) p.coef[c] = c < n ? g(c) * in : 0.f;
+    if (threadIdx.x == 0) last = atomicAdd(&p.meta->tickets, 1u) == all_tickets - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    float sum = 0.f;
+#pragma unroll 8
+    for (i64 r = threadIdx.x; r < p.rows; r += 256) sum += __ldcg(p.row_loss + r);
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+    if (lane == 0) sums[0][warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float all = 0.f;
+        for (int w = 0; w < 8; ++w) all += sums[0][w];
+        p.loss[0] = p.reduction == STBPE_REDUCE_MEAN ? all / (float)(counted > 0 ? counted : 1) : all;
+    }
 }
 
-// dH in the caller's rows and type: sums over the pieces and splits of the vocabulary, zeros where a row does not count.
+// dH of several pieces in the caller's rows and type, zeros where a row does not count.
 template <class T>
 __global__ void __launch_bounds__(256) scatter_kernel(Plan p) {
-    const float scale = p.meta->error ? NAN : p.meta->out_scale;
+    const float scale = p.meta->out_scale;
     const i64 total = p.rows * p.dim;
     for (i64 x = (i64)blockIdx.x * 256 + threadIdx.x; x < total; x += (i64)gridDim.x * 256) {
         const i64 row = x / p.dim, d = x - row * p.dim;
         const int c = p.slot_of[row];
-        float v = 0.f;
-        if (c >= 0) {
-            for (int s = 0; s < p.splits; ++s) v += p.acc[((i64)s * p.rows_padded + c) * p.acc_stride + d];
-            v *= scale;
-        }
-        ((T *)p.grad_hidden)[x] = T(v);
+        ((T *)p.grad_hidden)[x] = T(c < 0 ? 0.f : p.acc[c * p.acc_stride + d] * scale);
     }
 }
 
@@ -305,6 +425,10 @@ int fail(char *err, size_t len, int status, const char *what, const char *why) {
 }
 
 i64 up_to(i64 x, i64 unit) { return (x + unit - 1) / unit * unit; }
+
+// CTAs to a tile of a product.  Pairs on 256 x 256 make 1.6 times as much per SM as single CTAs on 128 x 128, so they are worth it
+// unless the tiles are so few that single CTAs are through in one round, while pairs would leave half of the SMs idle.
+int group_of(i64 rows, i64 cols) { return ((rows + 255) / 256) * ((cols + 255) / 256) <= SMS / 4 ? 1 : 2; }
 
 // Checks the arguments and lays the workspace out; `bytes` gets its size.
 int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_len) {
@@ -327,7 +451,6 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     p.dim_padded = up_to(a->dim, 8);
     p.rows_padded = up_to(p.rows > 0 ? p.rows : 1, TILE_ROWS);
     p.pieces = (int)((a->vocab + PIECE - 1) / PIECE);
-    p.parts = (int)((a->vocab + 64 * VL_GROUP - 1) / (64 * VL_GROUP));
     p.k_sorted = 2;
     while (p.k_sorted < a->k) p.k_sorted *= 2;
     p.temperature = a->temperature, p.inv_temperature = 1.f / a->temperature;
@@ -343,14 +466,23 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     p.loss = a->loss, p.lse2 = a->lse2, p.grad_hidden = a->grad_hidden, p.grad_weight = a->grad_weight;
     const bool aligned = (uintptr_t)a->weight % 16 == 0 && a->weight_stride % 8 == 0 && a->dim % 8 == 0;
     p.weight_rows_stride = aligned ? a->weight_stride : p.dim_padded;
-    // as many columns of G at a time as 256 MiB hold
-    i64 width = up_to(a->vocab, PIECE);
-    const i64 most = (256ll << 20) / (2 * p.rows_padded) / PIECE * PIECE;
-    if (width > most) width = most > 2048 ? most : (width < 2048 ? width : 2048);
-    p.g_stride = width;
-    p.splits = 1;
+    // at most KEPT bytes of E or G at a time (for large vocabularies 2048 rows of E, for many rows 2048 columns of G)
+    constexpr i64 KEPT = 1ll << 30;
+    const i64 all = up_to(a->vocab, PIECE);
+    p.keep = p.want_loss && p.want_grads && a->type == STBPE_REAL_BF16;
+    p.chunk_rows = p.rows_padded, p.g_stride = all;
+    if (p.keep) {
+        const i64 most = KEPT / (2 * all) / TILE_ROWS * TILE_ROWS;
+        p.chunk_rows = p.rows_padded <= most ? p.rows_padded : most > 2048 ? most : p.rows_padded < 2048 ? p.rows_padded : 2048;
+    } else {
+        const i64 most = KEPT / (2 * p.rows_padded) / PIECE * PIECE;
+        p.g_stride = all <= most ? all : most > 2048 ? most : all < 2048 ? all : 2048;
+    }
+    p.group = group_of(p.keep ? p.chunk_rows : p.rows, a->vocab);
+    p.parts = (int)((a->vocab + 64 * p.group - 1) / (64 * p.group));
+    p.part_stride = p.chunk_rows;
     p.acc_stride = up_to(a->dim, 32);
-    p.grad_weight_aligned = (uintptr_t)a->grad_weight % 16 == 0 && a->dim % 8 == 0;
+    p.weight_out = a->grad_weight, p.weight_out_stride = a->dim;
     bytes = 0;
     char *base = (char *)a->workspace;
     auto take = [&](i64 n) {
@@ -370,15 +502,29 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     p.packed = take(p.rows_padded * p.dim_padded * 2);
     p.weight_rows = aligned ? a->weight : take(p.vocab * p.dim_padded * 2);
     if (p.want_loss) {
-        p.part_max = (float *)take(p.rows_padded * 4 * p.parts);
-        p.part_sum = (float *)take(p.rows_padded * 4 * p.parts);
-        p.part_pz = (float *)take(p.rows_padded * 4 * p.parts);
+        p.entry_z = (float *)take(p.rows_padded * 4 * (p.k ? p.k : 1));
+        p.part_max = (float *)take(p.chunk_rows * 4 * p.parts);
+        p.part_sum = (float *)take(p.chunk_rows * 4 * p.parts);
         p.row_loss = a->reduction == STBPE_REDUCE_NONE ? a->loss : (float *)take(p.rows_padded * 4);
     }
     if (p.want_grads) {
         p.coef = (float *)take(p.rows_padded * 4);
-        p.g = take(p.rows_padded * p.g_stride * 2);
-        if (p.grad_hidden) p.acc = (float *)take((i64)p.splits * p.rows_padded * p.acc_stride * 4);
+        p.g = take(p.chunk_rows * p.g_stride * 2);
+        p.split_sums = (float *)take((i64)SMS * 8 * 64 * 2 * 32 * 4);
+        p.split_done = (unsigned int *)take(SMS * 8 * 4);
+        if (p.keep) {
+            p.reference = (float *)take(p.rows_padded * 4);
+            p.out_row = (float *)take(p.rows_padded * 4);
+            p.again = (int *)take(p.rows_padded / TILE_ROWS * 4);
+            p.scaled = take(p.chunk_rows * p.dim_padded * 2);
+            if (p.chunk_rows < p.rows_padded) p.weight_acc = (float *)take(p.vocab * p.acc_stride * 4);
+        } else if (p.g_stride < all) {
+            p.acc = (float *)take(p.rows_padded * p.acc_stride * 4);
+        }
+        if (a->dim % 8) {
+            p.weight_out_stride = p.dim_padded;
+            p.weight_out = take(p.vocab * p.dim_padded * 2);
+        }
     }
     return STBPE_OK;
 }
@@ -404,14 +550,8 @@ int tensor_map(CUtensorMap *map, int type, const void *at, i64 rows, i64 cols, i
     return r == CUDA_SUCCESS ? STBPE_OK : fail(err, err_len, STBPE_E_CUDA, "cuTensorMapEncodeTiled", "refused");
 }
 
-constexpr int SMS = 148;
-
 template <class T, int KIND, int GROUP>
-int launch(const Plan &p, const Job &job, const CUtensorMap &a, const CUtensorMap &b, cudaStream_t s, char *err, size_t err_len) {
-    const i64 tile = 128 * GROUP;
-    const i64 rows = KIND == GRAD_WEIGHT ? job.width : p.rows, cols = KIND <= MAKE_G ? job.width : p.dim;
-    const i64 tiles = ((rows + tile - 1) / tile) * ((cols + tile - 1) / tile);
-    if (tiles == 0) return STBPE_OK;
+int launch(const Plan &p, const Job &job, const CUtensorMap &a, const CUtensorMap &b, i64 tiles, cudaStream_t s, char *err, size_t err_len) {
     auto *kernel = product_kernel<T, KIND, GROUP>;
     VCK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PRODUCT_SMEM));
     cudaLaunchConfig_t c = {};
@@ -427,42 +567,72 @@ int launch(const Plan &p, const Job &job, const CUtensorMap &a, const CUtensorMa
     return STBPE_OK;
 }
 
+template <class T, int KIND>
+int product(const Plan &p, const Job &job, const CUtensorMap &a, const CUtensorMap &b, cudaStream_t s, char *err, size_t err_len) {
+    const i64 rows = KIND == GRAD_WEIGHT ? job.width : p.rows < job.rows ? p.rows : job.rows, cols = KIND <= MAKE_G ? job.width : p.dim;
+    if (rows == 0) return STBPE_OK;
+    const int group = KIND <= MAKE_G ? p.group : group_of(rows, cols);  // (the parts of the columns go by p.group)
+    const i64 tile = 128 * group, tiles = ((rows + tile - 1) / tile) * ((cols + tile - 1) / tile) * (KIND <= MAKE_G ? 1 : SPLITS);
+    return group == 1 ? launch<T, KIND, 1>(p, job, a, b, tiles, s, err, err_len) : launch<T, KIND, 2>(p, job, a, b, tiles, s, err, err_len);
+}
+
 #define VTRY(call)                        \
     do {                                  \
         const int st_ = (call);           \
         if (st_ != STBPE_OK) return st_;  \
     } while (0)
 
-template <class T, int GROUP>
+template <class T>
 int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
     const int wide = SMS * 8;
     auto blocks = [&](i64 n, i64 per) { return (unsigned)(n <= 0 ? 1 : (n + per - 1) / per < wide ? (n + per - 1) / per : wide); };
+    auto map = [&](CUtensorMap *m, const void *at, i64 rows, i64 cols, i64 stride, int box) {
+        return tensor_map(m, type, at, rows, cols, stride, box, err, err_len);
+    };
     if (p.k) teacher_kernel<<<blocks(p.rows, 4), 128, 4 * p.k_sorted * sizeof(u64), s>>>(p);
     rows_kernel<<<1, 1024, 0, s>>>(p);
-    gather_kernel<T><<<blocks(p.rows_padded, 8), 256, 0, s>>>(p);
+    gather_kernel<T><<<blocks(p.rows + TILE_ROWS, 8), 256, 0, s>>>(p);
     if (p.weight_rows != p.weight) align_weight_kernel<T><<<blocks(p.vocab, 8), 256, 0, s>>>(p, (T *)p.weight_rows);
-    CUtensorMap h, w;
-    VTRY(tensor_map(&h, type, p.packed, p.rows_padded, p.dim, p.dim_padded, 128, err, err_len));
-    VTRY(tensor_map(&w, type, p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 128, err, err_len));
-    if (p.want_loss) {
-        VTRY((launch<T, STATS, GROUP>(p, Job{0, p.vocab, 0}, h, w, s, err, err_len)));
-        join_kernel<<<blocks(p.rows, 8), 256, 0, s>>>(p);
-    }
-    if (p.want_grads || p.reduction != STBPE_REDUCE_NONE) finish_kernel<<<1, 1024, 0, s>>>(p);
+    CUtensorMap h, w, h_across, w_across, g, g_across;
+    VTRY(map(&h, p.packed, p.rows_padded, p.dim, p.dim_padded, 128));
+    VTRY(map(&w, p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 128));
     if (p.want_grads) {
-        CUtensorMap h_across, w_across, g, g_across;
-        VTRY(tensor_map(&h_across, type, p.packed, p.rows_padded, p.dim, p.dim_padded, 64, err, err_len));
-        VTRY(tensor_map(&w_across, type, p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 64, err, err_len));
-        VTRY(tensor_map(&g, type, p.g, p.rows_padded, p.g_stride, p.g_stride, 128, err, err_len));
-        VTRY(tensor_map(&g_across, type, p.g, p.rows_padded, p.g_stride, p.g_stride, 64, err, err_len));
-        for (i64 v0 = 0; v0 < p.vocab; v0 += p.g_stride) {
-            const Job job{v0, p.vocab - v0 < p.g_stride ? p.vocab - v0 : p.g_stride, v0 == 0};
-            VTRY((launch<T, MAKE_G, GROUP>(p, job, h, w, s, err, err_len)));
-            if (p.grad_hidden) VTRY((launch<T, GRAD_HIDDEN, GROUP>(p, job, g, w_across, s, err, err_len)));
-            if (p.grad_weight) VTRY((launch<T, GRAD_WEIGHT, GROUP>(p, job, g_across, h_across, s, err, err_len)));
-        }
-        if (p.grad_hidden) scatter_kernel<T><<<blocks(p.rows * p.dim, 256), 256, 0, s>>>(p);
+        VTRY(map(&h_across, p.keep ? p.scaled : p.packed, p.keep ? p.chunk_rows : p.rows_padded, p.dim, p.dim_padded, 64));
+        VTRY(map(&w_across, p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 64));
+        VTRY(map(&g, p.g, p.chunk_rows, p.g_stride, p.g_stride, 128));
+        VTRY(map(&g_across, p.g, p.chunk_rows, p.g_stride, p.g_stride, 64));
     }
+    const unsigned joins = blocks(p.chunk_rows, 32);
+    if (p.keep) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const unsigned tickets = joins * (unsigned)((p.rows_padded + p.chunk_rows - 1) / p.chunk_rows);
+            for (i64 r0 = 0; r0 < p.rows_padded; r0 += p.chunk_rows) {
+                Job job{0, p.vocab, r0, p.chunk_rows, false};
+                VTRY((product<T, MAKE_E>(p, job, h, w, s, err, err_len)));
+                join_kernel<T><<<joins, 256, 0, s>>>(p, r0, p.chunk_rows, false, 0);
+                job.again = true;
+                VTRY((product<T, MAKE_E>(p, job, h, w, s, err, err_len)));
+                join_kernel<T><<<joins, 256, 0, s>>>(p, r0, p.chunk_rows, true, tickets);
+                if (p.grad_hidden) VTRY((product<T, GRAD_HIDDEN>(p, job, g, w_across, s, err, err_len)));
+                if (p.grad_weight) VTRY((product<T, GRAD_WEIGHT>(p, job, g_across, h_across, s, err, err_len)));
+            }
+        }
+    } else {
+        if (p.want_loss) {
+            VTRY((product<T, STATS>(p, Job{0, p.vocab, 0, p.rows_padded, false}, h, w, s, err, err_len)));
+            join_kernel<T><<<joins, 256, 0, s>>>(p, 0, p.rows_padded, false, joins);
+        }
+        if (p.want_grads) {
+            for (i64 v0 = 0; v0 < p.vocab; v0 += p.g_stride) {
+                const Job job{v0, p.vocab - v0 < p.g_stride ? p.vocab - v0 : p.g_stride, 0, p.rows_padded, false};
+                VTRY((product<T, MAKE_G>(p, job, h, w, s, err, err_len)));
+                if (p.grad_hidden) VTRY((product<T, GRAD_HIDDEN>(p, job, g, w_across, s, err, err_len)));
+                if (p.grad_weight) VTRY((product<T, GRAD_WEIGHT>(p, job, g_across, h_across, s, err, err_len)));
+            }
+            if (p.grad_hidden && p.acc) scatter_kernel<T><<<blocks(p.rows * p.dim, 256), 256, 0, s>>>(p);
+        }
+    }
+    if (p.want_grads && p.grad_weight && p.weight_out != p.grad_weight) unalign_weight_kernel<T><<<blocks(p.vocab, 8), 256, 0, s>>>(p);
     VCK(cudaGetLastError());
     return STBPE_OK;
 }
@@ -490,10 +660,12 @@ STBPE_VISIBLE int stbpe_vocab_loss_run(const stbpe_vocab_loss *args, void *strea
         return fail(err, err_len, STBPE_E_CAPACITY, "stbpe_vocab_loss", "workspace missing, not on a 1024-byte boundary or too small");
     if (!args->lse2 || (p.want_loss && !args->loss) || (p.want_grads && !args->grad_hidden && !args->grad_weight))
         return fail(err, err_len, STBPE_E_BADARG, "stbpe_vocab_loss", "an output is missing");
+    if ((uintptr_t)args->grad_hidden % 16 || (uintptr_t)args->grad_weight % 16)
+        return fail(err, err_len, STBPE_E_BADARG, "stbpe_vocab_loss", "gradients start on 16-byte boundaries");
     if (!args->weight || (p.rows && (!args->hidden || !args->ids || (p.k && !args->logits))))
         return fail(err, err_len, STBPE_E_BADARG, "stbpe_vocab_loss", "an input is missing");
-    return args->type == STBPE_REAL_BF16 ? run<__nv_bfloat16, VL_GROUP>(p, args->type, (cudaStream_t)stream, err, err_len)
-                                         : run<__half, VL_GROUP>(p, args->type, (cudaStream_t)stream, err, err_len);
+    return args->type == STBPE_REAL_BF16 ? run<__nv_bfloat16>(p, args->type, (cudaStream_t)stream, err, err_len)
+                                         : run<__half>(p, args->type, (cudaStream_t)stream, err, err_len);
 }
 
 }  // extern "C"

@@ -1,4 +1,4 @@
-// What the kernels of the losses over a large vocabulary share (vocab_loss.cu).
+// What the kernels of the losses over a large vocabulary share (vocab_loss.cu, vocab_products.cuh).
 #pragma once
 #include <limits.h>
 #include <stdint.h>
@@ -8,23 +8,24 @@ namespace vloss {
 typedef unsigned long long u64;
 typedef long long i64;
 
+constexpr int SMS = 148;
 constexpr int PIECE = 256;      // columns per step of the table that finds a row's entries
-constexpr int TILE_ROWS = 256;  // the packed rows end on this boundary
+constexpr int TILE_ROWS = 256;  // packed rows are filled up with zeros to this boundary
 
 // the running maximum starts at a finite value: a logit of -inf then adds 0 to the sum, and one of NaN or +inf makes it NaN
 #define LOWEST (-3.0e38f)
 
 struct Meta {
     int counted;          // rows that count
-    unsigned int error;   // a wait inside a product ran out
+    unsigned int tickets; // blocks that are through with their rows' losses
     float out_scale;      // what both gradients are multiplied by in the end
 };
 
 struct Plan {
     i64 rows, inner;  // row = outer * inner + inner index
     i64 vocab, dim, dim_padded, rows_padded;
-    int k, k_sorted, pieces, parts, reduction, splits;
-    bool want_loss, want_grads, hidden_aligned, grad_weight_aligned;
+    int k, k_sorted, pieces, parts, reduction, group;
+    bool want_loss, want_grads, hidden_aligned;
     float temperature, inv_temperature;
     const void *hidden, *weight, *ids, *logits;
     const unsigned char *valid;
@@ -42,15 +43,29 @@ struct Plan {
     int2 *entries;           // (id, share) of a row in ascending order of the ids, INT_MAX behind the last one
     unsigned short *first;   // first entry of a row at or behind a piece's first column
     unsigned char *has_entries;
+    float *entry_z;          // logits at the entries of a packed row
     void *packed;            // counted rows of hidden, one behind another
     const void *weight_rows; // weight, or its copy with rows on 16-byte boundaries
     i64 weight_rows_stride;
-    float *part_max, *part_sum, *part_pz, *row_loss;  // [part][packed row]; per row
-    float *coef;             // what a packed row of G is multiplied by
-    void *g;                 // G of one piece of the vocabulary, [packed row][g_stride]
-    i64 g_stride;
-    float *acc;              // dH of packed rows in 32 bits, [split][packed row][acc_stride]
+    float *part_max, *part_sum, *row_loss;  // [part][packed row of the chunk]; per row
+    i64 part_stride;
+    float *coef;             // what a packed row of dlogits is multiplied by
+    // G (16 bits) of one piece of the vocabulary and all packed rows; or E = exp2(logits - reference) of the whole
+    // vocabulary and a chunk of the packed rows (keep)
+    bool keep;
+    void *g;
+    i64 g_stride, chunk_rows;
+    float *reference;        // keep: per packed row
+    int *again;              // keep: [packed row / TILE_ROWS] a reference was too far from the row's maximum
+    float *out_row;          // keep: what a packed row of dH is multiplied by
+    void *scaled;            // keep: packed rows of the chunk, times coef exp2(reference - lse2)
+    float *acc;              // several pieces: dH of packed rows in 32 bits, [packed row][acc_stride]
+    float *weight_acc;       // several chunks: dW in 32 bits, [vocab][acc_stride]
     i64 acc_stride;
+    void *weight_out;        // where dW goes: grad_weight, or rows on 16-byte boundaries
+    i64 weight_out_stride;
+    float *split_sums;       // sums of tiles whose depth is split
+    unsigned int *split_done;
 };
 
 }  // namespace vloss

@@ -1,14 +1,17 @@
 // The products of the losses over a large vocabulary on the tensor cores: tcgen05 with its operands in shared memory, filled by
 // TMA, and its sums (32 bits) in TMEM.
 //
-//   STATS        Z = H W^T of the whole vocabulary; per row and piece of columns the maximum, the sum of exp and sum p z
-//   MAKE_G       Z again, of one piece of the vocabulary, and G from it in 16 bits
-//   GRAD_HIDDEN  dH += G W      (k over the piece's columns: W is read with the other dimension contiguous)
-//   GRAD_WEIGHT  dW = G^T H     (k over the rows: both are read with the other dimension contiguous)
+//   STATS        Z = H W^T; per row and part of the columns the maximum and the sum of exp, the logits at the entries
+//   MAKE_E       the same, and E = exp2(Z - reference) in 16 bits
+//   MAKE_G       Z again, of one piece of the vocabulary, and G = dlogits from it in 16 bits
+//   GRAD_HIDDEN  dH = E W or G W        (k over the columns: W is read with the other dimension contiguous)
+//   GRAD_WEIGHT  dW = E^T H' or G^T H   (k over the rows: both are read with the other dimension contiguous)
 //
 // A group of GROUP CTAs makes a tile of 128 GROUP x 128 GROUP: with GROUP = 2 the two CTAs of a cluster share one
 // 256 x 256 tile (cta_group::2), each holding its half of both operands, so that a byte brought into shared memory serves twice as
-// many products.  A CTA loads 128 x 64 of each operand per step in either case.  Persistent: the tiles are dealt out
+// many products.  A CTA loads 128 x 64 of each operand per step in either case: 64 bytes per SM and clock at the full rate
+// with GROUP = 2, 128 with GROUP = 1, which L2 does not deliver (0.93 to 0.98 PFLOP/s against 1.24 to 1.59 at
+// 8 188 x 32 256 x 2 048).  Persistent: the tiles are dealt out
 // to the clusters in turn, and the sums of one tile are looked at while the next one is being made (two buffers in TMEM).
 // Warp 0 loads, warp 1 of the group's first CTA multiplies, warp 2 owns the TMEM, warps 4 to 11 take the sums.
 #pragma once
@@ -22,17 +25,19 @@
 
 namespace vloss {
 
-enum { STATS, MAKE_G, GRAD_HIDDEN, GRAD_WEIGHT };
+enum { STATS, MAKE_E, MAKE_G, GRAD_HIDDEN, GRAD_WEIGHT };
 
 constexpr int STAGES = 6;
 constexpr int OPERAND_BYTES = 128 * 64 * 2;  // what a CTA loads of one operand per step of 64 terms
 constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
+constexpr int SPLITS = 8;
 constexpr int PRODUCT_THREADS = 384;
 constexpr int PRODUCT_SMEM = STAGES * STAGE_BYTES + 1024 + 256;
 
 struct Job {
-    i64 v0, width;   // the piece of the vocabulary
-    int first;       // GRAD_HIDDEN: nothing to add to
+    i64 v0, width;  // the piece of the vocabulary
+    i64 r0, rows;   // the chunk of the packed rows
+    bool again;     // MAKE_E: only where a reference was too far off
 };
 
 // ---------------------------------------------------------------------------------------------- instructions
@@ -56,8 +61,9 @@ __device__ __forceinline__ void barrier_arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// Every wait ends: after two seconds the error is recorded, and all roles leave their loops as they meet it.
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, unsigned int *error) {
+// Every wait ends: after two seconds it fails, all roles leave their loops as that happens to them, and what was to be
+// computed becomes NaN.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
     uint32_t done;
     u64 began = 0;
     for (;;) {
@@ -72,10 +78,7 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, unsi
         u64 now;
         asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
         if (!began) began = now;
-        if (now - began > 2000000000ull) {
-            atomicOr(error, 1u);
-            return false;
-        }
+        if (now - began > 2000000000ull) return false;
     }
 }
 
@@ -201,7 +204,7 @@ template <class T, int KIND, int GROUP>
 __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
     product_kernel(const __grid_constant__ Plan p, const __grid_constant__ Job job, const __grid_constant__ CUtensorMap map_a,
                    const __grid_constant__ CUtensorMap map_b) {
-    constexpr bool LOGITS = KIND == STATS || KIND == MAKE_G;
+    constexpr bool LOGITS = KIND <= MAKE_G, GRADS = !LOGITS;
     constexpr bool A_ALONG_K = KIND != GRAD_WEIGHT, B_ALONG_K = LOGITS;
     constexpr u64 A_NEXT = (A_ALONG_K ? 32 : 2048) >> 4, B_NEXT = (B_ALONG_K ? 32 : 2048) >> 4;  // 16 k further, for the descriptors
     constexpr int TILE = 128 * GROUP, COLUMNS = TILE / 2;  // columns that one epilogue thread takes of its row
@@ -216,7 +219,6 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t rank = 0;
     if (GROUP == 2) asm("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
-    unsigned int *error = &p.meta->error;
 
     if (warp == 0 && lane == 0) {
         for (int s = 0; s < STAGES; ++s) barrier_init(full + 8 * s, 1), barrier_init(empty + 8 * s, 1);
@@ -240,21 +242,47 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
 
     // the tiles and their depth
-    const i64 n = p.meta->counted;
+    const i64 counted = p.meta->counted;
+    const i64 n = counted - job.r0 < 0 ? 0 : counted - job.r0 < job.rows ? counted - job.r0 : job.rows;  // rows of this chunk
     const i64 rows = KIND == GRAD_WEIGHT ? job.width : n, cols = LOGITS ? job.width : p.dim;
     const i64 depth = LOGITS ? p.dim : KIND == GRAD_HIDDEN ? job.width : n;
     const i64 tiles_m = (rows + TILE - 1) / TILE, tiles_n = (cols + TILE - 1) / TILE;
     const int steps = (int)((depth + 63) / 64);
-    const i64 tiles = tiles_m * tiles_n;
+    const i64 tiles = KIND == GRAD_WEIGHT && job.r0 > 0 && n == 0 ? 0 : tiles_m * tiles_n;
     const i64 cluster = blockIdx.x / GROUP, clusters = gridDim.x / GROUP;
+    // The tiles behind the last full round of all clusters are split in depth, so that the round that is not full is shorter, too:
+    // up to SPLITS units per tile of eight steps at least.
+    const bool may_split = GRADS && (KIND == GRAD_WEIGHT ? !p.weight_acc : !p.acc);
+    const i64 left = tiles % clusters;
+    i64 splits = 1;
+    if (may_split && left > 0) {
+        splits = clusters / left < SPLITS ? clusters / left : SPLITS;
+        if (splits > steps / 8) splits = steps / 8;
+        if (splits < 1) splits = 1;
+    }
+    const i64 whole = tiles - left, units = whole + left * splits;
     // a band of BAND tiles of rows goes through all columns, its rows first: that much of A stays in L2
     constexpr i64 BAND = 16;
-    auto place = [&](i64 tile, i64 &m0, i64 &n0) {
+    struct Unit {
+        i64 m0, n0;
+        int k0, k1, split, index;  // steps; number of the split tile
+    };
+    auto unit_at = [&](i64 u) {
+        Unit t;
+        i64 tile = u;
+        t.k0 = 0, t.k1 = steps, t.split = -1, t.index = 0;
+        if (u >= whole && splits > 1) {
+            t.index = (int)((u - whole) % left), t.split = (int)((u - whole) / left);
+            tile = whole + t.index;
+            t.k0 = (int)((i64)steps * t.split / splits), t.k1 = (int)((i64)steps * (t.split + 1) / splits);
+        }
         const i64 band = tile / (BAND * tiles_n), in = tile - band * BAND * tiles_n;
         const i64 high = tiles_m - band * BAND < BAND ? tiles_m - band * BAND : BAND;
-        n0 = in / high * TILE;
-        m0 = (band * BAND + in % high) * TILE;
+        t.n0 = in / high * TILE;
+        t.m0 = (band * BAND + in % high) * TILE;
+        return t;
     };
+    auto skipped = [&](const Unit &t) { return KIND == MAKE_E && job.again && !p.again[(job.r0 + t.m0) / TILE_ROWS]; };
 
     if (warp == 0) {
         if (lane == 0) {
@@ -262,12 +290,12 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             uint32_t phase = 0;
             i64 issued = 0;
             bool alive = true;
-            for (i64 tile = cluster; tile < tiles && alive; tile += clusters) {
-                i64 m0, n0;
-                place(tile, m0, n0);
-                const int am = (int)(m0 + rank * 128), bn = (int)(n0 + rank * 128);
-                for (int k = 0; k < steps; ++k) {
-                    if (!barrier_wait(empty + 8 * s, phase ^ 1, error)) {
+            for (i64 u = cluster; u < units && alive; u += clusters) {
+                const Unit t = unit_at(u);
+                if (skipped(t)) continue;
+                const int am = (int)(t.m0 + rank * 128), bn = (int)(t.n0 + rank * 128);
+                for (int k = t.k0; k < t.k1; ++k) {
+                    if (!barrier_wait(empty + 8 * s, phase ^ 1)) {
                         alive = false;
                         break;
                     }
@@ -275,7 +303,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     const uint32_t bar = GROUP == 2 ? in_cta(full + 8 * s, 0) : full + 8 * s;
                     if (rank == 0) barrier_expect(full + 8 * s, GROUP * STAGE_BYTES);
                     if (A_ALONG_K) {
-                        tma_load<GROUP>(a, &map_a, k * 64, am, bar);
+                        tma_load<GROUP>(a, &map_a, k * 64, (LOGITS ? (int)job.r0 : 0) + am, bar);
                     } else {
                         tma_load<GROUP>(a, &map_a, am, k * 64, bar);
                         tma_load<GROUP>(a + 8192, &map_a, am + 64, k * 64, bar);
@@ -293,8 +321,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             }
             if (!alive && rank == 0) {  // copies in flight land before the memory is given up
                 const i64 pending = issued < STAGES ? issued : STAGES;
-                for (i64 x = issued - pending; x < issued; ++x)
-                    barrier_wait(full + 8 * (int)(x % STAGES), (uint32_t)(x / STAGES & 1), error);
+                for (i64 x = issued - pending; x < issued; ++x) barrier_wait(full + 8 * (int)(x % STAGES), (uint32_t)(x / STAGES & 1));
             }
         }
         __syncwarp();
@@ -303,23 +330,24 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             int s = 0, buffer = 0;
             uint32_t phase = 0, sums_phase = 0;
             bool alive = true;
-            for (i64 tile = cluster; tile < tiles && alive; tile += clusters) {
-                if (!barrier_wait(sums_empty + 8 * buffer, sums_phase ^ 1, error)) {
+            for (i64 u = cluster; u < units && alive; u += clusters) {
+                const Unit t = unit_at(u);
+                if (skipped(t)) continue;
+                if (!barrier_wait(sums_empty + 8 * buffer, sums_phase ^ 1)) {
                     alive = false;
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t d = tmem + buffer * TILE;
-                for (int k = 0; k < steps; ++k) {
-                    if (!barrier_wait(full + 8 * s, phase, error)) {
+                for (int k = t.k0; k < t.k1; ++k) {
+                    if (!barrier_wait(full + 8 * s, phase)) {
                         alive = false;
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const u64 a = operand<A_ALONG_K>(base + s * STAGE_BYTES), b = operand<B_ALONG_K>(base + s * STAGE_BYTES + OPERAND_BYTES);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        mma<GROUP>(d, a + x * A_NEXT, b + x * B_NEXT, WHAT, k > 0 || x > 0);
+                    for (int x = 0; x < 4; ++x) mma<GROUP>(d, a + x * A_NEXT, b + x * B_NEXT, WHAT, k > t.k0 || x > 0);
                     mma_commit<GROUP>(empty + 8 * s);
                     if (++s == STAGES) s = 0, phase ^= 1;
                 }
@@ -329,55 +357,123 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             }
             if (!alive) {  // products in flight end before the TMEM is given up
                 mma_commit<GROUP>(drained);
-                barrier_wait(drained, 0, error);
+                barrier_wait(drained, 0);
             }
         }
         __syncwarp();
     } else if (warp >= 4) {
         const int quarter = warp & 3, half = (warp - 4) >> 2;
+        const float scale = p.inv_temperature * 1.4426950408889634f;
+        const int entries_of_row = p.k ? p.k : 1;
         int buffer = 0;
         uint32_t sums_phase = 0;
-        for (i64 tile = cluster; tile < tiles; tile += clusters) {
-            i64 m0, n0;
-            place(tile, m0, n0);
-            const i64 m = m0 + rank * 128 + quarter * 32 + lane;  // this thread's row of the result
-            const i64 c0 = n0 + half * COLUMNS;                   // and its first column
-            i64 row = -1;
-            float lse2 = 0.f, coef = 0.f, top = LOWEST, sum = 0.f, pz = 0.f;
-            const float scale = p.inv_temperature * 1.4426950408889634f;
+        bool alive = true;  // once a wait has run out, all that is left becomes NaN
+        for (i64 u = cluster; u < units; u += clusters) {
+            const Unit t = unit_at(u);
+            if (skipped(t)) continue;
+            const i64 m = t.m0 + rank * 128 + quarter * 32 + lane;  // this thread's row of the result
+            const i64 c0 = t.n0 + half * COLUMNS;                   // and its first column
+            const i64 slot = job.r0 + m;
+            int row = -1;
+            // exp2(0 - inf) = 0 in the rows that fill the last tile up
+            float shift = INFINITY, coef = 0.f, top = LOWEST, sum = 0.f;
             Walk walk;
             if (LOGITS) {
-                row = m < p.rows_padded ? p.row_of[m] : -1;
+                row = slot < p.rows_padded ? p.row_of[slot] : -1;
                 if (row >= 0 && job.v0 + c0 < p.vocab) walk.start(p, row, job.v0 + c0);
                 else walk.next.x = INT_MAX, walk.at = walk.all = 0;
-                if (KIND == MAKE_G && row >= 0) lse2 = p.lse2[row], coef = p.coef[m];
+                if (KIND == MAKE_E && row >= 0) shift = p.reference[slot];
+                if (KIND == MAKE_G && row >= 0) shift = p.lse2[row], coef = p.coef[slot];
             }
-            const float out_scale = KIND == GRAD_WEIGHT ? p.meta->out_scale : 1.f;
-            if (!__all_sync(~0u, barrier_wait(sums_full + 8 * buffer, sums_phase, error))) break;
+            if (KIND == GRAD_HIDDEN && m < n) {
+                row = p.row_of[slot];
+                coef = p.keep ? p.out_row[slot] : p.meta->out_scale;
+            }
+            if (KIND == GRAD_WEIGHT) coef = p.meta->out_scale;
+            // 32 sums of dH or dW, at column c of this thread's columns
+            auto emit = [&](int c, float(&v)[32]) {
+                if (KIND == GRAD_HIDDEN) {
+                    if (m >= n || c0 + c >= p.dim) return;
+                    if (!p.acc) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) v[x] *= coef;
+                        store_row((T *)p.grad_hidden + (i64)row * p.dim + c0 + c, v, p.dim - c0 - c, p.dim % 8 == 0);
+                    } else {
+                        float4 *to = (float4 *)(p.acc + m * p.acc_stride + c0 + c);
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            float4 y = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+                            if (job.v0 > 0) {
+                                const float4 z = to[x];
+                                y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+                            }
+                            to[x] = y;
+                        }
+                    }
+                }
+                if (KIND == GRAD_WEIGHT) {
+                    if (m >= job.width || c0 + c >= p.dim) return;
+                    const i64 id = job.v0 + m;
+                    const bool last = counted <= job.r0 + job.rows;
+                    float4 *to = (float4 *)(p.weight_acc + id * p.acc_stride + c0 + c);
+                    if (job.r0 > 0) {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const float4 z = to[x];
+                            v[4 * x] += z.x, v[4 * x + 1] += z.y, v[4 * x + 2] += z.z, v[4 * x + 3] += z.w;
+                        }
+                    }
+                    if (last) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) v[x] *= coef;
+                        store_row((T *)p.weight_out + id * p.weight_out_stride + c0 + c, v, p.dim - c0 - c, true);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) to[x] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+                    }
+                }
+            };
+            if (alive) alive = __all_sync(~0u, barrier_wait(sums_full + 8 * buffer, sums_phase));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t from = tmem + buffer * TILE + half * COLUMNS + ((uint32_t)(quarter * 32) << 16);
+            // [split tile][split][CTA][warp][column][lane]
+            float *sums = p.split_sums + ((((i64)t.index * splits + t.split) * GROUP + rank) * 8 + warp - 4) * (COLUMNS * 32) + lane;
 #pragma unroll 1
             for (int c = 0; c < COLUMNS; c += 32) {
-                uint32_t bits[32];
+                float v[32];
                 __syncwarp();
-                tmem_load(from + c, bits);
-                if (c + 32 == COLUMNS) {  // the buffer is free
+                if (alive) {
+                    uint32_t bits[32];
+                    tmem_load(from + c, bits);
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) v[x] = t.k1 > t.k0 ? __uint_as_float(bits[x]) : 0.f;  // (no rows: nothing was summed)
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) v[x] = NAN;
+                }
+                if (c + 32 == COLUMNS && alive) {  // the buffer is free
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) barrier_arrive_cluster(GROUP == 2 ? in_cta(sums_empty + 8 * buffer, 0) : sums_empty + 8 * buffer);
                 }
-                float v[32];
+                if (GRADS) {
+                    if (t.split < 0) {
+                        emit(c, v);
+                    } else {
 #pragma unroll
-                for (int x = 0; x < 32; ++x) v[x] = steps ? __uint_as_float(bits[x]) : 0.f;  // (no rows: nothing was summed)
-                const i64 j = job.v0 + c0 + c;  // first column, as a token id (LOGITS)
-                if (KIND == STATS) {
+                        for (int x = 0; x < 32; ++x) __stcg(sums + (c + x) * 32, v[x]);
+                    }
+                    continue;
+                }
+                const i64 j = job.v0 + c0 + c;  // first column, as a token id
+                if (KIND == STATS || KIND == MAKE_E) {
                     while (walk.next.x < j + 32) {
                         const int x0 = walk.next.x - (int)j;
                         float z = 0.f;
 #pragma unroll
                         for (int x = 0; x < 32; ++x)
                             if (x == x0) z = v[x];
-                        pz += __int_as_float(walk.next.y) * z;
+                        p.entry_z[slot * entries_of_row + walk.at] = z;
                         walk.advance();
                     }
                     if (j + 32 > p.vocab) {
@@ -388,15 +484,21 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     float most = v[0];
 #pragma unroll
                     for (int x = 1; x < 32; ++x) most = fmaxf(most, v[x]);
-                    const float now = fmaxf(top, most * scale);
-                    sum *= exp2_fast(top - now);
-                    top = now;
+                    if (KIND == STATS) {
+                        shift = fmaxf(top, most * scale);
+                        sum *= exp2_fast(top - shift);
+                        top = shift;
+                    } else {
+                        top = fmaxf(top, most * scale);
+                    }
+                }
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) sum += exp2_fast(fmaf(v[x], scale, -now));
+                for (int x = 0; x < 32; ++x) v[x] = exp2_fast(fmaf(v[x], scale, -shift));
+                if (KIND == STATS || KIND == MAKE_E) {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) sum += v[x];
                 }
                 if (KIND == MAKE_G) {
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) v[x] = exp2_fast(fmaf(v[x], scale, -lse2));
                     while (walk.next.x < j + 32) {
                         const int x0 = walk.next.x - (int)j;
 #pragma unroll
@@ -405,35 +507,45 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                         walk.advance();
                     }
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) v[x] = row >= 0 && j + x < p.vocab ? v[x] * coef : 0.f;
-                    if (m < p.rows_padded && c0 + c < p.g_stride) store_row((T *)p.g + m * p.g_stride + c0 + c, v, 32, true);
-                }
-                if (KIND == GRAD_HIDDEN) {
-                    if (m < n && c0 + c < p.acc_stride) {
-                        float4 *to = (float4 *)(p.acc + m * p.acc_stride + c0 + c);
+                    for (int x = 0; x < 32; ++x) v[x] *= coef;
+                    if (j + 32 > p.vocab) {
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) {
-                            float4 y = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
-                            if (!job.first) {
-                                const float4 z = to[x];
-                                y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
-                            }
-                            to[x] = y;
-                        }
+                        for (int x = 0; x < 32; ++x)
+                            if (j + x >= p.vocab) v[x] = 0.f;
                     }
                 }
-                if (KIND == GRAD_WEIGHT) {
-                    const i64 id = job.v0 + m;
-                    if (m < job.width && c0 + c < p.dim) {
-#pragma unroll
-                        for (int x = 0; x < 32; ++x) v[x] *= out_scale;
-                        store_row((T *)p.grad_weight + id * p.dim + c0 + c, v, p.dim - c0 - c, p.grad_weight_aligned);
-                    }
+                if (KIND == MAKE_E || KIND == MAKE_G) {
+                    if (m < p.chunk_rows && c0 + c < p.g_stride) store_row((T *)p.g + m * p.g_stride + c0 + c, v, 32, true);
                 }
             }
-            if (KIND == STATS && row >= 0 && job.v0 + c0 < p.vocab) {
-                const i64 to = (job.v0 + c0) / COLUMNS * p.rows_padded + m;
-                p.part_max[to] = top, p.part_sum[to] = sum, p.part_pz[to] = pz;
+            if ((KIND == STATS || KIND == MAKE_E) && row >= 0 && job.v0 + c0 < p.vocab) {
+                const i64 to = (job.v0 + c0) / COLUMNS * p.part_stride + m;
+                p.part_max[to] = top, p.part_sum[to] = sum;
+            }
+            if (GRADS && t.split >= 0) {
+                // the last of the splits to get here adds them up, in their order
+                __threadfence();
+                __syncwarp();
+                unsigned int *done = p.split_done + (t.index * GROUP + rank) * 8 + warp - 4;
+                unsigned int before = 0;
+                if (lane == 0) before = atomicAdd(done, 1u);
+                before = __shfl_sync(~0u, before, 0);
+                if (before == splits - 1) {
+                    __threadfence();
+                    if (lane == 0) *done = 0;
+                    const i64 next = (i64)GROUP * 8 * COLUMNS * 32;
+                    sums -= t.split * next;
+#pragma unroll 1
+                    for (int c = 0; c < COLUMNS; c += 32) {
+                        float v[32];
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) v[x] = __ldcg(sums + (c + x) * 32);
+                        for (int s = 1; s < splits; ++s)
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) v[x] += __ldcg(sums + s * next + (c + x) * 32);
+                        emit(c, v);
+                    }
+                }
             }
             buffer ^= 1;
             if (buffer == 0) sums_phase ^= 1;

@@ -7,7 +7,9 @@ for sums that truncate):
              of at most 256 terms
   G          u |G| for its rounding, and (2 s max|dz| + 16 e (1 + |lse|)) (q + p) for the logits; fp16 steps are 2^-25 of the
              largest |g T| at least
-  gradients  sums of |dG| times the other factor, (terms) e of the sum of |G| times it, and u of the result's own rounding
+  gradients  sums of |dG| times the other factor, (terms) e of the sum of |G| times it, and u of the result's own rounding; in dW
+             of the call that returns loss and gradients h times its row's factor is rounded to 16 bits, too:
+             G (1 + a) h (1 + b) with |a|, |b| <= u is off by at most (u + u + u^2) |G h|
 """
 import math
 
@@ -69,7 +71,7 @@ def formula(hidden, weight, ids, logits=None, valid=None, T=1.0, reduction="mean
         tiny * f.abs().amax() * live[:, None]
     gh, gw = G @ w, G.T @ h
     gh_tol = dG @ w.abs() + (V + 4) * E32 * (G.abs() @ w.abs())
-    gw_tol = dG.T @ h.abs() + (n + 4) * E32 * (G.abs().T @ h.abs())
+    gw_tol = (dG + (u + u * u) * G.abs()).T @ h.abs() + (n + 4) * E32 * (G.abs().T @ h.abs())
     out = {"gh": gh.view(*shape, D), "gw": gw,
            "gh_tol": (gh_tol + u * (gh.abs() + gh_tol) + tiny).view(*shape, D),
            "gw_tol": gw_tol + u * (gw.abs() + gw_tol) + tiny}
@@ -98,7 +100,7 @@ def check(hidden, weight, *args, valid=None, T=None, reduction="mean", grad=None
     loss, gh, gw = grads_of(hidden, weight, *args, valid, grad, reduction=reduction, **more)
     assert loss.dtype == torch.float32 and gh.dtype == gw.dtype == hidden.dtype
     near(loss, want, "loss"), near(gh, want, "gh"), near(gw, want, "gw")
-    assert torch.equal(loss_of(hidden, weight, *args, valid, reduction=reduction, **more), loss)
+    near(loss_of(hidden, weight, *args, valid, reduction=reduction, **more), want, "loss")  # (sums about another reference)
     h, w = hidden.detach().requires_grad_(True), weight.detach().requires_grad_(True)
     auto = loss_of(h, w, *args, valid, reduction=reduction, **more)
     up = torch.ones_like(auto) if grad is None else torch.as_tensor(grad, device="cuda", dtype=torch.float32).expand_as(auto)
@@ -448,3 +450,31 @@ def test_a_vocabulary_is_trained_and_a_model_over_it():
         near(gw, want, "gw")
         with torch.no_grad():
             student -= gw
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K", [0, 5])
+def test_more_rows_and_ids_than_are_held_at_a_time(K, dtype):
+    """2 300 rows over 300 001 ids are two chunks of rows (or two pieces of the vocabulary); fewer rows than a chunk count, too."""
+    args = make(1, 2300, 64, 300_001, K, dtype=dtype)
+    check(*args, grad=64.0)
+    valid = torch.arange(2300, device="cuda")[None] % 3 == 0
+    check(*args, valid=valid, grad=64.0)
+
+
+@pytest.mark.parametrize("K", [0, 7])
+def test_rows_of_any_height(K):
+    """Rows whose logits lie far above or below 0 beside ordinary ones: an offset along one column of hidden."""
+    hidden, weight, *rest = make(3, 200, 64, 1000, K)
+    weight[:, 0] = 1.0
+    hidden[..., 0] = 0.0
+    hidden[0, 17, 0], hidden[0, 18, 0], hidden[1, 150:, 0], hidden[2, :2, 0] = 90.0, -90.0, 250.0, -3000.0
+    check(hidden, weight, *rest)
+    check(hidden, weight, *rest, reduction="none")
+
+
+def test_splits_of_the_depth():
+    """Few tiles over a long vocabulary or many rows."""
+    check(*make(1, 5, 64, 40_000))
+    check(*make(2, 2500, 72, 130))
+    check(*make(1, 300, 520, 20_000, 3))
