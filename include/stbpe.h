@@ -377,6 +377,9 @@ typedef struct stbpe_vocab_loss {
 int stbpe_vocab_loss_workspace(const stbpe_vocab_loss *args, int64_t *bytes, char *err, size_t err_len);
 int stbpe_vocab_loss_run(const stbpe_vocab_loss *args, void *stream, char *err, size_t err_len);
 
+/* Two arrays of bf16 (NULL: none) on 16-byte boundaries times *by (device), in place; nothing is touched where it is 1. */
+int stbpe_scale_gradients(void *a, int64_t n_a, void *b, int64_t n_b, const float *by, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -104,6 +104,7 @@ SIGNATURES = {
                                               ctypes.c_char_p, ctypes.c_size_t]),
     "stbpe_vocab_loss_workspace": (_int, [_P(VocabLoss), _P(_i64), ctypes.c_char_p, ctypes.c_size_t]),
     "stbpe_vocab_loss_run": (_int, [_P(VocabLoss), _vp, ctypes.c_char_p, ctypes.c_size_t]),
+    "stbpe_scale_gradients": (_int, [_vp, _i64, _vp, _i64, _vp, _vp]),
     "stbpe_rows_apply_merge": (_int, [_vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp]),
 }
 

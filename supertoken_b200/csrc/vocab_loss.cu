@@ -399,6 +399,27 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
     }
 }
 
+// What comes down to the loss, onto gradients that were made with it.
+__global__ void __launch_bounds__(256) scale_kernel(__nv_bfloat16 *a, i64 n_a, __nv_bfloat16 *b, i64 n_b, const float *by) {
+    const float f = *by;
+    if (f == 1.f) return;
+    for (int which = 0; which < 2; ++which) {
+        __nv_bfloat16 *p = which ? b : a;
+        const i64 n = which ? n_b : n_a;
+        for (i64 x = ((i64)blockIdx.x * 256 + threadIdx.x) * 8; x < n; x += (i64)gridDim.x * 2048) {
+            if (x + 8 <= n) {
+                uint4 v = *(uint4 *)(p + x);
+                __nv_bfloat16 *e = (__nv_bfloat16 *)&v;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = __float2bfloat16(__bfloat162float(e[i]) * f);
+                *(uint4 *)(p + x) = v;
+            } else {
+                for (i64 i = x; i < n; ++i) p[i] = __float2bfloat16(__bfloat162float(p[i]) * f);
+            }
+        }
+    }
+}
+
 // dH of several pieces in the caller's rows and type, zeros where a row does not count.
 template <class T>
 __global__ void __launch_bounds__(256) scatter_kernel(Plan p) {
@@ -648,6 +669,16 @@ STBPE_VISIBLE int stbpe_vocab_loss_workspace(const stbpe_vocab_loss *args, int64
     const int st = plan(args, p, need, err, err_len);
     if (st == STBPE_OK && bytes) *bytes = need;
     return st;
+}
+
+STBPE_VISIBLE int stbpe_scale_gradients(void *a, int64_t n_a, void *b, int64_t n_b, const float *by, void *stream) {
+    if (n_a < 0 || n_b < 0 || (n_a && !a) || (n_b && !b) || !by || (uintptr_t)a % 16 || (uintptr_t)b % 16) return STBPE_E_BADARG;
+    const i64 most = n_a > n_b ? n_a : n_b;
+    if (most == 0) return STBPE_OK;
+    const i64 blocks = (most + 2047) / 2048;
+    scale_kernel<<<(unsigned)(blocks < SMS * 8 ? blocks : SMS * 8), 256, 0, (cudaStream_t)stream>>>(
+        (__nv_bfloat16 *)a, n_a, (__nv_bfloat16 *)b, n_b, by);
+    return cudaGetLastError() == cudaSuccess ? STBPE_OK : STBPE_E_CUDA;
 }
 
 STBPE_VISIBLE int stbpe_vocab_loss_run(const stbpe_vocab_loss *args, void *stream, char *err, size_t err_len) {

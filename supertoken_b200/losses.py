@@ -127,7 +127,7 @@ def _loss(hidden, weight, ids, logits, valid, temperature, reduction):
 
 
 def _grads(hidden, weight, ids, logits, valid, temperature, reduction, grad_loss, lse2, want_hidden=True, want_weight=True):
-    """(loss or None, grad_hidden or None, grad_weight or None); without ``lse2`` the loss is made, too."""
+    """(loss or None, grad_hidden or None, grad_weight or None, lse2); without ``lse2`` the loss is made, too."""
     a = _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
     dev, shape, loss = hidden.device, hidden.shape[:-1], None
     if grad_loss is not None:
@@ -153,17 +153,27 @@ def _grads(hidden, weight, ids, logits, valid, temperature, reduction, grad_loss
     a.lse2 = lse2.data_ptr()
     a.grad_hidden = gh.data_ptr() if want_hidden and gh.numel() else None
     a.grad_weight = gw.data_ptr() if want_weight else None
-    if a.grad_hidden or a.grad_weight:
+    if loss is not None or a.grad_hidden or a.grad_weight:
         _run(a, dev)
-    return loss, gh, gw
+    return loss, gh, gw, lse2
 
 
 class _VocabLoss(torch.autograd.Function):
+    """One loss for a batch in bfloat16 makes its gradients with it, three products instead of the four of a loss and a later
+    backward pass, which only multiplies them: exact for 1 and other powers of two, for other numbers one more rounding of the
+    result.  Where what comes down differs from row to row, in float16 (a loss scale has to come before the gradients' rounding)
+    and for a second backward pass, the gradients are made from the saved sums."""
+
     @staticmethod
     def forward(ctx, hidden, weight, ids, logits, valid, temperature, reduction):
-        loss, lse2 = _loss(hidden, weight, ids, logits, valid, temperature, reduction)
+        ctx.temperature, ctx.reduction, ctx.grads = temperature, reduction, None
+        if hidden.dtype == torch.bfloat16 and reduction != "none":
+            loss, gh, gw, lse2 = _grads(hidden, weight, ids, logits, valid, temperature, reduction, None, None,
+                                        ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+            ctx.grads = gh, gw
+        else:
+            loss, lse2 = _loss(hidden, weight, ids, logits, valid, temperature, reduction)
         ctx.save_for_backward(hidden, weight, ids, logits, valid, lse2)
-        ctx.temperature, ctx.reduction = temperature, reduction
         return loss
 
     @staticmethod
@@ -171,9 +181,22 @@ class _VocabLoss(torch.autograd.Function):
     def backward(ctx, grad_loss):
         hidden, weight, ids, logits, valid, lse2 = ctx.saved_tensors
         _refuse_capture(hidden.device)
-        _, gh, gw = _grads(hidden, weight, ids, logits, valid, ctx.temperature, ctx.reduction, grad_loss, lse2,
-                           ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        if ctx.grads is not None:
+            (gh, gw), ctx.grads = ctx.grads, None  # they are given away: a second pass makes its own
+            _scale(gh, gw, grad_loss)
+        else:
+            _, gh, gw, _ = _grads(hidden, weight, ids, logits, valid, ctx.temperature, ctx.reduction, grad_loss, lse2,
+                                  ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return gh, gw, None, None, None, None, None
+
+
+def _scale(gh: Optional[torch.Tensor], gw: Optional[torch.Tensor], by: torch.Tensor) -> None:
+    with torch.cuda.device(by.device):
+        st = L.load().stbpe_scale_gradients(gh.data_ptr() if gh is not None else None, gh.numel() if gh is not None else 0,
+                                            gw.data_ptr() if gw is not None else None, gw.numel() if gw is not None else 0,
+                                            by.data_ptr(), torch.cuda.current_stream(by.device).cuda_stream)
+    if st != L.OK:
+        _raise(st, f"stbpe_scale_gradients failed with status {st}")
 
 
 def _refuse_capture(device: torch.device) -> None:
@@ -196,7 +219,8 @@ def _differentiable(hidden, weight, ids, logits, valid, temperature, reduction):
 def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
                         valid: Optional[torch.Tensor] = None, *, reduction: str = "mean") -> torch.Tensor:
     """``-log softmax(hidden @ weight.T)[targets]`` in float32: a scalar, or one per row with ``reduction="none"``.
-    Differentiable in ``hidden`` and ``weight``; without gradients wanted it can be captured into a graph."""
+    Differentiable in ``hidden`` and ``weight``.  A reduced loss in bfloat16 makes its gradients at once, so score under
+    ``torch.no_grad()``; without gradients wanted the call can be captured into a graph."""
     return _differentiable(hidden, weight, targets, None, valid, 1.0, reduction)
 
 
@@ -207,15 +231,15 @@ def vocab_cross_entropy_grads(hidden: torch.Tensor, weight: torch.Tensor, target
     gradients are contiguous, in the inputs' type, and times ``grad_loss``: a number, a float32 tensor of one element (a loss
     scale), or with ``reduction="none"`` one of the loss's shape."""
     with torch.no_grad():
-        return _grads(hidden, weight, targets, None, valid, 1.0, reduction, grad_loss, None)
+        return _grads(hidden, weight, targets, None, valid, 1.0, reduction, grad_loss, None)[:3]
 
 
 def vocab_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
                        teacher_logits: torch.Tensor, valid: Optional[torch.Tensor] = None, *, temperature: float = 1.0,
                        reduction: str = "mean") -> torch.Tensor:
     """``T^2 KL(p || softmax(hidden @ weight.T / T))`` with ``p = softmax(teacher_logits / T)`` over the teacher's up to 256
-    entries of a row (in any order; an id below 0 is no entry, the same id twice counts twice).  Differentiable in
-    ``hidden`` and ``weight``; without gradients wanted it can be captured into a graph."""
+    entries of a row (in any order; an id below 0 is no entry, the same id twice counts twice).  Gradients and captures as with
+    ``vocab_cross_entropy``."""
     if teacher_logits is None:
         raise TypeError("teacher_logits must be a tensor")
     return _differentiable(hidden, weight, teacher_ids, teacher_logits, valid, float(temperature), reduction)
@@ -229,4 +253,4 @@ def vocab_distillation_grads(hidden: torch.Tensor, weight: torch.Tensor, teacher
     if teacher_logits is None:
         raise TypeError("teacher_logits must be a tensor")
     with torch.no_grad():
-        return _grads(hidden, weight, teacher_ids, teacher_logits, valid, float(temperature), reduction, grad_loss, None)
+        return _grads(hidden, weight, teacher_ids, teacher_logits, valid, float(temperature), reduction, grad_loss, None)[:3]

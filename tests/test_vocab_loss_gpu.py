@@ -9,7 +9,8 @@ for sums that truncate):
              largest |g T| at least
   gradients  sums of |dG| times the other factor, (terms) e of the sum of |G| times it, and u of the result's own rounding; in dW
              of the call that returns loss and gradients h times its row's factor is rounded to 16 bits, too:
-             G (1 + a) h (1 + b) with |a|, |b| <= u is off by at most (u + u + u^2) |G h|
+             G (1 + a) h (1 + b) with |a|, |b| <= u is off by at most (u + u + u^2) |G h|; what comes down through autograd may be
+             multiplied onto them once they are rounded, by at most u of the result again
 """
 import math
 
@@ -105,6 +106,8 @@ def check(hidden, weight, *args, valid=None, T=None, reduction="mean", grad=None
     auto = loss_of(h, w, *args, valid, reduction=reduction, **more)
     up = torch.ones_like(auto) if grad is None else torch.as_tensor(grad, device="cuda", dtype=torch.float32).expand_as(auto)
     ah, aw = torch.autograd.grad(auto, (h, w), up)
+    for name in ("gh", "gw"):
+        want[name + "_tol"] = want[name + "_tol"] * (1 + 2 ** -8) + torch.finfo(gh.dtype).eps / 2 * want[name].abs()
     near(auto.detach(), want, "loss"), near(ah, want, "gh"), near(aw, want, "gw")
     return loss, gh, gw
 
@@ -287,6 +290,21 @@ def test_gradients_against_differences(K):
     cubes = ((reach.amax(1) - reach.amin(1)) ** 3).sum() / 6
     tol = cubes + 2 * want["loss_tol"] + (want["gh_tol"] * step.double().abs()).sum()
     assert abs(float((hi - lo) / 2 - along)) <= float(tol) < 0.1 * abs(float(along))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_backward_twice(dtype):
+    """The second pass does not change what the first one gave."""
+    hidden, weight, targets = make(2, 150, 72, 700, dtype=dtype)
+    h, w = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+    loss = ops.vocab_cross_entropy(h, w, targets)
+    want = formula(hidden, weight, targets)
+    one = torch.autograd.grad(loss, (h, w), torch.tensor(1.0, device="cuda"), retain_graph=True)
+    kept = [x.clone() for x in one]
+    two = torch.autograd.grad(loss, (h, w), torch.tensor(4.0, device="cuda"))
+    assert all(torch.equal(x, y) for x, y in zip(one, kept))
+    for x, y in zip(one, two):
+        near(x, want, "gh" if x.dim() == 3 else "gw"), near(y / 4, want, "gh" if x.dim() == 3 else "gw")
 
 
 def test_only_the_wanted_gradient_is_made():
