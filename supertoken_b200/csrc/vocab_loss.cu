@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(128) teacher_kernel(Plan p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     u64 *e = sorted + (size_t)warp * p.k_sorted;
     for (i64 row = (i64)blockIdx.x * 4 + warp; row < p.rows; row += (i64)gridDim.x * 4) {
-        const i64 o = row / p.inner, i = row - o * p.inner;
+        const i64 o = (unsigned)row / (unsigned)p.inner, i = row - o * p.inner;
         const i64 id_at = o * p.ids_outer + i * p.ids_inner, real_at = o * p.logits_outer + i * p.logits_inner;
         // rounded before anything is taken from it: the maximum less itself has to be 0 at the type's lowest value, too
         auto softened = [&](i64 at) { return __fmul_rn(load_real(p.logits, p.logits_type, at), p.inv_temperature); };
@@ -130,27 +130,34 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
     __shared__ int base;
     __shared__ float part[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool each = p.want_grads && p.reduction == STBPE_REDUCE_NONE && p.grad_loss;
+    const float one = p.want_grads && p.grad_loss && !each && p.rows > 0 ? p.grad_loss[0] : 1.f;
+    float most = fabsf(one);
+    if (each) most = 0.f;
     if (threadIdx.x == 0) base = 0;
     if (p.split_done)
         for (int x = threadIdx.x; x < SMS * 8; x += 1024) p.split_done[x] = 0;
     for (i64 r0 = 0; r0 < p.rows; r0 += EACH * 1024) {
         bool counted[EACH];
         unsigned votes[EACH];
+        float nan[EACH], up[EACH];
 #pragma unroll
         for (int x = 0; x < EACH; ++x) {
             const i64 row = r0 + x * 1024 + threadIdx.x;
-            counted[x] = false;
+            counted[x] = false, up[x] = 1.f, nan[x] = 0.f;
             if (row < p.rows) {
-                const i64 o = row / p.inner, i = row - o * p.inner;
+                const i64 o = (unsigned)row / (unsigned)p.inner, i = row - o * p.inner;
                 counted[x] = !p.valid || p.valid[o * p.valid_outer + i * p.valid_inner];
+                if (each) up[x] = p.grad_loss[o * p.grad_outer + i * p.grad_inner];
                 if (p.k) {
                     counted[x] = counted[x] && p.has_entries[row];
+                    nan[x] = p.plogp[row] * 0.f;
                 } else {
                     const i64 id = load_id(p.ids, p.ids_bytes, o * p.ids_outer + i * p.ids_inner);
                     counted[x] = counted[x] && id >= 0;
-                    const bool outside = id >= p.vocab;
-                    p.entries[row] = make_int2(outside || id < 0 ? INT_MAX : (int)id, __float_as_int(1.f));
-                    p.plogp[row] = outside ? NAN : 0.f;
+                    nan[x] = id >= p.vocab ? NAN : 0.f;
+                    p.entries[row] = make_int2(id >= p.vocab || id < 0 ? INT_MAX : (int)id, __float_as_int(1.f));
+                    p.plogp[row] = nan[x];
                 }
             }
         }
@@ -187,8 +194,13 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
             const int slot = in_warp[x * 32 + warp] + __popc(votes[x] & ((1u << lane) - 1));
             if (row < p.rows) {
                 p.slot_of[row] = counted[x] ? slot : -1;
-                if (counted[x]) p.row_of[slot] = (int)row;
-                else if (p.want_loss) p.row_loss[row] = p.lse2[row] = 0.f;
+                if (counted[x]) {
+                    p.row_of[slot] = (int)row;
+                    if (p.want_grads) p.coef[slot] = up[x] + nan[x];
+                    if (each) most = fmaxf(most, fabsf(up[x]));
+                } else if (p.want_loss) {
+                    p.row_loss[row] = p.lse2[row] = 0.f;
+                }
             }
         }
     }
@@ -199,31 +211,21 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
         for (i64 c = threadIdx.x; c < p.rows_padded; c += 1024) p.reference[c] = 0.f;
         for (i64 c = threadIdx.x; c < p.rows_padded / TILE_ROWS; c += 1024) p.again[c] = 0;
     }
-    if (threadIdx.x == 0) p.meta->counted = n, p.meta->tickets = 0;
-    if (!p.want_grads) return;
-    const float factor = p.temperature / (p.reduction == STBPE_REDUCE_MEAN ? (float)(n > 0 ? n : 1) : 1.f);
-    const bool each = p.reduction == STBPE_REDUCE_NONE && p.grad_loss;
-    auto g = [&](i64 row) {
-        const i64 o = row / p.inner, i = row - o * p.inner;
-        return (!p.grad_loss ? 1.f : p.grad_loss[each ? o * p.grad_outer + i * p.grad_inner : 0]) * factor;
-    };
-    float most = fabsf(g(0) * (p.rows > 0));
     if (each) {
-        most = 0.f;
-        for (i64 c = threadIdx.x; c < n; c += 1024) most = fmaxf(most, fabsf(g(p.row_of[c])));
         for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
         if (lane == 0) part[warp] = most;
         __syncthreads();
         for (int w = 0; w < 32; ++w) most = fmaxf(most, part[w]);
     }
-    int up = 0;  // the next power of two, both sides kept within what 32 bits hold as normal numbers
-    if (most > 0.f && most < INFINITY) frexpf(most, &up);
-    up = max(-100, min(100, up));
-    const float in = ldexpf(1.f, 14 - up);
-    if (threadIdx.x == 0) p.meta->out_scale = ldexpf(1.f, up - 14);
-    for (i64 c = threadIdx.x; c < n; c += 1024) {
-        const int row = p.row_of[c];
-        p.coef[c] = isnan(p.plogp[row]) ? NAN : g(row) * in;
+    if (threadIdx.x == 0) {
+        const float factor = p.temperature / (p.reduction == STBPE_REDUCE_MEAN ? (float)(n > 0 ? n : 1) : 1.f);
+        most *= factor;
+        int up = 0;  // the next power of two, both sides kept within what 32 bits hold as normal numbers
+        if (most > 0.f && most < INFINITY) frexpf(most, &up);
+        up = max(-100, min(100, up));
+        p.meta->counted = n, p.meta->tickets = 0, p.meta->again = 0;
+        p.meta->in_scale = (each ? 1.f : one) * factor * ldexpf(1.f, 14 - up);
+        p.meta->out_scale = ldexpf(1.f, up - 14);
     }
 }
 
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(256) gather_kernel(Plan p) {
             else
                 for (int d = lane; d < p.dim; d += 32) to[d] = T(0.f);
         } else {
-            const i64 o = x / p.inner, i = x - o * p.inner;
+            const i64 o = (unsigned)x / (unsigned)p.inner, i = x - o * p.inner;
             const T *from = (const T *)p.hidden + o * p.hidden_outer + i * p.hidden_inner;
             if (p.hidden_aligned)
 #pragma unroll 4
@@ -281,67 +283,58 @@ __global__ void __launch_bounds__(256) unalign_weight_kernel(Plan p) {
 }
 
 // ---------------------------------------------------------------------------------------------- after the products
-// 32 rows of a chunk to a block: joins what the parts of the columns left, in a fixed order, to lse and the loss of a row.  Where E is
-// kept, the row's E gets its entries and the packed row its factor.  `again`: the tiles that were made a second time.
+// Eight rows of a chunk to a block: joins what the parts of the columns left, in a fixed order (eight threads read a sector, 32 parts
+// at a time), to lse and the loss of a row; then a warp has a row.  Where E is kept, the row's E gets its entries and the packed row its factor.
+// `again`: the tiles that were made a second time.
 template <class T>
 __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, bool again, unsigned int all_tickets) {
-    __shared__ float tops[8][32], sums[8][32], lse2s[32], refs[32];
+    __shared__ float tops[8][8], sums[8][8], lse2s[8], refs[8];
     __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const i64 counted = p.meta->counted;
     const i64 n = counted - r0 < 0 ? 0 : counted - r0 < rows ? counted - r0 : rows;
-    const i64 until = p.keep ? (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS : n;
+    const i64 until = again && !p.meta->again ? 0 : p.keep ? (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS : n;
     const int entries_of_row = p.k ? p.k : 1;
     const float scale = p.inv_temperature * 1.4426950408889634f;
-    for (i64 m0 = (i64)blockIdx.x * 32; m0 < until; m0 += (i64)gridDim.x * 32) {
+    for (i64 m0 = (i64)blockIdx.x * 8; m0 < until; m0 += (i64)gridDim.x * 8) {
         if (again && !p.again[(r0 + m0) / TILE_ROWS]) continue;
         float top = LOWEST, sum = 0.f;
-        if (m0 + lane < n) {
-            const float *from_max = p.part_max + m0 + lane, *from_sum = p.part_sum + m0 + lane;
-            if (p.keep) {  // all parts have the row's reference
+        auto add = [&](float m, float x) {
+            const float both = fmaxf(top, m);
+            // (all parts of a row of E have the row's reference)
+            sum = p.keep ? sum + x : sum * exp2f(top - both) + x * exp2f(m - both);
+            top = both;
+        };
+        if (m0 + (lane & 7) < n) {
+            const float *from_max = p.part_max + m0 + (lane & 7), *from_sum = p.part_sum + m0 + (lane & 7);
 #pragma unroll 4
-                for (int t = warp; t < p.parts; t += 8) {
-                    top = fmaxf(top, from_max[t * p.part_stride]);
-                    sum += from_sum[t * p.part_stride];
-                }
-            } else {
-#pragma unroll 4
-                for (int t = warp; t < p.parts; t += 8) {
-                    const float m = from_max[t * p.part_stride], x = from_sum[t * p.part_stride], both = fmaxf(top, m);
-                    sum = sum * exp2f(top - both) + x * exp2f(m - both);
-                    top = both;
-                }
-            }
+            for (int t = warp * 4 + (lane >> 3); t < p.parts; t += 32) add(from_max[t * p.part_stride], from_sum[t * p.part_stride]);
         }
-        tops[warp][lane] = top, sums[warp][lane] = sum;
+        for (int d = 8; d < 32; d <<= 1) {
+            const float m = __shfl_xor_sync(~0u, top, d), x = __shfl_xor_sync(~0u, sum, d);
+            add(m, x);
+        }
+        if (lane < 8) tops[warp][lane] = top, sums[warp][lane] = sum;
         __syncthreads();
-        if (warp == 0) {
-            for (int w = 1; w < 8; ++w) {
-                const float m = tops[w][lane], x = sums[w][lane], both = fmaxf(top, m);
-                sum = p.keep ? sum + x : sum * exp2f(top - both) + x * exp2f(m - both);
-                top = both;
-            }
+        if (threadIdx.x < 8) {
+            top = tops[0][lane], sum = sums[0][lane];
+            for (int w = 1; w < 8; ++w) add(tops[w][lane], sums[w][lane]);
             float ref = top;
             if (p.keep && m0 + lane < n) {
                 ref = p.reference[r0 + m0 + lane];
                 if (!again && fabsf(top - ref) > 96.f && fabsf(top) < INFINITY) {
                     p.reference[r0 + m0 + lane] = top;
-                    p.again[(r0 + m0) / TILE_ROWS] = 1;
+                    p.again[(r0 + m0) / TILE_ROWS] = p.meta->again = 1;
                 }
             }
             refs[lane] = ref, lse2s[lane] = ref + log2f(sum);
         }
         __syncthreads();
-        for (int y = warp; y < 32; y += 8) {
-            const i64 m = m0 + y, slot = r0 + m;
-            if (m >= until) break;
-            T *scaled = (T *)p.scaled + m * p.dim_padded;
-            if (m >= n) {  // (keep) zeros behind the last row
-                for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)(scaled + d) = make_uint4(0, 0, 0, 0);
-                continue;
-            }
+        const i64 m = m0 + warp, slot = r0 + m;
+        T *scaled = (T *)p.scaled + m * p.dim_padded;
+        if (m < n) {
             const int row = p.row_of[slot];
-            const float lse2 = lse2s[y], ref = refs[y];
+            const float lse2 = lse2s[warp], ref = refs[warp];
             const float less = exp2f(lse2 - ref);  // keep: a share in the units of E
             const int2 *e = p.entries + (i64)row * entries_of_row;
             const float *z = p.entry_z + slot * entries_of_row;
@@ -363,7 +356,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
                 p.row_loss[row] = tau * tau * (lse2 * 0.69314718055994531f + p.plogp[row] - pz * p.inv_temperature);
             }
             if (p.keep) {
-                const float a = p.coef[slot] * exp2f(ref - lse2);
+                const float a = p.coef[slot] * p.meta->in_scale * exp2f(ref - lse2);
                 if (lane == 0) p.out_row[slot] = a * p.meta->out_scale;
                 const T *from = (const T *)p.packed + slot * p.dim_padded;
 #pragma unroll 4
@@ -375,6 +368,8 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
                     *(uint4 *)(scaled + d) = x;
                 }
             }
+        } else if (p.keep && m < until) {  // zeros behind the last row
+            for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)(scaled + d) = make_uint4(0, 0, 0, 0);
         }
         __syncthreads();
     }
@@ -447,9 +442,23 @@ int fail(char *err, size_t len, int status, const char *what, const char *why) {
 
 i64 up_to(i64 x, i64 unit) { return (x + unit - 1) / unit * unit; }
 
-// CTAs to a tile of a product.  Pairs on 256 x 256 make 1.6 times as much per SM as single CTAs on 128 x 128, so they are worth it
-// unless the tiles are so few that single CTAs are through in one round, while pairs would leave half of the SMs idle.
-int group_of(i64 rows, i64 cols) { return ((rows + 255) / 256) * ((cols + 255) / 256) <= SMS / 4 ? 1 : 2; }
+// CTAs to a tile of a product: rounds of all SMs (part of one where the last round's tiles are split in depth) times what a tile
+// costs, 1 for 256 x 256 by a pair and 0.8 for 128 x 128 by a single CTA, a quarter of it with twice as many at a time (0.95 against
+// 1.5 PFLOP/s).  Single CTAs win where pairs would leave more than half of the SMs idle.
+int group_of(i64 rows, i64 cols, i64 depth = 0, bool may_split = false) {
+    double cost[3];
+    for (int g = 1; g <= 2; ++g) {
+        const i64 side = 128 * g, tiles = ((rows + side - 1) / side) * ((cols + side - 1) / side), clusters = SMS / g, left = tiles % clusters;
+        i64 splits = 1;
+        if (may_split && left) {
+            splits = clusters / left < SPLITS ? clusters / left : SPLITS;
+            if (splits > depth / 64 / 8) splits = depth / 64 / 8;
+            if (splits < 1) splits = 1;
+        }
+        cost[g] = ((double)(tiles / clusters) + (left ? 1. / (double)splits : 0.)) * (g == 2 ? 1. : 0.8);
+    }
+    return cost[1] < cost[2] ? 1 : 2;
+}
 
 // Checks the arguments and lays the workspace out; `bytes` gets its size.
 int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_len) {
@@ -592,7 +601,8 @@ template <class T, int KIND>
 int product(const Plan &p, const Job &job, const CUtensorMap &a, const CUtensorMap &b, cudaStream_t s, char *err, size_t err_len) {
     const i64 rows = KIND == GRAD_WEIGHT ? job.width : p.rows < job.rows ? p.rows : job.rows, cols = KIND <= MAKE_G ? job.width : p.dim;
     if (rows == 0) return STBPE_OK;
-    const int group = KIND <= MAKE_G ? p.group : group_of(rows, cols);  // (the parts of the columns go by p.group)
+    // (the parts of the columns go by p.group)
+    const int group = KIND <= MAKE_G ? p.group : group_of(rows, cols, KIND == GRAD_HIDDEN ? job.width : p.rows, KIND == GRAD_HIDDEN ? !p.acc : !p.weight_acc);
     const i64 tile = 128 * group, tiles = ((rows + tile - 1) / tile) * ((cols + tile - 1) / tile) * (KIND <= MAKE_G ? 1 : SPLITS);
     return group == 1 ? launch<T, KIND, 1>(p, job, a, b, tiles, s, err, err_len) : launch<T, KIND, 2>(p, job, a, b, tiles, s, err, err_len);
 }
@@ -623,7 +633,7 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
         VTRY(map(&g, p.g, p.chunk_rows, p.g_stride, p.g_stride, 128));
         VTRY(map(&g_across, p.g, p.chunk_rows, p.g_stride, p.g_stride, 64));
     }
-    const unsigned joins = blocks(p.chunk_rows, 32);
+    const unsigned joins = blocks(p.chunk_rows, 8);
     if (p.keep) {
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
             const unsigned tickets = joins * (unsigned)((p.rows_padded + p.chunk_rows - 1) / p.chunk_rows);

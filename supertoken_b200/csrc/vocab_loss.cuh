@@ -18,7 +18,9 @@ constexpr int TILE_ROWS = 256;  // packed rows are filled up with zeros to this 
 struct Meta {
     int counted;          // rows that count
     unsigned int tickets; // blocks that are through with their rows' losses
+    float in_scale;       // what coef is multiplied by in the end
     float out_scale;      // what both gradients are multiplied by in the end
+    int again;            // keep: a reference was too far from its row's maximum
 };
 
 struct Plan {
@@ -49,7 +51,7 @@ struct Plan {
     i64 weight_rows_stride;
     float *part_max, *part_sum, *row_loss;  // [part][packed row of the chunk]; per row
     i64 part_stride;
-    float *coef;             // what a packed row of dlogits is multiplied by
+    float *coef;             // what a packed row of dlogits is multiplied by, and in_scale
     // G (16 bits) of one piece of the vocabulary and all packed rows; or E = exp2(logits - reference) of the whole
     // vocabulary and a chunk of the packed rows (keep)
     bool keep;

@@ -69,10 +69,10 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
     for (;;) {
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(done)
-            : "r"(bar), "r"(parity)
+            : "r"(bar), "r"(parity), "r"(100000)  // ns that the hardware may sleep at a time
             : "memory");
         if (done) return true;
         u64 now;
@@ -248,7 +248,8 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
     const i64 depth = LOGITS ? p.dim : KIND == GRAD_HIDDEN ? job.width : n;
     const i64 tiles_m = (rows + TILE - 1) / TILE, tiles_n = (cols + TILE - 1) / TILE;
     const int steps = (int)((depth + 63) / 64);
-    const i64 tiles = KIND == GRAD_WEIGHT && job.r0 > 0 && n == 0 ? 0 : tiles_m * tiles_n;
+    const bool nothing = KIND == GRAD_WEIGHT ? job.r0 > 0 && n == 0 : KIND == MAKE_E && job.again && !p.meta->again;
+    const i64 tiles = nothing ? 0 : tiles_m * tiles_n;
     const i64 cluster = blockIdx.x / GROUP, clusters = gridDim.x / GROUP;
     // The tiles behind the last full round of all clusters are split in depth, so that the round that is not full is shorter, too:
     // up to SPLITS units per tile of eight steps at least.
@@ -261,8 +262,11 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
         if (splits < 1) splits = 1;
     }
     const i64 whole = tiles - left, units = whole + left * splits;
-    // a band of BAND tiles of rows goes through all columns, its rows first: that much of A stays in L2
-    constexpr i64 BAND = 16;
+    // A band of tiles of rows goes through all columns, its rows first.  LOGITS: that much of H stays in L2 while W passes by.  Else the
+    // tiles that are being made at a time are as many columns as there are, or a square where both operands pass by, so that
+    // they share what comes from memory (8 188 x 32 256 x 2 048: 1.0 and 0.6 GB read instead of 1.7 with bands of 16).
+    const i64 high_band = LOGITS ? 16 : (clusters + tiles_n - 1) / (tiles_n > 0 ? tiles_n : 1);
+    const i64 BAND = KIND == GRAD_HIDDEN && high_band < 8 * 2 / GROUP ? 8 * 2 / GROUP : high_band;
     struct Unit {
         i64 m0, n0;
         int k0, k1, split, index;  // steps; number of the split tile
@@ -383,7 +387,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                 if (row >= 0 && job.v0 + c0 < p.vocab) walk.start(p, row, job.v0 + c0);
                 else walk.next.x = INT_MAX, walk.at = walk.all = 0;
                 if (KIND == MAKE_E && row >= 0) shift = p.reference[slot];
-                if (KIND == MAKE_G && row >= 0) shift = p.lse2[row], coef = p.coef[slot];
+                if (KIND == MAKE_G && row >= 0) shift = p.lse2[row], coef = p.coef[slot] * p.meta->in_scale;
             }
             if (KIND == GRAD_HIDDEN && m < n) {
                 row = p.row_of[slot];
