@@ -120,13 +120,39 @@ __global__ void __launch_bounds__(128) teacher_kernel(Plan p) {
     }
 }
 
-// One CTA: which rows count, in their order (row_of, slot_of); the entry of a cross entropy row; what each counted row's dlogits are
-// multiplied by.  dlogits are held in the inputs' 16-bit type, so they are brought into that type's range: the largest |g_i T|
+// 16-bit numbers of one row by one warp: 16, 4 or 2 bytes at a time as both rows allow, zeros from `inside` up to `all`.
+template <class T>
+__device__ __forceinline__ void copy_row(T *to, const T *from, i64 inside, i64 all, int lane) {
+    const uintptr_t at = (uintptr_t)to | (uintptr_t)from;
+    if (at % 16 == 0 && inside % 8 == 0 && all == inside) {
+#pragma unroll 4
+        for (i64 d = lane * 8; d < inside; d += 256) *(uint4 *)(to + d) = *(const uint4 *)(from + d);
+    } else if (at % 4 == 0) {
+#pragma unroll 8
+        for (i64 d = lane * 2; d < all; d += 64) {
+            const uint32_t both = d + 1 < inside ? *(const uint32_t *)(from + d) : d < inside ? *(const unsigned short *)(from + d) : 0u;
+            if (d + 1 < all) *(uint32_t *)(to + d) = both;
+            else *(unsigned short *)(to + d) = (unsigned short)both;
+        }
+    } else {
+#pragma unroll 8
+        for (i64 d = lane; d < all; d += 32) to[d] = d < inside ? from[d] : T(0.f);
+    }
+}
+
+// Which rows count, in their order (row_of, slot_of); the entry of a cross entropy row; what each counted row's dlogits are
+// multiplied by.  Every block goes through all rows by itself, 8 192 at a time, so that no launch lies between their numbers and
+// what follows; the first one writes them down.
+// Then counted rows of `hidden` go one behind another, zeros up to the end of the last tile, a warp to a row: products then do no
+// work for padding, never multiply what a masked row holds (it may be NaN), and may read rows of any stride or alignment.  The
+// rows of dH that do not count get their zeros here.
+// dlogits are held in the inputs' 16-bit type, so they are brought into that type's range: the largest |g_i T|
 // becomes up to 2^14 (by a power of two, so bf16 loses nothing; fp16 keeps shares down to 2^-28 at full precision and its
 // entries stay below 2^15), and both gradients are scaled back in 32 bits.
+template <class T>
 __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
     constexpr int EACH = 8;  // rows of a thread, 1024 apart: their loads are in flight together
-    __shared__ int in_warp[EACH * 32];
+    __shared__ int in_warp[EACH * 32], slots[EACH * 1024];
     __shared__ int base;
     __shared__ float part[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -135,7 +161,8 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
     float most = fabsf(one);
     if (each) most = 0.f;
     if (threadIdx.x == 0) base = 0;
-    if (p.split_done)
+    const bool first = blockIdx.x == 0;
+    if (first && p.split_done)
         for (int x = threadIdx.x; x < SMS * 8; x += 1024) p.split_done[x] = 0;
     for (i64 r0 = 0; r0 < p.rows; r0 += EACH * 1024) {
         bool counted[EACH];
@@ -156,8 +183,8 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
                     const i64 id = load_id(p.ids, p.ids_bytes, o * p.ids_outer + i * p.ids_inner);
                     counted[x] = counted[x] && id >= 0;
                     nan[x] = id >= p.vocab ? NAN : 0.f;
-                    p.entries[row] = make_int2(id >= p.vocab || id < 0 ? INT_MAX : (int)id, __float_as_int(1.f));
-                    p.plogp[row] = nan[x];
+                    if (first) p.entries[row] = make_int2(id >= p.vocab || id < 0 ? INT_MAX : (int)id, __float_as_int(1.f));
+                    if (first) p.plogp[row] = nan[x];
                 }
             }
         }
@@ -192,7 +219,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
         for (int x = 0; x < EACH; ++x) {
             const i64 row = r0 + x * 1024 + threadIdx.x;
             const int slot = in_warp[x * 32 + warp] + __popc(votes[x] & ((1u << lane) - 1));
-            if (row < p.rows) {
+            if (row < p.rows && first) {
                 p.slot_of[row] = counted[x] ? slot : -1;
                 if (counted[x]) {
                     p.row_of[slot] = (int)row;
@@ -202,10 +229,33 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
                     p.row_loss[row] = p.lse2[row] = 0.f;
                 }
             }
+            slots[x * 1024 + threadIdx.x] = counted[x] ? slot : -1;
+        }
+        __syncthreads();
+        // every gridDim.x-th row is this block's, one at a time to a warp
+        const i64 end = p.rows - r0 < EACH * 1024 ? p.rows - r0 : EACH * 1024;
+        for (i64 y = blockIdx.x + (i64)warp * gridDim.x; y < end; y += (i64)gridDim.x * 32) {
+            const i64 its = r0 + y;
+            const int to = slots[y];
+            if (to >= 0) {
+                const i64 o = (unsigned)its / (unsigned)p.inner, i = its - o * p.inner;
+                copy_row((T *)p.packed + (i64)to * p.dim_padded, (const T *)p.hidden + o * p.hidden_outer + i * p.hidden_inner, p.dim,
+                         p.dim_padded, lane);
+            } else if (p.grad_hidden) {
+                T *at = (T *)p.grad_hidden + its * p.dim;
+                if (p.dim % 8 == 0)
+                    for (int d = lane * 8; d < p.dim; d += 256) *(uint4 *)(at + d) = make_uint4(0, 0, 0, 0);
+                else
+                    for (int d = lane; d < p.dim; d += 32) at[d] = T(0.f);
+            }
         }
     }
     __syncthreads();
     const int n = base;
+    const i64 until = (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS;
+    for (i64 c = n + blockIdx.x * 32 + warp; c < until; c += gridDim.x * 32)
+        for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)((T *)p.packed + c * p.dim_padded + d) = make_uint4(0, 0, 0, 0);
+    if (!first) return;
     for (i64 c = n + threadIdx.x; c < p.rows_padded; c += 1024) p.row_of[c] = -1;
     if (p.keep) {
         for (i64 c = threadIdx.x; c < p.rows_padded; c += 1024) p.reference[c] = 0.f;
@@ -229,45 +279,12 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
     }
 }
 
-// Counted rows of `hidden` one behind another, zeros up to the end of the last tile: products then do no work for
-// padding, never multiply what a masked row holds (it may be NaN), and may read rows of any stride or alignment.  The rows of dH that do
-// not count get their zeros here.
-template <class T>
-__global__ void __launch_bounds__(256) gather_kernel(Plan p) {
-    const int lane = threadIdx.x & 31;
-    const i64 n = p.meta->counted, until = (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS;
-    for (i64 x = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); x < p.rows + until - n; x += (i64)gridDim.x * 8) {
-        const i64 slot = x < p.rows ? p.slot_of[x] : n + x - p.rows;
-        T *to = (T *)p.packed + slot * p.dim_padded;
-        if (x >= p.rows) {
-            for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)(to + d) = make_uint4(0, 0, 0, 0);
-        } else if (slot < 0) {
-            if (!p.grad_hidden) continue;
-            to = (T *)p.grad_hidden + x * p.dim;
-            if (p.dim % 8 == 0)
-                for (int d = lane * 8; d < p.dim; d += 256) *(uint4 *)(to + d) = make_uint4(0, 0, 0, 0);
-            else
-                for (int d = lane; d < p.dim; d += 32) to[d] = T(0.f);
-        } else {
-            const i64 o = (unsigned)x / (unsigned)p.inner, i = x - o * p.inner;
-            const T *from = (const T *)p.hidden + o * p.hidden_outer + i * p.hidden_inner;
-            if (p.hidden_aligned)
-#pragma unroll 4
-                for (int d = lane * 8; d < p.dim; d += 256) *(uint4 *)(to + d) = *(const uint4 *)(from + d);
-            else
-#pragma unroll 4
-                for (int d = lane; d < p.dim_padded; d += 32) to[d] = d < p.dim ? from[d] : T(0.f);
-        }
-    }
-}
-
 // A weight whose rows do not start on 16-byte boundaries, copied so that they do.
 template <class T>
 __global__ void __launch_bounds__(256) align_weight_kernel(Plan p, T *to) {
     const int lane = threadIdx.x & 31;
     for (i64 j = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); j < p.vocab; j += (i64)gridDim.x * 8) {
-        const T *from = (const T *)p.weight + j * p.weight_stride;
-        for (int d = lane; d < p.dim_padded; d += 32) to[j * p.dim_padded + d] = d < p.dim ? from[d] : T(0.f);
+        copy_row(to + j * p.dim_padded, (const T *)p.weight + j * p.weight_stride, p.dim, p.dim_padded, lane);
     }
 }
 
@@ -276,9 +293,7 @@ template <class T>
 __global__ void __launch_bounds__(256) unalign_weight_kernel(Plan p) {
     const int lane = threadIdx.x & 31;
     for (i64 j = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); j < p.vocab; j += (i64)gridDim.x * 8) {
-        const T *from = (const T *)p.weight_out + j * p.weight_out_stride;
-#pragma unroll 4
-        for (int d = lane; d < p.dim; d += 32) ((T *)p.grad_weight)[j * p.dim + d] = from[d];
+        copy_row((T *)p.grad_weight + j * p.dim, (const T *)p.weight_out + j * p.weight_out_stride, p.dim, p.dim, lane);
     }
 }
 
@@ -487,7 +502,6 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     p.reduction = a->reduction;
     p.want_loss = (a->want & STBPE_WANT_LOSS) != 0, p.want_grads = (a->want & STBPE_WANT_GRADS) != 0;
     p.hidden = a->hidden, p.hidden_outer = a->hidden_outer, p.hidden_inner = a->hidden_inner;
-    p.hidden_aligned = (uintptr_t)a->hidden % 16 == 0 && a->hidden_outer % 8 == 0 && a->hidden_inner % 8 == 0 && a->dim % 8 == 0;
     p.weight = a->weight, p.weight_stride = a->weight_stride;
     p.ids = a->ids, p.ids_bytes = a->ids_bytes, p.ids_outer = a->ids_outer, p.ids_inner = a->ids_inner;
     p.logits = a->logits, p.logits_type = a->logits_type, p.logits_outer = a->logits_outer, p.logits_inner = a->logits_inner;
@@ -531,6 +545,7 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     }
     p.packed = take(p.rows_padded * p.dim_padded * 2);
     p.weight_rows = aligned ? a->weight : take(p.vocab * p.dim_padded * 2);
+    if (!p.lse2) p.lse2 = (float *)take(p.rows_padded * 4);
     if (p.want_loss) {
         p.entry_z = (float *)take(p.rows_padded * 4 * (p.k ? p.k : 1));
         p.part_max = (float *)take(p.chunk_rows * 4 * p.parts);
@@ -621,8 +636,7 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
         return tensor_map(m, type, at, rows, cols, stride, box, err, err_len);
     };
     if (p.k) teacher_kernel<<<blocks(p.rows, 4), 128, 4 * p.k_sorted * sizeof(u64), s>>>(p);
-    rows_kernel<<<1, 1024, 0, s>>>(p);
-    gather_kernel<T><<<blocks(p.rows + TILE_ROWS, 8), 256, 0, s>>>(p);
+    rows_kernel<T><<<p.rows + TILE_ROWS <= 16 * SMS ? (unsigned)(p.rows + TILE_ROWS) / 16 : (unsigned)SMS, 1024, 0, s>>>(p);
     if (p.weight_rows != p.weight) align_weight_kernel<T><<<blocks(p.vocab, 8), 256, 0, s>>>(p, (T *)p.weight_rows);
     CUtensorMap h, w, h_across, w_across, g, g_across;
     VTRY(map(&h, p.packed, p.rows_padded, p.dim, p.dim_padded, 128));
@@ -699,7 +713,7 @@ STBPE_VISIBLE int stbpe_vocab_loss_run(const stbpe_vocab_loss *args, void *strea
     if (st != STBPE_OK) return st;
     if (!args->workspace || (uintptr_t)args->workspace % 1024 || args->workspace_bytes < need)
         return fail(err, err_len, STBPE_E_CAPACITY, "stbpe_vocab_loss", "workspace missing, not on a 1024-byte boundary or too small");
-    if (!args->lse2 || (p.want_loss && !args->loss) || (p.want_grads && !args->grad_hidden && !args->grad_weight))
+    if ((!p.want_loss && !args->lse2) || (p.want_loss && !args->loss) || (p.want_grads && p.rows && !args->grad_hidden && !args->grad_weight))
         return fail(err, err_len, STBPE_E_BADARG, "stbpe_vocab_loss", "an output is missing");
     if ((uintptr_t)args->grad_hidden % 16 || (uintptr_t)args->grad_weight % 16)
         return fail(err, err_len, STBPE_E_BADARG, "stbpe_vocab_loss", "gradients start on 16-byte boundaries");

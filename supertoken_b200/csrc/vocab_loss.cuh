@@ -27,7 +27,7 @@ struct Plan {
     i64 rows, inner;  // row = outer * inner + inner index
     i64 vocab, dim, dim_padded, rows_padded;
     int k, k_sorted, pieces, parts, reduction, group;
-    bool want_loss, want_grads, hidden_aligned;
+    bool want_loss, want_grads;
     float temperature, inv_temperature;
     const void *hidden, *weight, *ids, *logits;
     const unsigned char *valid;

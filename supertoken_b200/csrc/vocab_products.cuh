@@ -165,14 +165,17 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
     return *(uint32_t *)&v;
 }
 
-// 32 values of one row, 16 bits each; `inside`: how many of them there are
+// 32 values of one row, 16 bits each; `inside`: how many of them there are; `unit`: how many may be stored at a time, 8, 2 or 1
 template <class T>
-__device__ __forceinline__ void store_row(T *to, const float (&v)[32], i64 inside, bool aligned) {
-    if (aligned && inside >= 32) {
+__device__ __forceinline__ void store_row(T *to, const float (&v)[32], i64 inside, int unit) {
+    if (unit == 8 && inside >= 32) {
 #pragma unroll
         for (int x = 0; x < 32; x += 8)
             *(uint4 *)(to + x) = make_uint4(pack2<T>(v[x], v[x + 1]), pack2<T>(v[x + 2], v[x + 3]), pack2<T>(v[x + 4], v[x + 5]),
                                             pack2<T>(v[x + 6], v[x + 7]));
+    } else if (unit >= 2 && inside >= 32) {
+#pragma unroll
+        for (int x = 0; x < 32; x += 2) *(uint32_t *)(to + x) = pack2<T>(v[x], v[x + 1]);
     } else {
 #pragma unroll
         for (int x = 0; x < 32; ++x)
@@ -401,7 +404,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     if (!p.acc) {
 #pragma unroll
                         for (int x = 0; x < 32; ++x) v[x] *= coef;
-                        store_row((T *)p.grad_hidden + (i64)row * p.dim + c0 + c, v, p.dim - c0 - c, p.dim % 8 == 0);
+                        store_row((T *)p.grad_hidden + (i64)row * p.dim + c0 + c, v, p.dim - c0 - c, p.dim % 8 == 0 ? 8 : p.dim % 2 == 0 ? 2 : 1);
                     } else {
                         float4 *to = (float4 *)(p.acc + m * p.acc_stride + c0 + c);
 #pragma unroll
@@ -430,7 +433,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     if (last) {
 #pragma unroll
                         for (int x = 0; x < 32; ++x) v[x] *= coef;
-                        store_row((T *)p.weight_out + id * p.weight_out_stride + c0 + c, v, p.dim - c0 - c, true);
+                        store_row((T *)p.weight_out + id * p.weight_out_stride + c0 + c, v, p.dim - c0 - c, 8);
                     } else {
 #pragma unroll
                         for (int x = 0; x < 8; ++x) to[x] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
@@ -519,7 +522,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     }
                 }
                 if (KIND == MAKE_E || KIND == MAKE_G) {
-                    if (m < p.chunk_rows && c0 + c < p.g_stride) store_row((T *)p.g + m * p.g_stride + c0 + c, v, 32, true);
+                    if (m < p.chunk_rows && c0 + c < p.g_stride) store_row((T *)p.g + m * p.g_stride + c0 + c, v, 32, 8);
                 }
             }
             if ((KIND == STATS || KIND == MAKE_E) && row >= 0 && job.v0 + c0 < p.vocab) {
@@ -543,10 +546,19 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     for (int c = 0; c < COLUMNS; c += 32) {
                         float v[32];
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) v[x] = __ldcg(sums + (c + x) * 32);
-                        for (int s = 1; s < splits; ++s)
+                        for (int x0 = 0; x0 < 32; x0 += 8) {  // eight columns of all splits on their way at a time
+                            float y[SPLITS][8];
 #pragma unroll
-                            for (int x = 0; x < 32; ++x) v[x] += __ldcg(sums + s * next + (c + x) * 32);
+                            for (int s = 0; s < SPLITS; ++s)
+#pragma unroll
+                                for (int x = 0; x < 8; ++x) y[s][x] = s < splits ? __ldcg(sums + s * next + (c + x0 + x) * 32) : 0.f;
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) {
+                                v[x0 + x] = y[0][x];
+#pragma unroll
+                                for (int s = 1; s < SPLITS; ++s) v[x0 + x] += y[s][x];
+                            }
+                        }
                         emit(c, v);
                     }
                 }

@@ -97,43 +97,41 @@ def _arguments(hidden, weight, ids, logits, valid, temperature, reduction) -> L.
 
 
 def _run(a: L.VocabLoss, device: torch.device) -> None:
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _run(a, device)
     lib, need, err = L.load(), ctypes.c_int64(0), ctypes.create_string_buffer(256)
-    with torch.cuda.device(device):
-        st = lib.stbpe_vocab_loss_workspace(ctypes.byref(a), ctypes.byref(need), err, 256)
-        if st == L.OK:
-            # torch's allocator knows streams and captures: a graph's workspace is in the graph's own pool
-            space = torch.empty(need.value + 1024, dtype=torch.uint8, device=device)
-            a.workspace, a.workspace_bytes = (space.data_ptr() + 1023) // 1024 * 1024, need.value
-            stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-            st = lib.stbpe_vocab_loss_run(ctypes.byref(a), stream, err, 256)
+    st = lib.stbpe_vocab_loss_workspace(ctypes.byref(a), ctypes.byref(need), err, 256)
+    if st == L.OK:
+        # torch's allocator knows streams and captures: a graph's workspace is in the graph's own pool
+        space = torch.empty(need.value + 1024, dtype=torch.uint8, device=device)
+        a.workspace, a.workspace_bytes = (space.data_ptr() + 1023) // 1024 * 1024, need.value
+        st = lib.stbpe_vocab_loss_run(ctypes.byref(a), torch.cuda.current_stream(device).cuda_stream, err, 256)
     if st != L.OK:
         _raise(st, err.value.decode())
 
 
-def _loss(hidden, weight, ids, logits, valid, temperature, reduction):
+def _loss(hidden, weight, ids, logits, valid, temperature, reduction, for_backward=False):
     """The loss, and what the gradients need of it again."""
     a = _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
     shape = hidden.shape[:-1]
-    loss = torch.empty(shape if reduction == "none" else (), dtype=torch.float32, device=hidden.device)
-    lse2 = torch.empty(shape, dtype=torch.float32, device=hidden.device)
-    a.want, a.loss, a.lse2 = _WANT_LOSS, loss.data_ptr(), lse2.data_ptr()
-    if a.outer * a.inner == 0 and reduction == "none":
-        return loss, lse2
-    if lse2.numel() == 0:
-        lse2 = lse2.new_empty(1)  # no address without an element
-        a.lse2 = lse2.data_ptr()
-    _run(a, hidden.device)
+    loss = hidden.new_empty(shape if reduction == "none" else (), dtype=torch.float32)
+    lse2 = hidden.new_empty(max(1, a.outer * a.inner), dtype=torch.float32) if for_backward else None
+    a.want, a.loss, a.lse2 = _WANT_LOSS, loss.data_ptr(), lse2.data_ptr() if for_backward else None
+    if loss.numel():
+        _run(a, hidden.device)
     return loss, lse2
 
 
-def _grads(hidden, weight, ids, logits, valid, temperature, reduction, grad_loss, lse2, want_hidden=True, want_weight=True):
-    """(loss or None, grad_hidden or None, grad_weight or None, lse2); without ``lse2`` the loss is made, too."""
+def _grads(hidden, weight, ids, logits, valid, temperature, reduction, grad_loss, lse2, want_hidden=True, want_weight=True,
+           for_backward=False):
+    """(loss or None, grad_hidden or None, grad_weight or None, lse2 or None); without ``lse2`` the loss is made, too."""
     a = _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
-    dev, shape, loss = hidden.device, hidden.shape[:-1], None
+    shape, loss = hidden.shape[:-1], None
     if grad_loss is not None:
         if not isinstance(grad_loss, torch.Tensor):
-            grad_loss = torch.full((), float(grad_loss), dtype=torch.float32, device=dev)
-        if grad_loss.device != dev:
+            grad_loss = torch.full((), float(grad_loss), dtype=torch.float32, device=hidden.device)
+        if grad_loss.device != hidden.device:
             raise ValueError("tensors must be on one device")
         if grad_loss.dtype != torch.float32:
             raise TypeError("grad_loss must be float32")
@@ -142,19 +140,20 @@ def _grads(hidden, weight, ids, logits, valid, temperature, reduction, grad_loss
         elif grad_loss.numel() != 1:
             raise ValueError("grad_loss must have one element, or the shape of the loss")
         a.grad_loss = grad_loss.data_ptr()
+    gh = hidden.new_empty(hidden.shape) if want_hidden else None
+    gw = weight.new_empty(weight.shape) if want_weight else None
     a.want = _WANT_GRADS
     if lse2 is None:
-        loss = torch.empty(shape if reduction == "none" else (), dtype=torch.float32, device=dev)
-        lse2 = torch.empty(max(1, a.outer * a.inner), dtype=torch.float32, device=dev)
-        # (a tensor without elements has no address)
-        a.want, a.loss = _WANT_LOSS | _WANT_GRADS, (loss if loss.numel() else lse2).data_ptr()
-    gh = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if want_hidden else None
-    gw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want_weight else None
-    a.lse2 = lse2.data_ptr()
+        loss = hidden.new_empty(shape if reduction == "none" else (), dtype=torch.float32)
+        if for_backward:
+            lse2 = hidden.new_empty(max(1, a.outer * a.inner), dtype=torch.float32)
+        # (a tensor without elements has no address, and nothing is written to where it would be)
+        a.want, a.loss = _WANT_LOSS | _WANT_GRADS, (loss if loss.numel() else gw if gw is not None else weight).data_ptr()
+    a.lse2 = lse2.data_ptr() if lse2 is not None else None
     a.grad_hidden = gh.data_ptr() if want_hidden and gh.numel() else None
     a.grad_weight = gw.data_ptr() if want_weight else None
     if loss is not None or a.grad_hidden or a.grad_weight:
-        _run(a, dev)
+        _run(a, hidden.device)
     return loss, gh, gw, lse2
 
 
@@ -169,10 +168,10 @@ class _VocabLoss(torch.autograd.Function):
         ctx.temperature, ctx.reduction, ctx.grads = temperature, reduction, None
         if hidden.dtype == torch.bfloat16 and reduction != "none":
             loss, gh, gw, lse2 = _grads(hidden, weight, ids, logits, valid, temperature, reduction, None, None,
-                                        ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+                                        ctx.needs_input_grad[0], ctx.needs_input_grad[1], for_backward=True)
             ctx.grads = gh, gw
         else:
-            loss, lse2 = _loss(hidden, weight, ids, logits, valid, temperature, reduction)
+            loss, lse2 = _loss(hidden, weight, ids, logits, valid, temperature, reduction, for_backward=True)
         ctx.save_for_backward(hidden, weight, ids, logits, valid, lse2)
         return loss
 
