@@ -43,6 +43,8 @@ __device__ __forceinline__ float load_real(const void *p, int type, i64 at) {
 // come in the order of the logits; 64-bit words (id, share) are ordered by a bitonic network in shared memory.
 // Floor: 8 to 12 bytes per entry.
 __global__ void __launch_bounds__(128) teacher_kernel(Plan p) {
+    next_may_come();
+    before_is_done();
     extern __shared__ u64 sorted[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     u64 *e = sorted + (size_t)warp * p.k_sorted;
@@ -151,6 +153,8 @@ __device__ __forceinline__ void copy_row(T *to, const T *from, i64 inside, i64 a
 // entries stay below 2^15), and both gradients are scaled back in 32 bits.
 template <class T>
 __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
+    next_may_come();
+    before_is_done();
     constexpr int EACH = 8;  // rows of a thread, 1024 apart: their loads are in flight together
     __shared__ int in_warp[EACH * 32], slots[EACH * 1024];
     __shared__ int base;
@@ -282,6 +286,8 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
 // A weight whose rows do not start on 16-byte boundaries, copied so that they do.
 template <class T>
 __global__ void __launch_bounds__(256) align_weight_kernel(Plan p, T *to) {
+    next_may_come();
+    before_is_done();
     const int lane = threadIdx.x & 31;
     for (i64 j = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); j < p.vocab; j += (i64)gridDim.x * 8) {
         copy_row(to + j * p.dim_padded, (const T *)p.weight + j * p.weight_stride, p.dim, p.dim_padded, lane);
@@ -291,6 +297,8 @@ __global__ void __launch_bounds__(256) align_weight_kernel(Plan p, T *to) {
 // dW's rows on 16-byte boundaries to where the caller wants them.
 template <class T>
 __global__ void __launch_bounds__(256) unalign_weight_kernel(Plan p) {
+    next_may_come();
+    before_is_done();
     const int lane = threadIdx.x & 31;
     for (i64 j = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); j < p.vocab; j += (i64)gridDim.x * 8) {
         copy_row((T *)p.grad_weight + j * p.dim, (const T *)p.weight_out + j * p.weight_out_stride, p.dim, p.dim, lane);
@@ -303,6 +311,8 @@ __global__ void __launch_bounds__(256) unalign_weight_kernel(Plan p) {
 // `again`: the tiles that were made a second time.
 template <class T>
 __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, bool again, unsigned int all_tickets) {
+    next_may_come();
+    before_is_done();
     __shared__ float tops[8][8], sums[8][8], lse2s[8], refs[8];
     __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -411,6 +421,8 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
 
 // What comes down to the loss, onto gradients that were made with it.
 __global__ void __launch_bounds__(256) scale_kernel(__nv_bfloat16 *a, i64 n_a, __nv_bfloat16 *b, i64 n_b, const float *by) {
+    next_may_come();
+    before_is_done();
     const float f = *by;
     if (f == 1.f) return;
     for (int which = 0; which < 2; ++which) {
@@ -433,6 +445,8 @@ __global__ void __launch_bounds__(256) scale_kernel(__nv_bfloat16 *a, i64 n_a, _
 // dH of several pieces in the caller's rows and type, zeros where a row does not count.
 template <class T>
 __global__ void __launch_bounds__(256) scatter_kernel(Plan p) {
+    next_may_come();
+    before_is_done();
     const float scale = p.meta->out_scale;
     const i64 total = p.rows * p.dim;
     for (i64 x = (i64)blockIdx.x * 256 + threadIdx.x; x < total; x += (i64)gridDim.x * 256) {
@@ -595,20 +609,26 @@ int tensor_map(CUtensorMap *map, int type, const void *at, i64 rows, i64 cols, i
     return r == CUDA_SUCCESS ? STBPE_OK : fail(err, err_len, STBPE_E_CUDA, "cuTensorMapEncodeTiled", "refused");
 }
 
+// launched while the kernel before still runs (next_may_come, before_is_done)
+template <class... P, class... A>
+cudaError_t start(void (*kernel)(P...), i64 blocks, int threads, size_t smem, int group, cudaStream_t s, const A &...args) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((unsigned)blocks), c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem, c.stream = s;
+    cudaLaunchAttribute how[2];
+    how[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    how[0].val.programmaticStreamSerializationAllowed = 1;
+    how[1].id = cudaLaunchAttributeClusterDimension;
+    how[1].val.clusterDim = {(unsigned)group, 1, 1};
+    c.attrs = how, c.numAttrs = group > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&c, kernel, P(args)...);
+}
+
 template <class T, int KIND, int GROUP>
 int launch(const Plan &p, const Job &job, const CUtensorMap &a, const CUtensorMap &b, i64 tiles, cudaStream_t s, char *err, size_t err_len) {
     auto *kernel = product_kernel<T, KIND, GROUP>;
     VCK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PRODUCT_SMEM));
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3((unsigned)(tiles < SMS / GROUP ? tiles : SMS / GROUP) * GROUP);
-    c.blockDim = dim3(PRODUCT_THREADS);
-    c.dynamicSmemBytes = PRODUCT_SMEM;
-    c.stream = s;
-    cudaLaunchAttribute cluster;
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim = {GROUP, 1, 1};
-    c.attrs = &cluster, c.numAttrs = 1;
-    VCK(cudaLaunchKernelEx(&c, kernel, p, job, a, b));
+    VCK(start(kernel, (tiles < SMS / GROUP ? tiles : SMS / GROUP) * GROUP, PRODUCT_THREADS, PRODUCT_SMEM, GROUP, s, p, job, a, b));
     return STBPE_OK;
 }
 
@@ -635,9 +655,9 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
     auto map = [&](CUtensorMap *m, const void *at, i64 rows, i64 cols, i64 stride, int box) {
         return tensor_map(m, type, at, rows, cols, stride, box, err, err_len);
     };
-    if (p.k) teacher_kernel<<<blocks(p.rows, 4), 128, 4 * p.k_sorted * sizeof(u64), s>>>(p);
-    rows_kernel<T><<<p.rows + TILE_ROWS <= 16 * SMS ? (unsigned)(p.rows + TILE_ROWS) / 16 : (unsigned)SMS, 1024, 0, s>>>(p);
-    if (p.weight_rows != p.weight) align_weight_kernel<T><<<blocks(p.vocab, 8), 256, 0, s>>>(p, (T *)p.weight_rows);
+    if (p.k) VCK(start(teacher_kernel, blocks(p.rows, 4), 128, 4 * p.k_sorted * sizeof(u64), 1, s, p));
+    VCK(start(rows_kernel<T>, p.rows + TILE_ROWS <= 16 * SMS ? (p.rows + TILE_ROWS) / 16 : SMS, 1024, 0, 1, s, p));
+    if (p.weight_rows != p.weight) VCK(start(align_weight_kernel<T>, blocks(p.vocab, 8), 256, 0, 1, s, p, (T *)p.weight_rows));
     CUtensorMap h, w, h_across, w_across, g, g_across;
     VTRY(map(&h, p.packed, p.rows_padded, p.dim, p.dim_padded, 128));
     VTRY(map(&w, p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 128));
@@ -654,10 +674,10 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
             for (i64 r0 = 0; r0 < p.rows_padded; r0 += p.chunk_rows) {
                 Job job{0, p.vocab, r0, p.chunk_rows, false};
                 VTRY((product<T, MAKE_E>(p, job, h, w, s, err, err_len)));
-                join_kernel<T><<<joins, 256, 0, s>>>(p, r0, p.chunk_rows, false, 0);
+                VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, r0, p.chunk_rows, false, 0));
                 job.again = true;
                 VTRY((product<T, MAKE_E>(p, job, h, w, s, err, err_len)));
-                join_kernel<T><<<joins, 256, 0, s>>>(p, r0, p.chunk_rows, true, tickets);
+                VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, r0, p.chunk_rows, true, tickets));
                 if (p.grad_hidden) VTRY((product<T, GRAD_HIDDEN>(p, job, g, w_across, s, err, err_len)));
                 if (p.grad_weight) VTRY((product<T, GRAD_WEIGHT>(p, job, g_across, h_across, s, err, err_len)));
             }
@@ -665,7 +685,7 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
     } else {
         if (p.want_loss) {
             VTRY((product<T, STATS>(p, Job{0, p.vocab, 0, p.rows_padded, false}, h, w, s, err, err_len)));
-            join_kernel<T><<<joins, 256, 0, s>>>(p, 0, p.rows_padded, false, joins);
+            VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, 0, p.rows_padded, false, joins));
         }
         if (p.want_grads) {
             for (i64 v0 = 0; v0 < p.vocab; v0 += p.g_stride) {
@@ -674,11 +694,10 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
                 if (p.grad_hidden) VTRY((product<T, GRAD_HIDDEN>(p, job, g, w_across, s, err, err_len)));
                 if (p.grad_weight) VTRY((product<T, GRAD_WEIGHT>(p, job, g_across, h_across, s, err, err_len)));
             }
-            if (p.grad_hidden && p.acc) scatter_kernel<T><<<blocks(p.rows * p.dim, 256), 256, 0, s>>>(p);
+            if (p.grad_hidden && p.acc) VCK(start(scatter_kernel<T>, blocks(p.rows * p.dim, 256), 256, 0, 1, s, p));
         }
     }
-    if (p.want_grads && p.grad_weight && p.weight_out != p.grad_weight) unalign_weight_kernel<T><<<blocks(p.vocab, 8), 256, 0, s>>>(p);
-    VCK(cudaGetLastError());
+    if (p.want_grads && p.grad_weight && p.weight_out != p.grad_weight) VCK(start(unalign_weight_kernel<T>, blocks(p.vocab, 8), 256, 0, 1, s, p));
     return STBPE_OK;
 }
 
@@ -700,9 +719,11 @@ STBPE_VISIBLE int stbpe_scale_gradients(void *a, int64_t n_a, void *b, int64_t n
     const i64 most = n_a > n_b ? n_a : n_b;
     if (most == 0) return STBPE_OK;
     const i64 blocks = (most + 2047) / 2048;
-    scale_kernel<<<(unsigned)(blocks < SMS * 8 ? blocks : SMS * 8), 256, 0, (cudaStream_t)stream>>>(
-        (__nv_bfloat16 *)a, n_a, (__nv_bfloat16 *)b, n_b, by);
-    return cudaGetLastError() == cudaSuccess ? STBPE_OK : STBPE_E_CUDA;
+    if (start(scale_kernel, blocks < SMS * 8 ? blocks : SMS * 8, 256, 0, 1, (cudaStream_t)stream, (__nv_bfloat16 *)a, n_a, (__nv_bfloat16 *)b,
+              n_b, by) == cudaSuccess)
+        return STBPE_OK;
+    cudaGetLastError();
+    return STBPE_E_CUDA;
 }
 
 STBPE_VISIBLE int stbpe_vocab_loss_run(const stbpe_vocab_loss *args, void *stream, char *err, size_t err_len) {

@@ -15,6 +15,11 @@ constexpr int TILE_ROWS = 256;  // packed rows are filled up with zeros to this 
 // the running maximum starts at a finite value: a logit of -inf then adds 0 to the sum, and one of NaN or +inf makes it NaN
 #define LOWEST (-3.0e38f)
 
+// Every kernel is launched while the one before it still runs, and begins by letting the next one come; what it reads and
+// writes in memory comes behind before_is_done().
+__device__ __forceinline__ void next_may_come() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void before_is_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 struct Meta {
     int counted;          // rows that count
     unsigned int tickets; // blocks that are through with their rows' losses

@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
     uint32_t rank = 0;
     if (GROUP == 2) asm("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
 
+    next_may_come();
     if (warp == 0 && lane == 0) {
         for (int s = 0; s < STAGES; ++s) barrier_init(full + 8 * s, 1), barrier_init(empty + 8 * s, 1);
         for (int b = 0; b < 2; ++b) barrier_init(sums_full + 8 * b, 1), barrier_init(sums_empty + 8 * b, 8 * GROUP);
@@ -244,6 +245,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
     uint32_t tmem;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
 
+    before_is_done();
     // the tiles and their depth
     const i64 counted = p.meta->counted;
     const i64 n = counted - job.r0 < 0 ? 0 : counted - job.r0 < job.rows ? counted - job.r0 : job.rows;  // rows of this chunk
