@@ -471,20 +471,18 @@ int fail(char *err, size_t len, int status, const char *what, const char *why) {
 
 i64 up_to(i64 x, i64 unit) { return (x + unit - 1) / unit * unit; }
 
-// CTAs to a tile of a product: rounds of all SMs (part of one where the last round's tiles are split in depth) times what a tile
-// costs, 1 for 256 x 256 by a pair and 0.8 for 128 x 128 by a single CTA, a quarter of it with twice as many at a time (0.95 against
-// 1.5 PFLOP/s).  Single CTAs win where pairs would leave more than half of the SMs idle.
-int group_of(i64 rows, i64 cols, i64 depth = 0, bool may_split = false) {
+// CTAs to a tile of a product, by what it takes: rounds of all SMs (the last one's tiles may be split in depth) of steps of 64 terms, 0.36 us
+// for 256 x 256 by a pair and 0.28 for 128 x 128 by a single CTA, of which twice as many run at a time (1.4 against 0.95
+// PFLOP/s), and 3 us to begin and to store a tile, 5 more to join splits.
+int group_of(i64 rows, i64 cols, i64 depth, bool may_split) {
     double cost[3];
+    const i64 steps = (depth + 63) / 64;
     for (int g = 1; g <= 2; ++g) {
         const i64 side = 128 * g, tiles = ((rows + side - 1) / side) * ((cols + side - 1) / side), clusters = SMS / g, left = tiles % clusters;
-        i64 splits = 1;
-        if (may_split && left) {
-            splits = clusters / left < SPLITS ? clusters / left : SPLITS;
-            if (splits > depth / 64 / 8) splits = depth / 64 / 8;
-            if (splits < 1) splits = 1;
-        }
-        cost[g] = ((double)(tiles / clusters) + (left ? 1. / (double)splits : 0.)) * (g == 2 ? 1. : 0.8);
+        const i64 splits = may_split ? splits_of(left, clusters, steps) : 1;
+        const double step = g == 2 ? 0.36 : 0.28;
+        cost[g] = (double)(tiles / clusters) * steps * step;
+        if (left) cost[g] += (double)steps / splits * step + 3. + (splits > 1 ? 5. : 0.);
     }
     return cost[1] < cost[2] ? 1 : 2;
 }
@@ -536,7 +534,7 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
         const i64 most = KEPT / (2 * p.rows_padded) / PIECE * PIECE;
         p.g_stride = all <= most ? all : most > 2048 ? most : all < 2048 ? all : 2048;
     }
-    p.group = group_of(p.keep ? p.chunk_rows : p.rows, a->vocab);
+    p.group = group_of(p.keep && p.chunk_rows < p.rows ? p.chunk_rows : p.rows, a->vocab, a->dim, false);
     p.parts = (int)((a->vocab + 64 * p.group - 1) / (64 * p.group));
     p.part_stride = p.chunk_rows;
     p.acc_stride = up_to(a->dim, 32);

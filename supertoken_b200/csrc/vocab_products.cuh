@@ -34,6 +34,16 @@ constexpr int SPLITS = 8;
 constexpr int PRODUCT_THREADS = 384;
 constexpr int PRODUCT_SMEM = STAGES * STAGE_BYTES + 1024 + 256;
 
+// Units that each of the `left` tiles of the last round is split into: as many as the clusters allow, of SPLIT_STEPS steps at least,
+// which take as long as it takes to join them.
+constexpr int SPLIT_STEPS = 16;
+__host__ __device__ inline i64 splits_of(i64 left, i64 clusters, i64 steps) {
+    if (left <= 0) return 1;
+    i64 splits = clusters / left < SPLITS ? clusters / left : SPLITS;
+    if (splits > steps / SPLIT_STEPS) splits = steps / SPLIT_STEPS;
+    return splits < 1 ? 1 : splits;
+}
+
 struct Job {
     i64 v0, width;  // the piece of the vocabulary
     i64 r0, rows;   // the chunk of the packed rows
@@ -256,16 +266,10 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
     const bool nothing = KIND == GRAD_WEIGHT ? job.r0 > 0 && n == 0 : KIND == MAKE_E && job.again && !p.meta->again;
     const i64 tiles = nothing ? 0 : tiles_m * tiles_n;
     const i64 cluster = blockIdx.x / GROUP, clusters = gridDim.x / GROUP;
-    // The tiles behind the last full round of all clusters are split in depth, so that the round that is not full is shorter, too:
-    // up to SPLITS units per tile of eight steps at least.
+    // the tiles behind the last full round of all clusters may be split in depth, so that the round that is not full is shorter, too
     const bool may_split = GRADS && (KIND == GRAD_WEIGHT ? !p.weight_acc : !p.acc);
     const i64 left = tiles % clusters;
-    i64 splits = 1;
-    if (may_split && left > 0) {
-        splits = clusters / left < SPLITS ? clusters / left : SPLITS;
-        if (splits > steps / 8) splits = steps / 8;
-        if (splits < 1) splits = 1;
-    }
+    const i64 splits = may_split ? splits_of(left, clusters, steps) : 1;
     const i64 whole = tiles - left, units = whole + left * splits;
     // A band of tiles of rows goes through all columns, its rows first.  LOGITS: that much of H stays in L2 while W passes by.  Else the
     // tiles that are being made at a time are as many columns as there are, or a square where both operands pass by, so that

@@ -39,33 +39,36 @@ def _rows(t: torch.Tensor, lead: int) -> Tuple[int, int]:
 
 
 def _arguments(hidden, weight, ids, logits, valid, temperature, reduction) -> L.VocabLoss:
-    for t in (hidden, weight, ids) + ((logits,) if logits is not None else ()) + ((valid,) if valid is not None else ()):
+    device, kd = getattr(hidden, "device", None), logits is not None
+    for t in (hidden, weight, ids, logits if kd else ids, ids if valid is None else valid):
         if not isinstance(t, torch.Tensor):
             raise TypeError("hidden, weight, ids, teacher_logits and valid must be tensors")
         if not t.is_cuda:
             raise RuntimeError("supertoken_b200 operators need CUDA tensors; there is no CPU fallback")
-        if t.device != hidden.device:
+        if t.device != device:
             raise ValueError("tensors must be on one device")
-    if hidden.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != hidden.dtype:
+    dtype = hidden.dtype
+    if (dtype != torch.bfloat16 and dtype != torch.float16) or weight.dtype != dtype:
         raise TypeError("hidden and weight must both be bfloat16 or both be float16")
-    if ids.dtype not in (torch.int32, torch.int64):
+    if ids.dtype != torch.int32 and ids.dtype != torch.int64:
         raise TypeError("token ids must be int32 or int64")
-    if valid is not None and valid.dtype not in (torch.uint8, torch.bool):
+    if valid is not None and valid.dtype != torch.uint8 and valid.dtype != torch.bool:
         raise TypeError("valid must be uint8 or bool")
-    if hidden.dim() not in (2, 3) or weight.dim() != 2 or weight.size(1) != hidden.size(-1):
+    size, wide = hidden.shape, weight.shape
+    lead, shape, D = len(size) - 1, size[:-1], size[-1] if size else 0
+    if lead not in (1, 2) or len(wide) != 2 or wide[1] != D:
         raise ValueError("hidden must be [N, D] or [B, L, D] and weight [V, D]")
-    lead, shape = hidden.dim() - 1, hidden.shape[:-1]
-    if weight.size(0) < 1 or weight.size(1) < 1:
+    if wide[0] < 1 or D < 1:
         raise ValueError("weight must have at least one row and one column")
     if reduction not in _REDUCTIONS:
         raise ValueError("reduction must be 'none', 'sum' or 'mean'")
     if valid is not None and valid.shape != shape:
         raise ValueError("valid must have the shape of hidden without its last dimension")
-    if (hidden.stride(-1) != 1 and hidden.size(-1) > 1) or (weight.stride(-1) != 1 and weight.size(-1) > 1):
+    step, wide_step = hidden.stride(), weight.stride()
+    if D > 1 and (step[-1] != 1 or wide_step[1] != 1):
         raise ValueError("the last dimension of hidden and weight must be contiguous")
     a = L.VocabLoss()
-    a.k = 0
-    if logits is None:
+    if not kd:
         if ids.shape != shape:
             raise ValueError("targets must have the shape of hidden without its last dimension")
     else:
@@ -73,22 +76,26 @@ def _arguments(hidden, weight, ids, logits, valid, temperature, reduction) -> L.
             raise TypeError("teacher_logits must be bfloat16, float16 or float32")
         if ids.dim() != lead + 1 or ids.shape[:-1] != shape or logits.shape != ids.shape:
             raise ValueError("teacher_ids and teacher_logits must have the shape of hidden with K as last dimension")
-        a.k = ids.size(-1)
-        if not 1 <= a.k <= MAX_TEACHER_ENTRIES:
+        a.k = k = ids.size(-1)
+        if not 1 <= k <= MAX_TEACHER_ENTRIES:
             raise ValueError(f"a teacher gives 1 to {MAX_TEACHER_ENTRIES} entries per row")
-        if a.k > 1 and (ids.stride(-1) != 1 or logits.stride(-1) != 1):
+        if k > 1 and (ids.stride(-1) != 1 or logits.stride(-1) != 1):
             raise ValueError("the last dimension of teacher_ids and teacher_logits must be contiguous")
         if not (0.0 < temperature < float("inf")):
             raise ValueError("temperature must be positive and finite")
         a.logits, a.logits_type = logits.data_ptr(), _REAL[logits.dtype]
         a.logits_outer, a.logits_inner = _rows(logits, lead)
-    a.outer, a.inner = (shape[0], shape[1]) if lead == 2 else (1, shape[0])
-    a.vocab, a.dim = weight.shape
-    a.type, a.ids_bytes = _REAL[hidden.dtype], ids.element_size()
+    if lead == 2:
+        a.outer, a.inner = shape
+        a.hidden_outer = step[0]
+    else:
+        a.outer, a.inner = 1, shape[0]
+    a.hidden_inner = step[-2]
+    a.vocab, a.dim = wide
+    a.type, a.ids_bytes = _REAL[dtype], 4 if ids.dtype == torch.int32 else 8
     a.reduction, a.temperature = _REDUCTIONS[reduction], temperature
     a.hidden, a.weight, a.ids = hidden.data_ptr(), weight.data_ptr(), ids.data_ptr()
-    a.hidden_outer, a.hidden_inner = _rows(hidden, lead)
-    a.weight_stride = weight.stride(0)
+    a.weight_stride = wide_step[0]
     a.ids_outer, a.ids_inner = _rows(ids, lead)
     if valid is not None:
         a.valid = valid.data_ptr()
@@ -97,16 +104,18 @@ def _arguments(hidden, weight, ids, logits, valid, temperature, reduction) -> L.
 
 
 def _run(a: L.VocabLoss, device: torch.device) -> None:
-    if device.index != torch.cuda.current_device():
+    index = device.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return _run(a, device)
-    lib, need, err = L.load(), ctypes.c_int64(0), ctypes.create_string_buffer(256)
-    st = lib.stbpe_vocab_loss_workspace(ctypes.byref(a), ctypes.byref(need), err, 256)
+    lib, need, err, here = L.load(), ctypes.c_int64(0), ctypes.create_string_buffer(256), ctypes.byref(a)
+    st = lib.stbpe_vocab_loss_workspace(here, ctypes.byref(need), err, 256)
     if st == L.OK:
         # torch's allocator knows streams and captures: a graph's workspace is in the graph's own pool
-        space = torch.empty(need.value + 1024, dtype=torch.uint8, device=device)
-        a.workspace, a.workspace_bytes = (space.data_ptr() + 1023) // 1024 * 1024, need.value
-        st = lib.stbpe_vocab_loss_run(ctypes.byref(a), torch.cuda.current_stream(device).cuda_stream, err, 256)
+        size = need.value
+        space = torch.empty(size + 1024, dtype=torch.uint8, device=device)  # (held until all is launched)
+        a.workspace, a.workspace_bytes = (space.data_ptr() + 1023) // 1024 * 1024, size
+        st = lib.stbpe_vocab_loss_run(here, torch._C._cuda_getCurrentRawStream(index), err, 256)
     if st != L.OK:
         _raise(st, err.value.decode())
 
@@ -208,7 +217,7 @@ def _refuse_capture(device: torch.device) -> None:
 
 
 def _differentiable(hidden, weight, ids, logits, valid, temperature, reduction):
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (hidden, weight)):
+    if torch.is_grad_enabled() and (getattr(hidden, "requires_grad", False) or getattr(weight, "requires_grad", False)):
         _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
         _refuse_capture(hidden.device)
         return _VocabLoss.apply(hidden, weight, ids, logits, valid, temperature, reduction)
