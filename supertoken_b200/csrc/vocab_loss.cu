@@ -130,7 +130,7 @@ __device__ __forceinline__ void copy_row(T *to, const T *from, i64 inside, i64 a
 #pragma unroll 4
         for (i64 d = lane * 8; d < inside; d += 256) *(uint4 *)(to + d) = *(const uint4 *)(from + d);
     } else if (at % 4 == 0) {
-#pragma unroll 8
+#pragma unroll 16
         for (i64 d = lane * 2; d < all; d += 64) {
             const uint32_t both = d + 1 < inside ? *(const uint32_t *)(from + d) : d < inside ? *(const unsigned short *)(from + d) : 0u;
             if (d + 1 < all) *(uint32_t *)(to + d) = both;
@@ -155,6 +155,12 @@ template <class T>
 __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
     next_may_come();
     before_is_done();
+    if (blockIdx.x >= p.row_blocks) {  // a weight whose rows do not start on 16-byte boundaries is copied so that they do
+        const i64 blocks = gridDim.x - p.row_blocks;
+        for (i64 j = blockIdx.x - p.row_blocks + (threadIdx.x >> 5) * blocks; j < p.vocab; j += blocks * 32)
+            copy_row((T *)p.weight_rows + j * p.dim_padded, (const T *)p.weight + j * p.weight_stride, p.dim, p.dim_padded, threadIdx.x & 31);
+        return;
+    }
     constexpr int EACH = 8;  // rows of a thread, 1024 apart: their loads are in flight together
     __shared__ int in_warp[EACH * 32], slots[EACH * 1024];
     __shared__ int base;
@@ -236,9 +242,9 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
             slots[x * 1024 + threadIdx.x] = counted[x] ? slot : -1;
         }
         __syncthreads();
-        // every gridDim.x-th row is this block's, one at a time to a warp
+        // every p.row_blocks-th row is this block's, one at a time to a warp
         const i64 end = p.rows - r0 < EACH * 1024 ? p.rows - r0 : EACH * 1024;
-        for (i64 y = blockIdx.x + (i64)warp * gridDim.x; y < end; y += (i64)gridDim.x * 32) {
+        for (i64 y = blockIdx.x + (i64)warp * p.row_blocks; y < end; y += (i64)p.row_blocks * 32) {
             const i64 its = r0 + y;
             const int to = slots[y];
             if (to >= 0) {
@@ -257,7 +263,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
     __syncthreads();
     const int n = base;
     const i64 until = (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS;
-    for (i64 c = n + blockIdx.x * 32 + warp; c < until; c += gridDim.x * 32)
+    for (i64 c = n + blockIdx.x * 32 + warp; c < until; c += p.row_blocks * 32)
         for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)((T *)p.packed + c * p.dim_padded + d) = make_uint4(0, 0, 0, 0);
     if (!first) return;
     for (i64 c = n + threadIdx.x; c < p.rows_padded; c += 1024) p.row_of[c] = -1;
@@ -280,28 +286,6 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
         p.meta->counted = n, p.meta->tickets = 0, p.meta->again = 0;
         p.meta->in_scale = (each ? 1.f : one) * factor * ldexpf(1.f, 14 - up);
         p.meta->out_scale = ldexpf(1.f, up - 14);
-    }
-}
-
-// A weight whose rows do not start on 16-byte boundaries, copied so that they do.
-template <class T>
-__global__ void __launch_bounds__(256) align_weight_kernel(Plan p, T *to) {
-    next_may_come();
-    before_is_done();
-    const int lane = threadIdx.x & 31;
-    for (i64 j = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); j < p.vocab; j += (i64)gridDim.x * 8) {
-        copy_row(to + j * p.dim_padded, (const T *)p.weight + j * p.weight_stride, p.dim, p.dim_padded, lane);
-    }
-}
-
-// dW's rows on 16-byte boundaries to where the caller wants them.
-template <class T>
-__global__ void __launch_bounds__(256) unalign_weight_kernel(Plan p) {
-    next_may_come();
-    before_is_done();
-    const int lane = threadIdx.x & 31;
-    for (i64 j = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); j < p.vocab; j += (i64)gridDim.x * 8) {
-        copy_row((T *)p.grad_weight + j * p.dim, (const T *)p.weight_out + j * p.weight_out_stride, p.dim, p.dim, lane);
     }
 }
 
@@ -508,6 +492,7 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     p.dim_padded = up_to(a->dim, 8);
     p.rows_padded = up_to(p.rows > 0 ? p.rows : 1, TILE_ROWS);
     p.pieces = (int)((a->vocab + PIECE - 1) / PIECE);
+    p.row_blocks = p.rows + TILE_ROWS <= 16 * SMS ? (int)(p.rows + TILE_ROWS) / 16 : SMS;
     p.k_sorted = 2;
     while (p.k_sorted < a->k) p.k_sorted *= 2;
     p.temperature = a->temperature, p.inv_temperature = 1.f / a->temperature;
@@ -538,7 +523,6 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     p.parts = (int)((a->vocab + 64 * p.group - 1) / (64 * p.group));
     p.part_stride = p.chunk_rows;
     p.acc_stride = up_to(a->dim, 32);
-    p.weight_out = a->grad_weight, p.weight_out_stride = a->dim;
     bytes = 0;
     char *base = (char *)a->workspace;
     auto take = [&](i64 n) {
@@ -577,10 +561,6 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
             if (p.chunk_rows < p.rows_padded) p.weight_acc = (float *)take(p.vocab * p.acc_stride * 4);
         } else if (p.g_stride < all) {
             p.acc = (float *)take(p.rows_padded * p.acc_stride * 4);
-        }
-        if (a->dim % 8) {
-            p.weight_out_stride = p.dim_padded;
-            p.weight_out = take(p.vocab * p.dim_padded * 2);
         }
     }
     return STBPE_OK;
@@ -654,8 +634,7 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
         return tensor_map(m, type, at, rows, cols, stride, box, err, err_len);
     };
     if (p.k) VCK(start(teacher_kernel, blocks(p.rows, 4), 128, 4 * p.k_sorted * sizeof(u64), 1, s, p));
-    VCK(start(rows_kernel<T>, p.rows + TILE_ROWS <= 16 * SMS ? (p.rows + TILE_ROWS) / 16 : SMS, 1024, 0, 1, s, p));
-    if (p.weight_rows != p.weight) VCK(start(align_weight_kernel<T>, blocks(p.vocab, 8), 256, 0, 1, s, p, (T *)p.weight_rows));
+    VCK(start(rows_kernel<T>, p.row_blocks + (p.weight_rows != p.weight ? SMS : 0), 1024, 0, 1, s, p));
     CUtensorMap h, w, h_across, w_across, g, g_across;
     VTRY(map(&h, p.packed, p.rows_padded, p.dim, p.dim_padded, 128));
     VTRY(map(&w, p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 128));
@@ -695,7 +674,6 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
             if (p.grad_hidden && p.acc) VCK(start(scatter_kernel<T>, blocks(p.rows * p.dim, 256), 256, 0, 1, s, p));
         }
     }
-    if (p.want_grads && p.grad_weight && p.weight_out != p.grad_weight) VCK(start(unalign_weight_kernel<T>, blocks(p.vocab, 8), 256, 0, 1, s, p));
     return STBPE_OK;
 }
 

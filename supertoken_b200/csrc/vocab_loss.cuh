@@ -69,8 +69,7 @@ struct Plan {
     float *acc;              // several pieces: dH of packed rows in 32 bits, [packed row][acc_stride]
     float *weight_acc;       // several chunks: dW in 32 bits, [vocab][acc_stride]
     i64 acc_stride;
-    void *weight_out;        // where dW goes: grad_weight, or rows on 16-byte boundaries
-    i64 weight_out_stride;
+    int row_blocks;          // blocks that number and pack the rows; those behind them align the weight
     float *split_sums;       // sums of tiles whose depth is split
     unsigned int *split_done;
 };

@@ -32,7 +32,7 @@ constexpr int OPERAND_BYTES = 128 * 64 * 2;  // what a CTA loads of one operand 
 constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
 constexpr int SPLITS = 8;
 constexpr int PRODUCT_THREADS = 384;
-constexpr int PRODUCT_SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr int PRODUCT_SMEM = STAGES * STAGE_BYTES + 1024 + 256 + 8 * 2048;
 
 // Units that each of the `left` tiles of the last round is split into: as many as the clusters allow, of SPLIT_STEPS steps at least,
 // which take as long as it takes to join them.
@@ -175,21 +175,48 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
     return *(uint32_t *)&v;
 }
 
-// 32 values of one row, 16 bits each; `inside`: how many of them there are; `unit`: how many may be stored at a time, 8, 2 or 1
+// 32 columns of a warp's 32 rows in 16 bits, a row to a lane, by way of shared memory (2 KB of the warp's own), so that lanes side by side
+// store to one row: 16 bytes by 4 lanes, 4 by 16 or 2 by 32 (`unit` numbers at a time), where a lane that stores its own row
+// touches a sector of its own each time.  `to`: where the lane's row goes, null: nowhere; `inside`: how many of the columns there are.
 template <class T>
-__device__ __forceinline__ void store_row(T *to, const float (&v)[32], i64 inside, int unit) {
+__device__ __forceinline__ void store_rows(T *to, const float (&v)[32], i64 inside, int unit, uint32_t stage, int lane) {
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 4; ++c)  // units of 16 bytes change places so that eight rows fall into different banks
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + (c ^ ((lane >> 1) & 3)) * 16),
+                     "r"(pack2<T>(v[8 * c], v[8 * c + 1])), "r"(pack2<T>(v[8 * c + 2], v[8 * c + 3])),
+                     "r"(pack2<T>(v[8 * c + 4], v[8 * c + 5])), "r"(pack2<T>(v[8 * c + 6], v[8 * c + 7]))
+                     : "memory");
+    __syncwarp();
     if (unit == 8 && inside >= 32) {
 #pragma unroll
-        for (int x = 0; x < 32; x += 8)
-            *(uint4 *)(to + x) = make_uint4(pack2<T>(v[x], v[x + 1]), pack2<T>(v[x + 2], v[x + 3]), pack2<T>(v[x + 4], v[x + 5]),
-                                            pack2<T>(v[x + 6], v[x + 7]));
+        for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + (lane >> 2), c = lane & 3;
+            uint4 x;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                         : "r"(stage + row * 64 + (c ^ ((row >> 1) & 3)) * 16)
+                         : "memory");
+            T *at = (T *)__shfl_sync(~0u, (u64)to, row);
+            if (at) *(uint4 *)(at + c * 8) = x;
+        }
     } else if (unit >= 2 && inside >= 32) {
 #pragma unroll
-        for (int x = 0; x < 32; x += 2) *(uint32_t *)(to + x) = pack2<T>(v[x], v[x + 1]);
+        for (int i = 0; i < 16; ++i) {
+            const int row = i * 2 + (lane >> 4), c = (lane & 15) >> 2;
+            uint32_t x;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(stage + row * 64 + (c ^ ((row >> 1) & 3)) * 16 + (lane & 3) * 4) : "memory");
+            T *at = (T *)__shfl_sync(~0u, (u64)to, row);
+            if (at) *(uint32_t *)(at + (lane & 15) * 2) = x;
+        }
     } else {
-#pragma unroll
-        for (int x = 0; x < 32; ++x)
-            if (x < inside) to[x] = T(v[x]);
+#pragma unroll 8
+        for (int row = 0; row < 32; ++row) {
+            unsigned short x;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(stage + row * 64 + ((lane >> 3) ^ ((row >> 1) & 3)) * 16 + (lane & 7) * 2) : "memory");
+            T *at = (T *)__shfl_sync(~0u, (u64)to, row);
+            if (at && lane < inside) *(unsigned short *)(at + lane) = x;
+        }
     }
 }
 
@@ -378,6 +405,8 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const float scale = p.inv_temperature * 1.4426950408889634f;
         const int entries_of_row = p.k ? p.k : 1;
+        const uint32_t stage = bars + 256 + (warp - 4) * 2048;
+        const int unit = p.dim % 8 == 0 ? 8 : p.dim % 2 == 0 ? 2 : 1;  // of the caller's rows
         int buffer = 0;
         uint32_t sums_phase = 0;
         bool alive = true;  // once a wait has run out, all that is left becomes NaN
@@ -405,13 +434,13 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             if (KIND == GRAD_WEIGHT) coef = p.meta->out_scale;
             // 32 sums of dH or dW, at column c of this thread's columns
             auto emit = [&](int c, float(&v)[32]) {
+                if (c0 + c >= p.dim) return;
                 if (KIND == GRAD_HIDDEN) {
-                    if (m >= n || c0 + c >= p.dim) return;
                     if (!p.acc) {
 #pragma unroll
                         for (int x = 0; x < 32; ++x) v[x] *= coef;
-                        store_row((T *)p.grad_hidden + (i64)row * p.dim + c0 + c, v, p.dim - c0 - c, p.dim % 8 == 0 ? 8 : p.dim % 2 == 0 ? 2 : 1);
-                    } else {
+                        store_rows(m < n ? (T *)p.grad_hidden + (i64)row * p.dim + c0 + c : nullptr, v, p.dim - c0 - c, unit, stage, lane);
+                    } else if (m < n) {
                         float4 *to = (float4 *)(p.acc + m * p.acc_stride + c0 + c);
 #pragma unroll
                         for (int x = 0; x < 8; ++x) {
@@ -425,11 +454,10 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     }
                 }
                 if (KIND == GRAD_WEIGHT) {
-                    if (m >= job.width || c0 + c >= p.dim) return;
                     const i64 id = job.v0 + m;
-                    const bool last = counted <= job.r0 + job.rows;
+                    const bool there = m < job.width, last = counted <= job.r0 + job.rows;
                     float4 *to = (float4 *)(p.weight_acc + id * p.acc_stride + c0 + c);
-                    if (job.r0 > 0) {
+                    if (job.r0 > 0 && there) {
 #pragma unroll
                         for (int x = 0; x < 8; ++x) {
                             const float4 z = to[x];
@@ -439,8 +467,8 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     if (last) {
 #pragma unroll
                         for (int x = 0; x < 32; ++x) v[x] *= coef;
-                        store_row((T *)p.weight_out + id * p.weight_out_stride + c0 + c, v, p.dim - c0 - c, 8);
-                    } else {
+                        store_rows(there ? (T *)p.grad_weight + id * p.dim + c0 + c : nullptr, v, p.dim - c0 - c, unit, stage, lane);
+                    } else if (there) {
 #pragma unroll
                         for (int x = 0; x < 8; ++x) to[x] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
                     }
@@ -528,7 +556,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     }
                 }
                 if (KIND == MAKE_E || KIND == MAKE_G) {
-                    if (m < p.chunk_rows && c0 + c < p.g_stride) store_row((T *)p.g + m * p.g_stride + c0 + c, v, 32, 8);
+                    if (c0 + c < p.g_stride) store_rows((T *)p.g + m * p.g_stride + c0 + c, v, 32, 8, stage, lane);
                 }
             }
             if ((KIND == STATS || KIND == MAKE_E) && row >= 0 && job.v0 + c0 < p.vocab) {
