@@ -40,85 +40,105 @@ __device__ __forceinline__ float load_real(const void *p, int type, i64 at) {
 
 // One warp per row: softmax of the teacher's entries in 32 bits, entries in ascending order of their ids (the order in
 // which the products meet them), and for each piece of columns the first entry that lies in it or behind.  The ids
-// come in the order of the logits; 64-bit words (id, share) are ordered by a bitonic network in shared memory.
+// come in the order of the logits; 64-bit words (id, share), ITEMS to a lane, are ordered by a bitonic network of shuffles.
 // Floor: 8 to 12 bytes per entry.
+template <int ITEMS>
 __global__ void __launch_bounds__(128) teacher_kernel(Plan p) {
     next_may_come();
     before_is_done();
-    extern __shared__ u64 sorted[];
+    __shared__ u64 sorted[4][ITEMS * 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    u64 *e = sorted + (size_t)warp * p.k_sorted;
+    u64 *e = sorted[warp];
     for (i64 row = (i64)blockIdx.x * 4 + warp; row < p.rows; row += (i64)gridDim.x * 4) {
         const i64 o = (unsigned)row / (unsigned)p.inner, i = row - o * p.inner;
         const i64 id_at = o * p.ids_outer + i * p.ids_inner, real_at = o * p.logits_outer + i * p.logits_inner;
-        // rounded before anything is taken from it: the maximum less itself has to be 0 at the type's lowest value, too
-        auto softened = [&](i64 at) { return __fmul_rn(load_real(p.logits, p.logits_type, at), p.inv_temperature); };
-        float top = -INFINITY;
-        bool outside = false, nan = false;
-        for (int k = lane; k < p.k; k += 32) {
-            const i64 id = load_id(p.ids, p.ids_bytes, id_at + k);
-            if (id < 0) continue;
-            const float t = softened(real_at + k);
-            outside |= id >= p.vocab;
-            nan |= isnan(t) || t == INFINITY;
-            top = fmaxf(top, t);
+        i64 id[ITEMS];
+        float t[ITEMS];
+#pragma unroll
+        for (int x = 0; x < ITEMS; ++x) {
+            const int k = x * 32 + lane;
+            id[x] = k < p.k ? load_id(p.ids, p.ids_bytes, id_at + k) : -1;
+            // rounded before anything is taken from it: the maximum less itself has to be 0 at the type's lowest value, too
+            t[x] = k < p.k ? __fmul_rn(load_real(p.logits, p.logits_type, real_at + k), p.inv_temperature) : 0.f;
+        }
+        float top = -INFINITY, sum = 0.f, plogp = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int x = 0; x < ITEMS; ++x) {
+            if (id[x] < 0) continue;
+            bad |= id[x] >= p.vocab || isnan(t[x]) || t[x] == INFINITY;
+            top = fmaxf(top, t[x]);
         }
         for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-        outside = __any_sync(~0u, outside), nan = __any_sync(~0u, nan);
+        bool nan = false;
+#pragma unroll
+        for (int x = 0; x < ITEMS; ++x) nan |= id[x] >= 0 && isnan(t[x]);
+        bad = __any_sync(~0u, bad), nan = __any_sync(~0u, nan);
         const bool counted = top > -INFINITY || nan;
-        float sum = 0.f;
-        for (int k = lane; k < p.k; k += 32) {
-            const i64 id = load_id(p.ids, p.ids_bytes, id_at + k);
-            if (id >= 0 && counted) sum += expf(softened(real_at + k) - top);
-        }
+#pragma unroll
+        for (int x = 0; x < ITEMS; ++x)
+            if (id[x] >= 0 && counted) sum += expf(t[x] - top);
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
         const float inv = 1.f / sum, log_sum = logf(sum);
-        float plogp = 0.f;
-        for (int k = lane; k < p.k_sorted; k += 32) {
-            u64 word = ~0ull;  // no entry: behind all others
-            if (k < p.k && counted && !outside && !nan) {
-                const i64 id = load_id(p.ids, p.ids_bytes, id_at + k);
-                if (id >= 0) {
-                    const float x = softened(real_at + k) - top;
-                    const float share = expf(x) * inv;
-                    if (share > 0.f) {
-                        plogp += share * (x - log_sum);
-                        word = ((u64)id << 32) | __float_as_uint(share);
+        u64 word[ITEMS];
+#pragma unroll
+        for (int x = 0; x < ITEMS; ++x) {
+            word[x] = ~0ull;  // no entry: behind all others
+            if (id[x] < 0 || !counted || bad) continue;
+            const float share = expf(t[x] - top) * inv;
+            if (share > 0.f) {
+                plogp += share * (t[x] - top - log_sum);
+                word[x] = ((u64)id[x] << 32) | __float_as_uint(share);
+            }
+        }
+        for (int d = 16; d; d >>= 1) plogp += __shfl_xor_sync(~0u, plogp, d);
+#pragma unroll
+        for (int size = 2; size <= ITEMS * 32; size <<= 1) {
+#pragma unroll
+            for (int step = size >> 1; step; step >>= 1) {
+                if (step >= 32) {
+#pragma unroll
+                    for (int x = 0; x < ITEMS; ++x) {
+                        const int y = x ^ (step >> 5);
+                        if (y < x) continue;
+                        const bool up = !((x * 32) & size);
+                        if ((word[x] > word[y]) == up) {
+                            const u64 w = word[x];
+                            word[x] = word[y], word[y] = w;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < ITEMS; ++x) {
+                        const u64 w = __shfl_xor_sync(~0u, word[x], step);
+                        const bool up = !((x * 32 + lane) & size), low = !(lane & step);
+                        // the lower place of an ascending pair keeps the smaller word
+                        if ((w < word[x]) == (up == low)) word[x] = w;
                     }
                 }
             }
-            e[k] = word;
         }
-        for (int d = 16; d; d >>= 1) plogp += __shfl_xor_sync(~0u, plogp, d);
         __syncwarp();
-        for (int size = 2; size <= p.k_sorted; size <<= 1)
-            for (int step = size >> 1; step; step >>= 1) {
-                for (int k = lane; k < p.k_sorted / 2; k += 32) {
-                    const int a = 2 * k - (k & (step - 1)), b = a + step;
-                    const u64 x = e[a], y = e[b];
-                    if ((x > y) == !(a & size)) e[a] = y, e[b] = x;
-                }
-                __syncwarp();
-            }
-        for (int k = lane; k < p.k; k += 32) {
-            const u64 word = e[k];
-            p.entries[row * p.k + k] = word == ~0ull ? make_int2(INT_MAX, 0) : make_int2((int)(word >> 32), (int)word);
+#pragma unroll
+        for (int x = 0; x < ITEMS; ++x) {
+            const int k = x * 32 + lane;
+            e[k] = word[x];
+            if (k < p.k) p.entries[row * p.k + k] = word[x] == ~0ull ? make_int2(INT_MAX, 0) : make_int2((int)(word[x] >> 32), (int)word[x]);
         }
+        __syncwarp();
         for (int t = lane; t < p.pieces; t += 32) {  // first entry at or behind the piece's first column
             const u64 from = (u64)t * PIECE << 32;
-            int lo = 0, hi = p.k;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (e[mid] < from) lo = mid + 1;
-                else hi = mid;
-            }
-            p.first[row * p.pieces + t] = (unsigned short)lo;
+            int at = 0;
+#pragma unroll
+            for (int step = ITEMS * 16; step; step >>= 1)
+                if (e[at + step - 1] < from) at += step;
+            if (at < ITEMS * 32 && e[at] < from) ++at;
+            p.first[row * p.pieces + t] = (unsigned short)(at < p.k ? at : p.k);
         }
         if (lane == 0) {
-            p.plogp[row] = outside || nan ? NAN : plogp;
+            p.plogp[row] = bad ? NAN : plogp;
             p.has_entries[row] = counted;
         }
-        __syncwarp();
     }
 }
 
@@ -493,8 +513,6 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     p.rows_padded = up_to(p.rows > 0 ? p.rows : 1, TILE_ROWS);
     p.pieces = (int)((a->vocab + PIECE - 1) / PIECE);
     p.row_blocks = p.rows + TILE_ROWS <= 16 * SMS ? (int)(p.rows + TILE_ROWS) / 16 : SMS;
-    p.k_sorted = 2;
-    while (p.k_sorted < a->k) p.k_sorted *= 2;
     p.temperature = a->temperature, p.inv_temperature = 1.f / a->temperature;
     p.reduction = a->reduction;
     p.want_loss = (a->want & STBPE_WANT_LOSS) != 0, p.want_grads = (a->want & STBPE_WANT_GRADS) != 0;
@@ -633,7 +651,10 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
     auto map = [&](CUtensorMap *m, const void *at, i64 rows, i64 cols, i64 stride, int box) {
         return tensor_map(m, type, at, rows, cols, stride, box, err, err_len);
     };
-    if (p.k) VCK(start(teacher_kernel, blocks(p.rows, 4), 128, 4 * p.k_sorted * sizeof(u64), 1, s, p));
+    if (p.k) {
+        auto *teacher = p.k <= 32 ? teacher_kernel<1> : p.k <= 64 ? teacher_kernel<2> : p.k <= 128 ? teacher_kernel<4> : teacher_kernel<8>;
+        VCK(start(teacher, blocks(p.rows, 4), 128, 0, 1, s, p));
+    }
     VCK(start(rows_kernel<T>, p.row_blocks + (p.weight_rows != p.weight ? SMS : 0), 1024, 0, 1, s, p));
     CUtensorMap h, w, h_across, w_across, g, g_across;
     VTRY(map(&h, p.packed, p.rows_padded, p.dim, p.dim_padded, 128));
@@ -644,17 +665,17 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
         VTRY(map(&g, p.g, p.chunk_rows, p.g_stride, p.g_stride, 128));
         VTRY(map(&g_across, p.g, p.chunk_rows, p.g_stride, p.g_stride, 64));
     }
-    const unsigned joins = blocks(p.chunk_rows, 8);
+    const unsigned joins = blocks(p.chunk_rows, 8), few = joins < SMS ? joins : SMS;  // (few: mostly they find nothing made again)
     if (p.keep) {
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-            const unsigned tickets = joins * (unsigned)((p.rows_padded + p.chunk_rows - 1) / p.chunk_rows);
+            const unsigned tickets = few * (unsigned)((p.rows_padded + p.chunk_rows - 1) / p.chunk_rows);
             for (i64 r0 = 0; r0 < p.rows_padded; r0 += p.chunk_rows) {
                 Job job{0, p.vocab, r0, p.chunk_rows, false};
                 VTRY((product<T, MAKE_E>(p, job, h, w, s, err, err_len)));
                 VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, r0, p.chunk_rows, false, 0));
                 job.again = true;
                 VTRY((product<T, MAKE_E>(p, job, h, w, s, err, err_len)));
-                VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, r0, p.chunk_rows, true, tickets));
+                VCK(start(join_kernel<T>, few, 256, 0, 1, s, p, r0, p.chunk_rows, true, tickets));
                 if (p.grad_hidden) VTRY((product<T, GRAD_HIDDEN>(p, job, g, w_across, s, err, err_len)));
                 if (p.grad_weight) VTRY((product<T, GRAD_WEIGHT>(p, job, g_across, h_across, s, err, err_len)));
             }

@@ -31,7 +31,7 @@ struct Meta {
 struct Plan {
     i64 rows, inner;  // row = outer * inner + inner index
     i64 vocab, dim, dim_padded, rows_padded;
-    int k, k_sorted, pieces, parts, reduction, group;
+    int k, pieces, parts, reduction, group;
     bool want_loss, want_grads;
     float temperature, inv_temperature;
     const void *hidden, *weight, *ids, *logits;

@@ -67,8 +67,9 @@ __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
+// nothing in memory goes with it (the loads from TMEM have arrived), so it does not wait for the thread's stores
 __device__ __forceinline__ void barrier_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // Every wait ends: after two seconds it fails, all roles leave their loops as that happens to them, and what was to be
@@ -488,14 +489,14 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     tmem_load(from + c, bits);
 #pragma unroll
                     for (int x = 0; x < 32; ++x) v[x] = t.k1 > t.k0 ? __uint_as_float(bits[x]) : 0.f;  // (no rows: nothing was summed)
+                    if (c + 32 == COLUMNS) {  // the buffer is free
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) barrier_arrive_cluster(GROUP == 2 ? in_cta(sums_empty + 8 * buffer, 0) : sums_empty + 8 * buffer);
+                    }
                 } else {
 #pragma unroll
                     for (int x = 0; x < 32; ++x) v[x] = NAN;
-                }
-                if (c + 32 == COLUMNS && alive) {  // the buffer is free
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) barrier_arrive_cluster(GROUP == 2 ? in_cta(sums_empty + 8 * buffer, 0) : sums_empty + 8 * buffer);
                 }
                 if (GRADS) {
                     if (t.split < 0) {
