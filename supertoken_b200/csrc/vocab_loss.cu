@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
     if (threadIdx.x == 0) base = 0;
     const bool first = blockIdx.x == 0;
     if (first && p.split_done)
-        for (int x = threadIdx.x; x < SMS * 8; x += 1024) p.split_done[x] = 0;
+        for (int x = threadIdx.x; x < 2 * SMS * 8; x += 1024) p.split_done[x] = 0;
     for (i64 r0 = 0; r0 < p.rows; r0 += EACH * 1024) {
         bool counted[EACH];
         unsigned votes[EACH];
@@ -475,18 +475,15 @@ int fail(char *err, size_t len, int status, const char *what, const char *why) {
 
 i64 up_to(i64 x, i64 unit) { return (x + unit - 1) / unit * unit; }
 
-// CTAs to a tile of a product, by what it takes: rounds of all SMs (the last one's tiles may be split in depth) of steps of 64 terms, 0.36 us
-// for 256 x 256 by a pair and 0.28 for 128 x 128 by a single CTA, of which twice as many run at a time (1.4 against 0.95
-// PFLOP/s), and 3 us to begin and to store a tile, 5 more to join splits.
-int group_of(i64 rows, i64 cols, i64 depth, bool may_split) {
+// CTAs to a tile of a product, by what it takes: steps of 64 terms, 0.36 us for 256 x 256 by a pair and 0.28 for 128 x 128 by a single
+// CTA, of which twice as many run at a time (1.4 against 0.95 PFLOP/s).
+int group_of(i64 rows, i64 cols, i64 rows2, i64 cols2, i64 depth, i64 depth2, bool split, bool split2) {
     double cost[3];
-    const i64 steps = (depth + 63) / 64;
     for (int g = 1; g <= 2; ++g) {
-        const i64 side = 128 * g, tiles = ((rows + side - 1) / side) * ((cols + side - 1) / side), clusters = SMS / g, left = tiles % clusters;
-        const i64 splits = may_split ? splits_of(left, clusters, steps) : 1;
-        const double step = g == 2 ? 0.36 : 0.28;
-        cost[g] = (double)(tiles / clusters) * steps * step;
-        if (left) cost[g] += (double)steps / splits * step + 3. + (splits > 1 ? 5. : 0.);
+        const i64 side = 128 * g;
+        const i64 tiles[2] = {((rows + side - 1) / side) * ((cols + side - 1) / side), ((rows2 + side - 1) / side) * ((cols2 + side - 1) / side)};
+        const int steps[2] = {(int)((depth + 63) / 64), (int)((depth2 + 63) / 64)};
+        cost[g] = (double)deal(tiles, steps, {split, split2}, SMS / g).steps * (g == 2 ? 0.36 : 0.28);
     }
     return cost[1] < cost[2] ? 1 : 2;
 }
@@ -537,7 +534,7 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
         const i64 most = KEPT / (2 * p.rows_padded) / PIECE * PIECE;
         p.g_stride = all <= most ? all : most > 2048 ? most : all < 2048 ? all : 2048;
     }
-    p.group = group_of(p.keep && p.chunk_rows < p.rows ? p.chunk_rows : p.rows, a->vocab, a->dim, false);
+    p.group = group_of(p.keep && p.chunk_rows < p.rows ? p.chunk_rows : p.rows, a->vocab, 0, 0, a->dim, 0, false, false);
     p.parts = (int)((a->vocab + 64 * p.group - 1) / (64 * p.group));
     p.part_stride = p.chunk_rows;
     p.acc_stride = up_to(a->dim, 32);
@@ -569,8 +566,8 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     if (p.want_grads) {
         p.coef = (float *)take(p.rows_padded * 4);
         p.g = take(p.chunk_rows * p.g_stride * 2);
-        p.split_sums = (float *)take((i64)SMS * 8 * 64 * 2 * 32 * 4);
-        p.split_done = (unsigned int *)take(SMS * 8 * 4);
+        p.split_sums = (float *)take((i64)2 * SMS * 8 * 64 * 2 * 32 * 4);
+        p.split_done = (unsigned int *)take(2 * SMS * 8 * 4);
         if (p.keep) {
             p.reference = (float *)take(p.rows_padded * 4);
             p.out_row = (float *)take(p.rows_padded * 4);
@@ -621,21 +618,24 @@ cudaError_t start(void (*kernel)(P...), i64 blocks, int threads, size_t smem, in
 }
 
 template <class T, int KIND, int GROUP>
-int launch(const Plan &p, const Job &job, const CUtensorMap &a, const CUtensorMap &b, i64 tiles, cudaStream_t s, char *err, size_t err_len) {
+int launch(const Plan &p, const Job &job, const Maps &maps, i64 tiles, cudaStream_t s, char *err, size_t err_len) {
     auto *kernel = product_kernel<T, KIND, GROUP>;
     VCK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PRODUCT_SMEM));
-    VCK(start(kernel, (tiles < SMS / GROUP ? tiles : SMS / GROUP) * GROUP, PRODUCT_THREADS, PRODUCT_SMEM, GROUP, s, p, job, a, b));
+    VCK(start(kernel, (tiles < SMS / GROUP ? tiles : SMS / GROUP) * GROUP, PRODUCT_THREADS, PRODUCT_SMEM, GROUP, s, p, job, maps));
     return STBPE_OK;
 }
 
 template <class T, int KIND>
-int product(const Plan &p, const Job &job, const CUtensorMap &a, const CUtensorMap &b, cudaStream_t s, char *err, size_t err_len) {
-    const i64 rows = KIND == GRAD_WEIGHT ? job.width : p.rows < job.rows ? p.rows : job.rows, cols = KIND <= MAKE_G ? job.width : p.dim;
-    if (rows == 0) return STBPE_OK;
-    // (the parts of the columns go by p.group)
-    const int group = KIND <= MAKE_G ? p.group : group_of(rows, cols, KIND == GRAD_HIDDEN ? job.width : p.rows, KIND == GRAD_HIDDEN ? !p.acc : !p.weight_acc);
-    const i64 tile = 128 * group, tiles = ((rows + tile - 1) / tile) * ((cols + tile - 1) / tile) * (KIND <= MAKE_G ? 1 : SPLITS);
-    return group == 1 ? launch<T, KIND, 1>(p, job, a, b, tiles, s, err, err_len) : launch<T, KIND, 2>(p, job, a, b, tiles, s, err, err_len);
+int product(const Plan &p, const Job &job, const Maps &maps, cudaStream_t s, char *err, size_t err_len) {
+    const i64 rows = p.rows < job.rows ? p.rows : job.rows;
+    if (KIND != GRADS) {
+        if (rows == 0) return STBPE_OK;
+        const i64 side = 128 * p.group, tiles = ((rows + side - 1) / side) * ((job.width + side - 1) / side);
+        return p.group == 1 ? launch<T, KIND, 1>(p, job, maps, tiles, s, err, err_len) : launch<T, KIND, 2>(p, job, maps, tiles, s, err, err_len);
+    }
+    const i64 tall = p.grad_hidden ? rows : 0, wide = p.grad_weight ? job.width : 0;
+    const int group = group_of(tall, p.dim, wide, p.dim, job.width, rows, !p.acc, !p.weight_acc);
+    return group == 1 ? launch<T, KIND, 1>(p, job, maps, SMS, s, err, err_len) : launch<T, KIND, 2>(p, job, maps, SMS, s, err, err_len);
 }
 
 #define VTRY(call)                        \
@@ -656,41 +656,40 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
         VCK(start(teacher, blocks(p.rows, 4), 128, 0, 1, s, p));
     }
     VCK(start(rows_kernel<T>, p.row_blocks + (p.weight_rows != p.weight ? SMS : 0), 1024, 0, 1, s, p));
-    CUtensorMap h, w, h_across, w_across, g, g_across;
-    VTRY(map(&h, p.packed, p.rows_padded, p.dim, p.dim_padded, 128));
-    VTRY(map(&w, p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 128));
+    Maps logits, grads;
+    VTRY(map(&logits.map[0], p.packed, p.rows_padded, p.dim, p.dim_padded, 128));
+    VTRY(map(&logits.map[1], p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 128));
+    logits.map[2] = logits.map[3] = logits.map[0];
     if (p.want_grads) {
-        VTRY(map(&h_across, p.keep ? p.scaled : p.packed, p.keep ? p.chunk_rows : p.rows_padded, p.dim, p.dim_padded, 64));
-        VTRY(map(&w_across, p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 64));
-        VTRY(map(&g, p.g, p.chunk_rows, p.g_stride, p.g_stride, 128));
-        VTRY(map(&g_across, p.g, p.chunk_rows, p.g_stride, p.g_stride, 64));
+        VTRY(map(&grads.map[0], p.g, p.chunk_rows, p.g_stride, p.g_stride, 128));
+        VTRY(map(&grads.map[1], p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 64));
+        VTRY(map(&grads.map[2], p.g, p.chunk_rows, p.g_stride, p.g_stride, 64));
+        VTRY(map(&grads.map[3], p.keep ? p.scaled : p.packed, p.keep ? p.chunk_rows : p.rows_padded, p.dim, p.dim_padded, 64));
     }
-    const unsigned joins = blocks(p.chunk_rows, 8), few = joins < SMS ? joins : SMS;  // (few: mostly they find nothing made again)
+    const unsigned joins = blocks(p.chunk_rows, 8), few = joins < SMS ? joins : (unsigned)SMS;  // (few: mostly they find nothing made again)
     if (p.keep) {
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
             const unsigned tickets = few * (unsigned)((p.rows_padded + p.chunk_rows - 1) / p.chunk_rows);
             for (i64 r0 = 0; r0 < p.rows_padded; r0 += p.chunk_rows) {
                 Job job{0, p.vocab, r0, p.chunk_rows, false};
-                VTRY((product<T, MAKE_E>(p, job, h, w, s, err, err_len)));
+                VTRY((product<T, MAKE_E>(p, job, logits, s, err, err_len)));
                 VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, r0, p.chunk_rows, false, 0));
                 job.again = true;
-                VTRY((product<T, MAKE_E>(p, job, h, w, s, err, err_len)));
+                VTRY((product<T, MAKE_E>(p, job, logits, s, err, err_len)));
                 VCK(start(join_kernel<T>, few, 256, 0, 1, s, p, r0, p.chunk_rows, true, tickets));
-                if (p.grad_hidden) VTRY((product<T, GRAD_HIDDEN>(p, job, g, w_across, s, err, err_len)));
-                if (p.grad_weight) VTRY((product<T, GRAD_WEIGHT>(p, job, g_across, h_across, s, err, err_len)));
+                VTRY((product<T, GRADS>(p, job, grads, s, err, err_len)));
             }
         }
     } else {
         if (p.want_loss) {
-            VTRY((product<T, STATS>(p, Job{0, p.vocab, 0, p.rows_padded, false}, h, w, s, err, err_len)));
+            VTRY((product<T, STATS>(p, Job{0, p.vocab, 0, p.rows_padded, false}, logits, s, err, err_len)));
             VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, 0, p.rows_padded, false, joins));
         }
         if (p.want_grads) {
             for (i64 v0 = 0; v0 < p.vocab; v0 += p.g_stride) {
                 const Job job{v0, p.vocab - v0 < p.g_stride ? p.vocab - v0 : p.g_stride, 0, p.rows_padded, false};
-                VTRY((product<T, MAKE_G>(p, job, h, w, s, err, err_len)));
-                if (p.grad_hidden) VTRY((product<T, GRAD_HIDDEN>(p, job, g, w_across, s, err, err_len)));
-                if (p.grad_weight) VTRY((product<T, GRAD_WEIGHT>(p, job, g_across, h_across, s, err, err_len)));
+                VTRY((product<T, MAKE_G>(p, job, logits, s, err, err_len)));
+                VTRY((product<T, GRADS>(p, job, grads, s, err, err_len)));
             }
             if (p.grad_hidden && p.acc) VCK(start(scatter_kernel<T>, blocks(p.rows * p.dim, 256), 256, 0, 1, s, p));
         }

@@ -4,8 +4,10 @@
 //   STATS        Z = H W^T; per row and part of the columns the maximum and the sum of exp, the logits at the entries
 //   MAKE_E       the same, and E = exp2(Z - reference) in 16 bits
 //   MAKE_G       Z again, of one piece of the vocabulary, and G = dlogits from it in 16 bits
-//   GRAD_HIDDEN  dH = E W or G W        (k over the columns: W is read with the other dimension contiguous)
-//   GRAD_WEIGHT  dW = E^T H' or G^T H   (k over the rows: both are read with the other dimension contiguous)
+//   GRADS        dH = E W or G W        (k over the columns: W is read with the other dimension contiguous) and
+//                dW = E^T H' or G^T H   (k over the rows: both are read with the other dimension contiguous),
+//                which wait for the same and fill each other's last round: a step over 2 048 x 1 256 x 512 takes 42 us with
+//                both in one launch and 51 with one each
 //
 // A group of GROUP CTAs makes a tile of 128 GROUP x 128 GROUP: with GROUP = 2 the two CTAs of a cluster share one
 // 256 x 256 tile (cta_group::2), each holding its half of both operands, so that a byte brought into shared memory serves twice as
@@ -25,7 +27,7 @@
 
 namespace vloss {
 
-enum { STATS, MAKE_E, MAKE_G, GRAD_HIDDEN, GRAD_WEIGHT };
+enum { STATS, MAKE_E, MAKE_G, GRADS };
 
 constexpr int STAGES = 6;
 constexpr int OPERAND_BYTES = 128 * 64 * 2;  // what a CTA loads of one operand per step of 64 terms
@@ -34,15 +36,39 @@ constexpr int SPLITS = 8;
 constexpr int PRODUCT_THREADS = 384;
 constexpr int PRODUCT_SMEM = STAGES * STAGE_BYTES + 1024 + 256 + 8 * 2048;
 
-// Units that each of the `left` tiles of the last round is split into: as many as the clusters allow, of SPLIT_STEPS steps at least,
-// which take as long as it takes to join them.
-constexpr int SPLIT_STEPS = 16;
-__host__ __device__ inline i64 splits_of(i64 left, i64 clusters, i64 steps) {
-    if (left <= 0) return 1;
-    i64 splits = clusters / left < SPLITS ? clusters / left : SPLITS;
-    if (splits > steps / SPLIT_STEPS) splits = steps / SPLIT_STEPS;
-    return splits < 1 ? 1 : splits;
+// How the tiles of one or two results are dealt out: whole ones in rounds of all clusters, first those of the first result, and those
+// that are left behind the full rounds split in depth, up to SPLITS units per tile of SPLIT_STEPS steps at least, so that the last
+// round is shorter, too.  Joining the units of a tile costs about as much as JOIN_STEPS steps.
+constexpr int SPLIT_STEPS = 16, JOIN_STEPS = 14;
+struct Deal {
+    i64 whole[2], left[2], units;
+    int splits[2];
+    i64 steps;  // what the busiest cluster goes through, about
+};
+__host__ __device__ inline Deal deal(const i64 (&tiles)[2], const int (&steps)[2], const bool (&may_split)[2], i64 clusters) {
+    Deal d;
+    i64 rounds = 0;
+    for (int r = 0; r < 2; ++r) {
+        d.left[r] = tiles[r] % clusters, d.whole[r] = tiles[r] - d.left[r], d.splits[r] = 1;
+        rounds += d.whole[r] / clusters * steps[r];
+    }
+    i64 best = -1;
+    for (int a = 1; a <= (may_split[0] && d.left[0] ? SPLITS : 1); a *= 2)
+        for (int b = 1; b <= (may_split[1] && d.left[1] ? SPLITS : 1); b *= 2) {
+            if ((a > 1 && (steps[0] < a * SPLIT_STEPS || d.left[0] * a > clusters)) || (b > 1 && (steps[1] < b * SPLIT_STEPS || d.left[1] * b > clusters)))
+                continue;
+            const i64 x = d.left[0] ? steps[0] / a + (a > 1 ? JOIN_STEPS : 0) : 0, y = d.left[1] ? steps[1] / b + (b > 1 ? JOIN_STEPS : 0) : 0;
+            const i64 cost = d.left[0] * a + d.left[1] * b <= clusters ? (x > y ? x : y) : x + y;
+            if (best < 0 || cost < best) best = cost, d.splits[0] = a, d.splits[1] = b;
+        }
+    d.units = d.whole[0] + d.whole[1] + d.left[0] * d.splits[0] + d.left[1] * d.splits[1];
+    d.steps = rounds + best;
+    return d;
 }
+
+struct Maps {
+    CUtensorMap map[4];
+};
 
 struct Job {
     i64 v0, width;  // the piece of the vocabulary
@@ -241,17 +267,16 @@ struct Walk {
 };
 
 // ---------------------------------------------------------------------------------------------- the kernel
+// maps: H and W (logits); E or G and W for dH, E or G and H for dW
 template <class T, int KIND, int GROUP>
 __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
-    product_kernel(const __grid_constant__ Plan p, const __grid_constant__ Job job, const __grid_constant__ CUtensorMap map_a,
-                   const __grid_constant__ CUtensorMap map_b) {
-    constexpr bool LOGITS = KIND <= MAKE_G, GRADS = !LOGITS;
-    constexpr bool A_ALONG_K = KIND != GRAD_WEIGHT, B_ALONG_K = LOGITS;
-    constexpr u64 A_NEXT = (A_ALONG_K ? 32 : 2048) >> 4, B_NEXT = (B_ALONG_K ? 32 : 2048) >> 4;  // 16 k further, for the descriptors
+    product_kernel(const __grid_constant__ Plan p, const __grid_constant__ Job job, const __grid_constant__ Maps maps) {
+    constexpr bool LOGITS = KIND != GRADS;
     constexpr int TILE = 128 * GROUP, COLUMNS = TILE / 2;  // columns that one epilogue thread takes of its row
-    constexpr uint32_t WHAT = 1u << 4 | (std::is_same<T, __nv_bfloat16>::value ? 1u << 7 | 1u << 10 : 0u) |
-                              (A_ALONG_K ? 0u : 1u << 15) | (B_ALONG_K ? 0u : 1u << 16) | (uint32_t)(TILE >> 3) << 17 |
-                              (uint32_t)(TILE >> 4) << 24;
+    // sums in 32 bits, the operands' type, TILE x TILE; dH has only its second operand across, dW both
+    constexpr uint32_t WHAT = 1u << 4 | (std::is_same<T, __nv_bfloat16>::value ? 1u << 7 | 1u << 10 : 0u) | (LOGITS ? 0u : 1u << 16) |
+                              (uint32_t)(TILE >> 3) << 17 | (uint32_t)(TILE >> 4) << 24;
+    constexpr uint32_t A_ACROSS = 1u << 15;
     extern __shared__ char raw[];
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
     const uint32_t bars = base + STAGES * STAGE_BYTES;
@@ -267,8 +292,8 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
         for (int b = 0; b < 2; ++b) barrier_init(sums_full + 8 * b, 1), barrier_init(sums_empty + 8 * b, 8 * GROUP);
         barrier_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+#pragma unroll
+        for (int x = 0; x < (LOGITS ? 2 : 4); ++x) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.map[x]) : "memory");
     }
     if (warp == 2) {
         if (GROUP == 2)
@@ -284,43 +309,59 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_at));
 
     before_is_done();
-    // the tiles and their depth
+    // The tiles and their depth.  Result 0 is Z or dH, result 1 is dW.
     const i64 counted = p.meta->counted;
     const i64 n = counted - job.r0 < 0 ? 0 : counted - job.r0 < job.rows ? counted - job.r0 : job.rows;  // rows of this chunk
-    const i64 rows = KIND == GRAD_WEIGHT ? job.width : n, cols = LOGITS ? job.width : p.dim;
-    const i64 depth = LOGITS ? p.dim : KIND == GRAD_HIDDEN ? job.width : n;
-    const i64 tiles_m = (rows + TILE - 1) / TILE, tiles_n = (cols + TILE - 1) / TILE;
-    const int steps = (int)((depth + 63) / 64);
-    const bool nothing = KIND == GRAD_WEIGHT ? job.r0 > 0 && n == 0 : KIND == MAKE_E && job.again && !p.meta->again;
-    const i64 tiles = nothing ? 0 : tiles_m * tiles_n;
     const i64 cluster = blockIdx.x / GROUP, clusters = gridDim.x / GROUP;
-    // the tiles behind the last full round of all clusters may be split in depth, so that the round that is not full is shorter, too
-    const bool may_split = GRADS && (KIND == GRAD_WEIGHT ? !p.weight_acc : !p.acc);
-    const i64 left = tiles % clusters;
-    const i64 splits = may_split ? splits_of(left, clusters, steps) : 1;
-    const i64 whole = tiles - left, units = whole + left * splits;
-    // A band of tiles of rows goes through all columns, its rows first.  LOGITS: that much of H stays in L2 while W passes by.  Else the
-    // tiles that are being made at a time are as many columns as there are, or a square where both operands pass by, so that
-    // they share what comes from memory (8 188 x 32 256 x 2 048: 1.0 and 0.6 GB read instead of 1.7 with bands of 16).
-    const i64 high_band = LOGITS ? 16 : (clusters + tiles_n - 1) / (tiles_n > 0 ? tiles_n : 1);
-    const i64 BAND = KIND == GRAD_HIDDEN && high_band < 8 * 2 / GROUP ? 8 * 2 / GROUP : high_band;
+    const i64 rows[2] = {n, job.width}, cols[2] = {LOGITS ? job.width : p.dim, p.dim};
+    const int steps[2] = {(int)(((LOGITS ? p.dim : job.width) + 63) / 64), (int)((n + 63) / 64)};
+    i64 tiles_m[2], tiles_n[2], tiles[2], band[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        tiles_m[r] = (rows[r] + TILE - 1) / TILE, tiles_n[r] = (cols[r] + TILE - 1) / TILE;
+        tiles[r] = tiles_m[r] * tiles_n[r];
+        // A band of tiles of rows goes through all columns, its rows first.  Z: that much of H stays in L2 while W passes by.  Else the
+        // tiles that are being made at a time are as many columns as there are, or a square where both operands pass by, so that
+        // they share what comes from memory (8 188 x 32 256 x 2 048: 1.0 and 0.6 GB read instead of 1.7 with bands of 16).
+        band[r] = LOGITS ? 16 : (clusters + tiles_n[r] - 1) / tiles_n[r];
+        if (!LOGITS && r == 0 && band[r] < 16 / GROUP) band[r] = 16 / GROUP;
+    }
+    if (LOGITS || !p.grad_weight || (job.r0 > 0 && n == 0)) tiles[1] = 0;
+    if ((!LOGITS && !p.grad_hidden) || (KIND == MAKE_E && job.again && !p.meta->again)) tiles[0] = 0;
+    const Deal dealt = deal(tiles, steps, {!LOGITS && !p.acc, !LOGITS && !p.weight_acc}, clusters);
+    const i64 units = dealt.units;
     struct Unit {
         i64 m0, n0;
-        int k0, k1, split, index;  // steps; number of the split tile
+        int k0, k1, split, splits;  // steps; split < 0: the whole tile
+        int result, sums, done;     // where its sums go and are counted, if it is split
     };
     auto unit_at = [&](i64 u) {
         Unit t;
-        i64 tile = u;
-        t.k0 = 0, t.k1 = steps, t.split = -1, t.index = 0;
-        if (u >= whole && splits > 1) {
-            t.index = (int)((u - whole) % left), t.split = (int)((u - whole) / left);
-            tile = whole + t.index;
-            t.k0 = (int)((i64)steps * t.split / splits), t.k1 = (int)((i64)steps * (t.split + 1) / splits);
+        const i64 whole = dealt.whole[0] + dealt.whole[1], first = dealt.left[0] * dealt.splits[0];
+        i64 tile;
+        t.split = -1, t.sums = t.done = 0;
+        if (u < whole) {
+            t.result = u >= dealt.whole[0];
+            tile = t.result ? u - dealt.whole[0] : u;
+            t.splits = 1;
+        } else {
+            t.result = u - whole >= first;
+            const i64 x = t.result ? u - whole - first : u - whole, left = t.result ? dealt.left[1] : dealt.left[0];
+            const i64 index = x % left;
+            tile = (t.result ? dealt.whole[1] : dealt.whole[0]) + index;
+            t.splits = t.result ? dealt.splits[1] : dealt.splits[0];
+            if (t.splits > 1) {
+                t.split = (int)(x / left);
+                t.sums = (int)((t.result ? first : 0) + index * t.splits), t.done = (int)((t.result ? dealt.left[0] : 0) + index);
+            }
         }
-        const i64 band = tile / (BAND * tiles_n), in = tile - band * BAND * tiles_n;
-        const i64 high = tiles_m - band * BAND < BAND ? tiles_m - band * BAND : BAND;
+        const i64 deep = t.result ? steps[1] : steps[0], high_m = t.result ? tiles_m[1] : tiles_m[0], wide_n = t.result ? tiles_n[1] : tiles_n[0],
+                  b = t.result ? band[1] : band[0];
+        t.k0 = t.split < 0 ? 0 : (int)(deep * t.split / t.splits), t.k1 = t.split < 0 ? (int)deep : (int)(deep * (t.split + 1) / t.splits);
+        const i64 which = tile / (b * wide_n), in = tile - which * b * wide_n;
+        const i64 high = high_m - which * b < b ? high_m - which * b : b;
         t.n0 = in / high * TILE;
-        t.m0 = (band * BAND + in % high) * TILE;
+        t.m0 = (which * b + in % high) * TILE;
         return t;
     };
     auto skipped = [&](const Unit &t) { return KIND == MAKE_E && job.again && !p.again[(job.r0 + t.m0) / TILE_ROWS]; };
@@ -343,18 +384,20 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     const uint32_t a = base + s * STAGE_BYTES, b = a + OPERAND_BYTES;
                     const uint32_t bar = GROUP == 2 ? in_cta(full + 8 * s, 0) : full + 8 * s;
                     if (rank == 0) barrier_expect(full + 8 * s, GROUP * STAGE_BYTES);
-                    if (A_ALONG_K) {
-                        tma_load<GROUP>(a, &map_a, k * 64, (LOGITS ? (int)job.r0 : 0) + am, bar);
-                    } else {
-                        tma_load<GROUP>(a, &map_a, am, k * 64, bar);
-                        tma_load<GROUP>(a + 8192, &map_a, am + 64, k * 64, bar);
-                    }
                     if (LOGITS) {
-                        tma_load<GROUP>(b, &map_b, k * 64, (int)job.v0 + bn, bar);
+                        tma_load<GROUP>(a, &maps.map[0], k * 64, (int)job.r0 + am, bar);
+                        tma_load<GROUP>(b, &maps.map[1], k * 64, (int)job.v0 + bn, bar);
                     } else {
-                        const int row = (KIND == GRAD_HIDDEN ? (int)job.v0 : 0) + k * 64;
-                        tma_load<GROUP>(b, &map_b, bn, row, bar);
-                        tma_load<GROUP>(b + 8192, &map_b, bn + 64, row, bar);
+                        if (t.result == 0) {
+                            tma_load<GROUP>(a, &maps.map[0], k * 64, am, bar);
+                        } else {
+                            tma_load<GROUP>(a, &maps.map[2], am, k * 64, bar);
+                            tma_load<GROUP>(a + 8192, &maps.map[2], am + 64, k * 64, bar);
+                        }
+                        const CUtensorMap *map = t.result == 0 ? &maps.map[1] : &maps.map[3];
+                        const int row = (t.result == 0 ? (int)job.v0 : 0) + k * 64;
+                        tma_load<GROUP>(b, map, bn, row, bar);
+                        tma_load<GROUP>(b + 8192, map, bn + 64, row, bar);
                     }
                     ++issued;
                     if (++s == STAGES) s = 0, phase ^= 1;
@@ -386,9 +429,12 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const u64 a = operand<A_ALONG_K>(base + s * STAGE_BYTES), b = operand<B_ALONG_K>(base + s * STAGE_BYTES + OPERAND_BYTES);
+                    const uint32_t at = base + s * STAGE_BYTES;
+                    const bool across = t.result == 1;
+                    const u64 a = across ? operand<false>(at) : operand<true>(at), b = operand<LOGITS>(at + OPERAND_BYTES);
+                    const u64 a_next = (across ? 2048 : 32) >> 4, b_next = (LOGITS ? 32 : 2048) >> 4;  // 16 k further
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) mma<GROUP>(d, a + x * A_NEXT, b + x * B_NEXT, WHAT, k > t.k0 || x > 0);
+                    for (int x = 0; x < 4; ++x) mma<GROUP>(d, a + x * a_next, b + x * b_next, across ? WHAT | A_ACROSS : WHAT, k > t.k0 || x > 0);
                     mma_commit<GROUP>(empty + 8 * s);
                     if (++s == STAGES) s = 0, phase ^= 1;
                 }
@@ -428,15 +474,17 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                 if (KIND == MAKE_E && row >= 0) shift = p.reference[slot];
                 if (KIND == MAKE_G && row >= 0) shift = p.lse2[row], coef = p.coef[slot] * p.meta->in_scale;
             }
-            if (KIND == GRAD_HIDDEN && m < n) {
-                row = p.row_of[slot];
-                coef = p.keep ? p.out_row[slot] : p.meta->out_scale;
+            if (!LOGITS) {
+                coef = p.meta->out_scale;
+                if (t.result == 0 && m < n) {
+                    row = p.row_of[slot];
+                    if (p.keep) coef = p.out_row[slot];
+                }
             }
-            if (KIND == GRAD_WEIGHT) coef = p.meta->out_scale;
             // 32 sums of dH or dW, at column c of this thread's columns
             auto emit = [&](int c, float(&v)[32]) {
                 if (c0 + c >= p.dim) return;
-                if (KIND == GRAD_HIDDEN) {
+                if (t.result == 0) {
                     if (!p.acc) {
 #pragma unroll
                         for (int x = 0; x < 32; ++x) v[x] *= coef;
@@ -453,8 +501,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                             to[x] = y;
                         }
                     }
-                }
-                if (KIND == GRAD_WEIGHT) {
+                } else {
                     const i64 id = job.v0 + m;
                     const bool there = m < job.width, last = counted <= job.r0 + job.rows;
                     float4 *to = (float4 *)(p.weight_acc + id * p.acc_stride + c0 + c);
@@ -478,8 +525,8 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             if (alive) alive = __all_sync(~0u, barrier_wait(sums_full + 8 * buffer, sums_phase));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t from = tmem + buffer * TILE + half * COLUMNS + ((uint32_t)(quarter * 32) << 16);
-            // [split tile][split][CTA][warp][column][lane]
-            float *sums = p.split_sums + ((((i64)t.index * splits + t.split) * GROUP + rank) * 8 + warp - 4) * (COLUMNS * 32) + lane;
+            // [unit of a split tile][CTA][warp][column][lane]
+            float *sums = p.split_sums + (((i64)(t.sums + (t.split < 0 ? 0 : t.split)) * GROUP + rank) * 8 + warp - 4) * (COLUMNS * 32) + lane;
 #pragma unroll 1
             for (int c = 0; c < COLUMNS; c += 32) {
                 float v[32];
@@ -498,7 +545,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
 #pragma unroll
                     for (int x = 0; x < 32; ++x) v[x] = NAN;
                 }
-                if (GRADS) {
+                if (!LOGITS) {
                     if (t.split < 0) {
                         emit(c, v);
                     } else {
@@ -564,15 +611,15 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                 const i64 to = (job.v0 + c0) / COLUMNS * p.part_stride + m;
                 p.part_max[to] = top, p.part_sum[to] = sum;
             }
-            if (GRADS && t.split >= 0) {
+            if (!LOGITS && t.split >= 0) {
                 // the last of the splits to get here adds them up, in their order
                 __threadfence();
                 __syncwarp();
-                unsigned int *done = p.split_done + (t.index * GROUP + rank) * 8 + warp - 4;
+                unsigned int *done = p.split_done + (t.done * GROUP + rank) * 8 + warp - 4;
                 unsigned int before = 0;
                 if (lane == 0) before = atomicAdd(done, 1u);
                 before = __shfl_sync(~0u, before, 0);
-                if (before == splits - 1) {
+                if (before == t.splits - 1) {
                     __threadfence();
                     if (lane == 0) *done = 0;
                     const i64 next = (i64)GROUP * 8 * COLUMNS * 32;
@@ -586,7 +633,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
 #pragma unroll
                             for (int s = 0; s < SPLITS; ++s)
 #pragma unroll
-                                for (int x = 0; x < 8; ++x) y[s][x] = s < splits ? __ldcg(sums + s * next + (c + x0 + x) * 32) : 0.f;
+                                for (int x = 0; x < 8; ++x) y[s][x] = s < t.splits ? __ldcg(sums + s * next + (c + x0 + x) * 32) : 0.f;
 #pragma unroll
                             for (int x = 0; x < 8; ++x) {
                                 v[x0 + x] = y[0][x];
