@@ -467,6 +467,12 @@ __global__ void __launch_bounds__(256) scatter_kernel(Plan p) {
         if (c_ != cudaSuccess) return fail(err, err_len, STBPE_E_CUDA, #call, cudaGetErrorString(c_)); \
     } while (0)
 
+#define VTRY(call)                        \
+    do {                                  \
+        const int st_ = (call);           \
+        if (st_ != STBPE_OK) return st_;  \
+    } while (0)
+
 int fail(char *err, size_t len, int status, const char *what, const char *why) {
     if (err && len) snprintf(err, len, "%s: %s", what, why);
     if (status == STBPE_E_CUDA) cudaGetLastError();
@@ -481,8 +487,9 @@ int group_of(i64 rows, i64 cols, i64 rows2, i64 cols2, i64 depth, i64 depth2, bo
     double cost[3];
     for (int g = 1; g <= 2; ++g) {
         const i64 side = 128 * g;
-        const i64 tiles[2] = {((rows + side - 1) / side) * ((cols + side - 1) / side), ((rows2 + side - 1) / side) * ((cols2 + side - 1) / side)};
-        const int steps[2] = {(int)((depth + 63) / 64), (int)((depth2 + 63) / 64)};
+        const unsigned tiles[2] = {(unsigned)(((rows + side - 1) / side) * ((cols + side - 1) / side)),
+                                   (unsigned)(((rows2 + side - 1) / side) * ((cols2 + side - 1) / side))};
+        const unsigned steps[2] = {(unsigned)((depth + 63) / 64), (unsigned)((depth2 + 63) / 64)};
         cost[g] = (double)deal(tiles, steps, {split, split2}, SMS / g).steps * (g == 2 ? 0.36 : 0.28);
     }
     return cost[1] < cost[2] ? 1 : 2;
@@ -495,6 +502,9 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     if (a->outer < 0 || a->inner < 0 || a->vocab < 1 || a->dim < 1) return bad("negative or empty size");
     if (a->vocab > INT_MAX - 65536 || a->dim > (1 << 20)) return bad("vocabulary or width too large");
     if (a->inner && a->outer > (INT_MAX - 65536) / a->inner) return bad("too many rows");
+    const i64 tall = (a->outer * a->inner + 127) / 128, wide = (a->vocab + 127) / 128, deep = (a->dim + 127) / 128;
+    if (tall * wide > INT_MAX / 4 || wide * deep > INT_MAX / 4 || tall * deep > INT_MAX / 4 || wide > INT_MAX / 128)
+        return bad("too many rows for this vocabulary and width");
     if (a->type != STBPE_REAL_BF16 && a->type != STBPE_REAL_FP16) return bad("hidden and weight are bf16 or fp16");
     if (a->k < 0 || a->k > STBPE_VOCAB_LOSS_MAX_K) return bad("number of teacher entries out of range");
     if (a->ids_bytes != 4 && a->ids_bytes != 8) return bad("ids have 4 or 8 bytes");
@@ -634,15 +644,17 @@ int product(const Plan &p, const Job &job, const Maps &maps, cudaStream_t s, cha
         return p.group == 1 ? launch<T, KIND, 1>(p, job, maps, tiles, s, err, err_len) : launch<T, KIND, 2>(p, job, maps, tiles, s, err, err_len);
     }
     const i64 tall = p.grad_hidden ? rows : 0, wide = p.grad_weight ? job.width : 0;
+    auto tiles = [&](i64 x) { return ((x + 255) / 256) * ((p.dim + 255) / 256); };
+    if (tall && wide && tiles(tall) + tiles(wide) > 4 * SMS / 2) {  // a launch each
+        Plan one = p;
+        one.grad_weight = nullptr;
+        VTRY((product<T, KIND>(one, job, maps, s, err, err_len)));
+        one.grad_weight = p.grad_weight, one.grad_hidden = nullptr;
+        return product<T, KIND>(one, job, maps, s, err, err_len);
+    }
     const int group = group_of(tall, p.dim, wide, p.dim, job.width, rows, !p.acc, !p.weight_acc);
     return group == 1 ? launch<T, KIND, 1>(p, job, maps, SMS, s, err, err_len) : launch<T, KIND, 2>(p, job, maps, SMS, s, err, err_len);
 }
-
-#define VTRY(call)                        \
-    do {                                  \
-        const int st_ = (call);           \
-        if (st_ != STBPE_OK) return st_;  \
-    } while (0)
 
 template <class T>
 int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {

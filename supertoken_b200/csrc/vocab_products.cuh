@@ -41,25 +41,24 @@ constexpr int PRODUCT_SMEM = STAGES * STAGE_BYTES + 1024 + 256 + 8 * 2048;
 // round is shorter, too.  Joining the units of a tile costs about as much as JOIN_STEPS steps.
 constexpr int SPLIT_STEPS = 16, JOIN_STEPS = 14;
 struct Deal {
-    i64 whole[2], left[2], units;
-    int splits[2];
-    i64 steps;  // what the busiest cluster goes through, about
+    unsigned whole[2], left[2], splits[2], units;
+    unsigned steps;  // what the busiest cluster goes through, about
 };
-__host__ __device__ inline Deal deal(const i64 (&tiles)[2], const int (&steps)[2], const bool (&may_split)[2], i64 clusters) {
+__host__ __device__ inline Deal deal(const unsigned (&tiles)[2], const unsigned (&steps)[2], const bool (&may_split)[2], unsigned clusters) {
     Deal d;
-    i64 rounds = 0;
+    unsigned rounds = 0;
     for (int r = 0; r < 2; ++r) {
         d.left[r] = tiles[r] % clusters, d.whole[r] = tiles[r] - d.left[r], d.splits[r] = 1;
         rounds += d.whole[r] / clusters * steps[r];
     }
-    i64 best = -1;
-    for (int a = 1; a <= (may_split[0] && d.left[0] ? SPLITS : 1); a *= 2)
-        for (int b = 1; b <= (may_split[1] && d.left[1] ? SPLITS : 1); b *= 2) {
+    unsigned best = UINT_MAX;
+    for (unsigned a = 1; a <= (may_split[0] && d.left[0] ? SPLITS : 1); a *= 2)
+        for (unsigned b = 1; b <= (may_split[1] && d.left[1] ? SPLITS : 1); b *= 2) {
             if ((a > 1 && (steps[0] < a * SPLIT_STEPS || d.left[0] * a > clusters)) || (b > 1 && (steps[1] < b * SPLIT_STEPS || d.left[1] * b > clusters)))
                 continue;
-            const i64 x = d.left[0] ? steps[0] / a + (a > 1 ? JOIN_STEPS : 0) : 0, y = d.left[1] ? steps[1] / b + (b > 1 ? JOIN_STEPS : 0) : 0;
-            const i64 cost = d.left[0] * a + d.left[1] * b <= clusters ? (x > y ? x : y) : x + y;
-            if (best < 0 || cost < best) best = cost, d.splits[0] = a, d.splits[1] = b;
+            const unsigned x = d.left[0] ? steps[0] / a + (a > 1 ? JOIN_STEPS : 0) : 0, y = d.left[1] ? steps[1] / b + (b > 1 ? JOIN_STEPS : 0) : 0;
+            const unsigned cost = d.left[0] * a + d.left[1] * b <= clusters ? (x > y ? x : y) : x + y;
+            if (cost < best) best = cost, d.splits[0] = a, d.splits[1] = b;
         }
     d.units = d.whole[0] + d.whole[1] + d.left[0] * d.splits[0] + d.left[1] * d.splits[1];
     d.steps = rounds + best;
@@ -312,56 +311,56 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
     // The tiles and their depth.  Result 0 is Z or dH, result 1 is dW.
     const i64 counted = p.meta->counted;
     const i64 n = counted - job.r0 < 0 ? 0 : counted - job.r0 < job.rows ? counted - job.r0 : job.rows;  // rows of this chunk
-    const i64 cluster = blockIdx.x / GROUP, clusters = gridDim.x / GROUP;
+    const unsigned cluster = blockIdx.x / GROUP, clusters = gridDim.x / GROUP;
     const i64 rows[2] = {n, job.width}, cols[2] = {LOGITS ? job.width : p.dim, p.dim};
-    const int steps[2] = {(int)(((LOGITS ? p.dim : job.width) + 63) / 64), (int)((n + 63) / 64)};
-    i64 tiles_m[2], tiles_n[2], tiles[2], band[2];
+    const unsigned steps[2] = {(unsigned)(((LOGITS ? p.dim : job.width) + 63) / 64), (unsigned)((n + 63) / 64)};
+    unsigned tiles_m[2], tiles_n[2], tiles[2], band[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        tiles_m[r] = (rows[r] + TILE - 1) / TILE, tiles_n[r] = (cols[r] + TILE - 1) / TILE;
+        tiles_m[r] = (unsigned)((rows[r] + TILE - 1) / TILE), tiles_n[r] = (unsigned)((cols[r] + TILE - 1) / TILE);
         tiles[r] = tiles_m[r] * tiles_n[r];
         // A band of tiles of rows goes through all columns, its rows first.  Z: that much of H stays in L2 while W passes by.  Else the
         // tiles that are being made at a time are as many columns as there are, or a square where both operands pass by, so that
-        // they share what comes from memory (8 188 x 32 256 x 2 048: 1.0 and 0.6 GB read instead of 1.7 with bands of 16).
+        // they share what comes from memory.
         band[r] = LOGITS ? 16 : (clusters + tiles_n[r] - 1) / tiles_n[r];
         if (!LOGITS && r == 0 && band[r] < 16 / GROUP) band[r] = 16 / GROUP;
     }
     if (LOGITS || !p.grad_weight || (job.r0 > 0 && n == 0)) tiles[1] = 0;
     if ((!LOGITS && !p.grad_hidden) || (KIND == MAKE_E && job.again && !p.meta->again)) tiles[0] = 0;
     const Deal dealt = deal(tiles, steps, {!LOGITS && !p.acc, !LOGITS && !p.weight_acc}, clusters);
-    const i64 units = dealt.units;
+    const unsigned units = dealt.units;
     struct Unit {
         i64 m0, n0;
         int k0, k1, split, splits;  // steps; split < 0: the whole tile
         int result, sums, done;     // where its sums go and are counted, if it is split
     };
-    auto unit_at = [&](i64 u) {
+    auto unit_at = [&](unsigned u) {  // (32-bit divisions: this stands between two tiles)
         Unit t;
-        const i64 whole = dealt.whole[0] + dealt.whole[1], first = dealt.left[0] * dealt.splits[0];
-        i64 tile;
-        t.split = -1, t.sums = t.done = 0;
+        const unsigned whole = dealt.whole[0] + dealt.whole[1], first = dealt.left[0] * dealt.splits[0];
+        unsigned tile;
+        t.split = -1, t.splits = 1, t.sums = t.done = 0;
         if (u < whole) {
             t.result = u >= dealt.whole[0];
             tile = t.result ? u - dealt.whole[0] : u;
-            t.splits = 1;
         } else {
             t.result = u - whole >= first;
-            const i64 x = t.result ? u - whole - first : u - whole, left = t.result ? dealt.left[1] : dealt.left[0];
-            const i64 index = x % left;
+            const unsigned x = t.result ? u - whole - first : u - whole, left = t.result ? dealt.left[1] : dealt.left[0];
+            const unsigned split = x / left, index = x - split * left;
             tile = (t.result ? dealt.whole[1] : dealt.whole[0]) + index;
-            t.splits = t.result ? dealt.splits[1] : dealt.splits[0];
+            t.splits = (int)(t.result ? dealt.splits[1] : dealt.splits[0]);
             if (t.splits > 1) {
-                t.split = (int)(x / left);
+                t.split = (int)split;
                 t.sums = (int)((t.result ? first : 0) + index * t.splits), t.done = (int)((t.result ? dealt.left[0] : 0) + index);
             }
         }
-        const i64 deep = t.result ? steps[1] : steps[0], high_m = t.result ? tiles_m[1] : tiles_m[0], wide_n = t.result ? tiles_n[1] : tiles_n[0],
-                  b = t.result ? band[1] : band[0];
-        t.k0 = t.split < 0 ? 0 : (int)(deep * t.split / t.splits), t.k1 = t.split < 0 ? (int)deep : (int)(deep * (t.split + 1) / t.splits);
-        const i64 which = tile / (b * wide_n), in = tile - which * b * wide_n;
-        const i64 high = high_m - which * b < b ? high_m - which * b : b;
-        t.n0 = in / high * TILE;
-        t.m0 = (which * b + in % high) * TILE;
+        const unsigned deep = t.result ? steps[1] : steps[0], high_m = t.result ? tiles_m[1] : tiles_m[0],
+                       wide_n = t.result ? tiles_n[1] : tiles_n[0], b = t.result ? band[1] : band[0];
+        t.k0 = t.split < 0 ? 0 : (int)(deep * (unsigned)t.split / (unsigned)t.splits);
+        t.k1 = t.split < 0 ? (int)deep : (int)(deep * (unsigned)(t.split + 1) / (unsigned)t.splits);
+        const unsigned which = tile / (b * wide_n), in = tile - which * b * wide_n;
+        const unsigned high = high_m - which * b < b ? high_m - which * b : b, column = in / high;
+        t.n0 = (i64)column * TILE;
+        t.m0 = (i64)(which * b + in - column * high) * TILE;
         return t;
     };
     auto skipped = [&](const Unit &t) { return KIND == MAKE_E && job.again && !p.again[(job.r0 + t.m0) / TILE_ROWS]; };
@@ -372,36 +371,40 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             uint32_t phase = 0;
             i64 issued = 0;
             bool alive = true;
-            for (i64 u = cluster; u < units && alive; u += clusters) {
+            for (unsigned u = cluster; u < units && alive; u += clusters) {
                 const Unit t = unit_at(u);
                 if (skipped(t)) continue;
                 const int am = (int)(t.m0 + rank * 128), bn = (int)(t.n0 + rank * 128);
-                for (int k = t.k0; k < t.k1; ++k) {
-                    if (!barrier_wait(empty + 8 * s, phase ^ 1)) {
-                        alive = false;
-                        break;
-                    }
-                    const uint32_t a = base + s * STAGE_BYTES, b = a + OPERAND_BYTES;
-                    const uint32_t bar = GROUP == 2 ? in_cta(full + 8 * s, 0) : full + 8 * s;
-                    if (rank == 0) barrier_expect(full + 8 * s, GROUP * STAGE_BYTES);
-                    if (LOGITS) {
-                        tma_load<GROUP>(a, &maps.map[0], k * 64, (int)job.r0 + am, bar);
-                        tma_load<GROUP>(b, &maps.map[1], k * 64, (int)job.v0 + bn, bar);
-                    } else {
-                        if (t.result == 0) {
+                // (a loop of its own for each result: what differs is known when it is compiled)
+                auto load = [&](auto which) {
+                    constexpr int RESULT = decltype(which)::value;
+                    for (int k = t.k0; k < t.k1; ++k) {
+                        if (!barrier_wait(empty + 8 * s, phase ^ 1)) {
+                            alive = false;
+                            break;
+                        }
+                        const uint32_t a = base + s * STAGE_BYTES, b = a + OPERAND_BYTES;
+                        const uint32_t bar = GROUP == 2 ? in_cta(full + 8 * s, 0) : full + 8 * s;
+                        if (rank == 0) barrier_expect(full + 8 * s, GROUP * STAGE_BYTES);
+                        if (LOGITS) {
+                            tma_load<GROUP>(a, &maps.map[0], k * 64, (int)job.r0 + am, bar);
+                            tma_load<GROUP>(b, &maps.map[1], k * 64, (int)job.v0 + bn, bar);
+                        } else if (RESULT == 0) {
                             tma_load<GROUP>(a, &maps.map[0], k * 64, am, bar);
+                            tma_load<GROUP>(b, &maps.map[1], bn, (int)job.v0 + k * 64, bar);
+                            tma_load<GROUP>(b + 8192, &maps.map[1], bn + 64, (int)job.v0 + k * 64, bar);
                         } else {
                             tma_load<GROUP>(a, &maps.map[2], am, k * 64, bar);
                             tma_load<GROUP>(a + 8192, &maps.map[2], am + 64, k * 64, bar);
+                            tma_load<GROUP>(b, &maps.map[3], bn, k * 64, bar);
+                            tma_load<GROUP>(b + 8192, &maps.map[3], bn + 64, k * 64, bar);
                         }
-                        const CUtensorMap *map = t.result == 0 ? &maps.map[1] : &maps.map[3];
-                        const int row = (t.result == 0 ? (int)job.v0 : 0) + k * 64;
-                        tma_load<GROUP>(b, map, bn, row, bar);
-                        tma_load<GROUP>(b + 8192, map, bn + 64, row, bar);
+                        ++issued;
+                        if (++s == STAGES) s = 0, phase ^= 1;
                     }
-                    ++issued;
-                    if (++s == STAGES) s = 0, phase ^= 1;
-                }
+                };
+                if (LOGITS || t.result == 0) load(std::integral_constant<int, 0>());
+                else load(std::integral_constant<int, 1>());
             }
             if (!alive && rank == 0) {  // copies in flight land before the memory is given up
                 const i64 pending = issued < STAGES ? issued : STAGES;
@@ -414,7 +417,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             int s = 0, buffer = 0;
             uint32_t phase = 0, sums_phase = 0;
             bool alive = true;
-            for (i64 u = cluster; u < units && alive; u += clusters) {
+            for (unsigned u = cluster; u < units && alive; u += clusters) {
                 const Unit t = unit_at(u);
                 if (skipped(t)) continue;
                 if (!barrier_wait(sums_empty + 8 * buffer, sums_phase ^ 1)) {
@@ -423,21 +426,26 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t d = tmem + buffer * TILE;
-                for (int k = t.k0; k < t.k1; ++k) {
-                    if (!barrier_wait(full + 8 * s, phase)) {
-                        alive = false;
-                        break;
-                    }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t at = base + s * STAGE_BYTES;
-                    const bool across = t.result == 1;
-                    const u64 a = across ? operand<false>(at) : operand<true>(at), b = operand<LOGITS>(at + OPERAND_BYTES);
-                    const u64 a_next = (across ? 2048 : 32) >> 4, b_next = (LOGITS ? 32 : 2048) >> 4;  // 16 k further
+                auto multiply = [&](auto which) {
+                    constexpr int RESULT = decltype(which)::value;
+                    constexpr u64 ALONG = 32 >> 4, ACROSS = 2048 >> 4;  // 16 k further
+                    for (int k = t.k0; k < t.k1; ++k) {
+                        if (!barrier_wait(full + 8 * s, phase)) {
+                            alive = false;
+                            break;
+                        }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const u64 a = operand<RESULT == 0>(base + s * STAGE_BYTES), b = operand<LOGITS>(base + s * STAGE_BYTES + OPERAND_BYTES);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) mma<GROUP>(d, a + x * a_next, b + x * b_next, across ? WHAT | A_ACROSS : WHAT, k > t.k0 || x > 0);
-                    mma_commit<GROUP>(empty + 8 * s);
-                    if (++s == STAGES) s = 0, phase ^= 1;
-                }
+                        for (int x = 0; x < 4; ++x)
+                            mma<GROUP>(d, a + x * (RESULT == 0 ? ALONG : ACROSS), b + x * (LOGITS ? ALONG : ACROSS), RESULT == 0 ? WHAT : WHAT | A_ACROSS,
+                                       k > t.k0 || x > 0);
+                        mma_commit<GROUP>(empty + 8 * s);
+                        if (++s == STAGES) s = 0, phase ^= 1;
+                    }
+                };
+                if (LOGITS || t.result == 0) multiply(std::integral_constant<int, 0>());
+                else multiply(std::integral_constant<int, 1>());
                 if (alive) mma_commit<GROUP>(sums_full + 8 * buffer);
                 buffer ^= 1;
                 if (buffer == 0) sums_phase ^= 1;
@@ -457,7 +465,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
         int buffer = 0;
         uint32_t sums_phase = 0;
         bool alive = true;  // once a wait has run out, all that is left becomes NaN
-        for (i64 u = cluster; u < units; u += clusters) {
+        for (unsigned u = cluster; u < units; u += clusters) {
             const Unit t = unit_at(u);
             if (skipped(t)) continue;
             const i64 m = t.m0 + rank * 128 + quarter * 32 + lane;  // this thread's row of the result
