@@ -309,10 +309,123 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
     }
 }
 
+// The losses of up to eight rows, as when text is scored as it is generated: bound by the weight, which is read once (V D 2 bytes), and by
+// launches, so numbering the rows and the product are one kernel.  A warp takes four of the weight's rows at a time, a lane 16 bytes of each per
+// 256 columns, against the rows of `hidden` in shared memory; sums in 32 bits, every block leaves its part as the tiles
+// of a product do.  17 MB of weight in 5 us, 13 us a call where the tensor cores' tiles of 128 rows and a launch more take 18.
+constexpr int FEW_ROWS = 8, FEW_NUMBERS = 16384;  // rows, and rows (rounded up to a power of two) times width
+template <class T, int ROWS>
+__global__ void __launch_bounds__(256) few_kernel(Plan p) {
+    next_may_come();
+    before_is_done();
+    __shared__ __align__(16) T h[FEW_NUMBERS];
+    __shared__ int ids[FEW_ROWS], slots[FEW_ROWS];
+    __shared__ float tops[8][FEW_ROWS], sums[8][FEW_ROWS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool first = blockIdx.x == 0;
+    const i64 warps = (i64)gridDim.x * 8;
+    // the weight's first rows come while the other inputs are looked at
+    for (int x = 0; x < 4; ++x) {
+        const i64 j = (i64)blockIdx.x * 8 + warp + x * warps;
+        if (j >= p.vocab) break;
+        for (int d = lane * 64; d < p.dim; d += 2048)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"((const T *)p.weight_rows + j * p.weight_rows_stride + d));
+    }
+    if (warp == 0) {
+        bool counted = false, outside = false;
+        i64 id = -1;
+        if (lane < p.rows) {
+            const i64 o = (unsigned)lane / (unsigned)p.inner, i = lane - o * p.inner;
+            id = load_id(p.ids, p.ids_bytes, o * p.ids_outer + i * p.ids_inner);
+            counted = id >= 0 && (!p.valid || p.valid[o * p.valid_outer + i * p.valid_inner]);
+            outside = id >= p.vocab;
+        }
+        const unsigned votes = __ballot_sync(~0u, counted);
+        const int slot = counted ? __popc(votes & ((1u << lane) - 1)) : -1;
+        if (lane < FEW_ROWS) slots[lane] = slot, ids[lane] = outside || !counted ? -1 : (int)id;
+        if (first && lane < p.rows) {
+            p.slot_of[lane] = slot;
+            p.entries[lane] = make_int2(!counted || outside ? INT_MAX : (int)id, __float_as_int(1.f));
+            p.plogp[lane] = outside ? NAN : 0.f;
+            if (counted) p.row_of[slot] = lane;
+            else p.row_loss[lane] = p.lse2[lane] = 0.f;
+        }
+        if (first && lane == 0) p.meta->counted = __popc(votes), p.meta->tickets = 0, p.meta->again = 0;
+    }
+    // rows that do not count take part in what nobody reads
+    for (int r = warp; r < ROWS; r += 8) {
+        const i64 row = r < p.rows ? r : 0, o = (unsigned)row / (unsigned)p.inner, i = row - o * p.inner;
+        copy_row(h + r * p.dim, (const T *)p.hidden + o * p.hidden_outer + i * p.hidden_inner, p.dim, p.dim, lane);
+    }
+    __syncthreads();
+    const float scale = 1.4426950408889634f;
+    float top[ROWS], sum[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) top[r] = LOWEST, sum[r] = 0.f;
+    for (i64 j0 = (i64)blockIdx.x * 8 + warp; j0 < p.vocab; j0 += 4 * warps) {
+        float z[4][ROWS];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) z[x][r] = 0.f;
+#pragma unroll 2
+        for (int d = lane * 8; d < p.dim; d += 256) {
+            uint4 w[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                w[x] = j0 + x * warps < p.vocab ? __ldcs((const uint4 *)((const T *)p.weight_rows + (j0 + x * warps) * p.weight_rows_stride + d))
+                                                : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const uint4 u = *(const uint4 *)(h + r * p.dim + d);
+                const T *a = (const T *)&u;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const T *b = (const T *)&w[x];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) z[x][r] = fmaf((float)a[i], (float)b[i], z[x][r]);
+                }
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const i64 j = j0 + x * warps;
+            if (j >= p.vocab) break;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                for (int d = 16; d; d >>= 1) z[x][r] += __shfl_xor_sync(~0u, z[x][r], d);
+                if (lane == 0 && ids[r] == j) p.entry_z[slots[r]] = z[x][r];
+                const float now = fmaxf(top[r], z[x][r] * scale);
+                sum[r] = sum[r] * exp2f(top[r] - now) + exp2f(fmaf(z[x][r], scale, -now));
+                top[r] = now;
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+        if (lane == 0) tops[warp][r] = top[r], sums[warp][r] = sum[r];
+    __syncthreads();
+    if (threadIdx.x < ROWS && slots[threadIdx.x] >= 0) {
+        float t = tops[0][threadIdx.x], s = sums[0][threadIdx.x];
+        for (int w = 1; w < 8; ++w) {
+            const float m = tops[w][threadIdx.x], both = fmaxf(t, m);
+            s = s * exp2f(t - both) + sums[w][threadIdx.x] * exp2f(m - both);
+            t = both;
+        }
+        const i64 to = blockIdx.x * p.part_stride + slots[threadIdx.x];
+        p.part_max[to] = t, p.part_sum[to] = s;
+    }
+}
+
 // ---------------------------------------------------------------------------------------------- after the products
 // Eight rows of a chunk to a block: joins what the parts of the columns left, in a fixed order (eight threads read a sector, 32 parts
 // at a time), to lse and the loss of a row; then a warp has a row.  Where E is kept, the row's E gets its entries and the packed row its factor.
 // `again`: the tiles that were made a second time.
+//
+// The tensor cores cut their sums off at each step of 16 terms, always towards 0, so a sum that grows all along, as the logit of a token
+// that the row points to does, comes out short by 1e-8 to 1e-7 of itself a step (measured; 5e-6 in bf16 and 1e-5 in fp16 at
+// a width of 4 096).  Against that the target's logit is summed once more in rounded 32 bits, in the loss and in lse.
+constexpr int REFINED_DIM = 512;
 template <class T>
 __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, bool again, unsigned int all_tickets) {
     next_may_come();
@@ -363,10 +476,28 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
         T *scaled = (T *)p.scaled + m * p.dim_padded;
         if (m < n) {
             const int row = p.row_of[slot];
-            const float lse2 = lse2s[warp], ref = refs[warp];
-            const float less = exp2f(lse2 - ref);  // keep: a share in the units of E
+            float lse2 = lse2s[warp];
+            const float ref = refs[warp];
             const int2 *e = p.entries + (i64)row * entries_of_row;
-            const float *z = p.entry_z + slot * entries_of_row;
+            float *z = p.entry_z + slot * entries_of_row;
+            if (!p.k && !p.few && p.dim > REFINED_DIM && e[0].x != INT_MAX) {
+                const T *w = (const T *)p.weight_rows + e[0].x * p.weight_rows_stride, *h = (const T *)p.packed + slot * p.dim_padded;
+                float sum_z = 0.f;
+#pragma unroll 4
+                for (int d = lane * 8; d < p.dim_padded; d += 256) {
+                    const uint4 x = *(const uint4 *)(h + d), y = *(const uint4 *)(w + d);
+                    const T *u = (const T *)&x, *v = (const T *)&y;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum_z = fmaf((float)u[i], (float)v[i], sum_z);
+                }
+                for (int d = 16; d; d >>= 1) sum_z += __shfl_xor_sync(~0u, sum_z, d);
+                const float before = z[0], share = exp2f(fmaf(before, scale, -lse2));
+                lse2 += log1pf(share * expm1f((sum_z - before) * p.inv_temperature)) * 1.4426950408889634f;
+                __syncwarp();
+                if (lane == 0) z[0] = sum_z;
+                __syncwarp();
+            }
+            const float less = exp2f(lse2 - ref);  // keep: a share in the units of E
             float pz = 0.f;
             for (int k = lane; k < entries_of_row; k += 32) {
                 const int2 it = e[k];
@@ -547,6 +678,8 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     p.group = group_of(p.keep && p.chunk_rows < p.rows ? p.chunk_rows : p.rows, a->vocab, 0, 0, a->dim, 0, false, false);
     p.parts = (int)((a->vocab + 64 * p.group - 1) / (64 * p.group));
     p.part_stride = p.chunk_rows;
+    p.few = !p.want_grads && !p.k && aligned && p.rows > 0 && p.rows <= FEW_ROWS && p.dim * (p.rows <= 2 ? p.rows : p.rows <= 4 ? 4 : 8) <= FEW_NUMBERS;
+    if (p.few) p.parts = (int)(a->vocab < 8 * 4 * 2 * SMS ? (a->vocab + 31) / 32 : 2 * SMS), p.part_stride = FEW_ROWS;
     p.acc_stride = up_to(a->dim, 32);
     bytes = 0;
     char *base = (char *)a->workspace;
@@ -569,8 +702,8 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     if (!p.lse2) p.lse2 = (float *)take(p.rows_padded * 4);
     if (p.want_loss) {
         p.entry_z = (float *)take(p.rows_padded * 4 * (p.k ? p.k : 1));
-        p.part_max = (float *)take(p.chunk_rows * 4 * p.parts);
-        p.part_sum = (float *)take(p.chunk_rows * 4 * p.parts);
+        p.part_max = (float *)take(p.part_stride * 4 * p.parts);
+        p.part_sum = (float *)take(p.part_stride * 4 * p.parts);
         p.row_loss = a->reduction == STBPE_REDUCE_NONE ? a->loss : (float *)take(p.rows_padded * 4);
     }
     if (p.want_grads) {
@@ -663,6 +796,12 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
     auto map = [&](CUtensorMap *m, const void *at, i64 rows, i64 cols, i64 stride, int box) {
         return tensor_map(m, type, at, rows, cols, stride, box, err, err_len);
     };
+    if (p.few) {
+        auto *few = p.rows == 1 ? few_kernel<T, 1> : p.rows == 2 ? few_kernel<T, 2> : p.rows <= 4 ? few_kernel<T, 4> : few_kernel<T, 8>;
+        VCK(start(few, p.parts, 256, 0, 1, s, p));
+        VCK(start(join_kernel<T>, 1, 256, 0, 1, s, p, 0, p.rows_padded, false, 1));
+        return STBPE_OK;
+    }
     if (p.k) {
         auto *teacher = p.k <= 32 ? teacher_kernel<1> : p.k <= 64 ? teacher_kernel<2> : p.k <= 128 ? teacher_kernel<4> : teacher_kernel<8>;
         VCK(start(teacher, blocks(p.rows, 4), 128, 0, 1, s, p));

@@ -32,7 +32,7 @@ struct Plan {
     i64 rows, inner;  // row = outer * inner + inner index
     i64 vocab, dim, dim_padded, rows_padded;
     int k, pieces, parts, reduction, group;
-    bool want_loss, want_grads;
+    bool want_loss, want_grads, few;
     float temperature, inv_temperature;
     const void *hidden, *weight, *ids, *logits;
     const unsigned char *valid;

@@ -496,3 +496,22 @@ def test_splits_of_the_depth():
     check(*make(1, 5, 64, 40_000))
     check(*make(2, 2500, 72, 130))
     check(*make(1, 300, 520, 20_000, 3))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,D,V", [(1, 8, 1), (1, 1024, 8256), (2, 64, 33), (3, 2000, 50_001), (4, 256, 9473), (8, 520, 20_011),
+                                      (8, 2048, 700), (8, 2056, 700), (9, 512, 3000), (1, 16_384, 300), (5, 70, 999)])
+def test_a_few_rows_are_scored(rows, D, V, dtype):
+    hidden, weight, targets = make(1, rows, D, V, dtype=dtype, seed=rows + V)
+    for reduction in ("none", "mean", "sum"):
+        near(ops.vocab_cross_entropy(hidden, weight, targets, reduction=reduction), formula(hidden, weight, targets, reduction=reduction), "loss")
+    valid = torch.arange(rows, device="cuda")[None] % 2 == 1
+    hidden = torch.where(valid[..., None], hidden, float("nan"))
+    want = formula(hidden, weight, targets, valid=valid)
+    near(ops.vocab_cross_entropy(hidden, weight, targets, valid), want, "loss")
+    near(ops.vocab_cross_entropy(hidden.transpose(0, 1), weight, targets.t().long(), valid.t()), want, "loss")
+    each = ops.vocab_cross_entropy(hidden, weight, torch.where(valid, targets, -1), reduction="none")
+    assert bool((each[~valid] == 0).all())
+    if rows > 1:
+        targets[0, 1] = V
+        assert ops.vocab_cross_entropy(hidden, weight, targets, valid, reduction="none").isnan().nonzero().tolist() == [[0, 1]]
