@@ -120,11 +120,9 @@ def _run(a: L.VocabLoss, device: torch.device) -> None:
         _raise(st, err.value.decode())
 
 
-def _loss(hidden, weight, ids, logits, valid, temperature, reduction, for_backward=False):
-    """The loss, and what the gradients need of it again."""
-    a = _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
-    shape = hidden.shape[:-1]
-    loss = hidden.new_empty(shape if reduction == "none" else (), dtype=torch.float32)
+def _loss(a, hidden, reduction, for_backward=False):
+    """The loss, and what the gradients need of it again; ``a``: the arguments."""
+    loss = hidden.new_empty(hidden.shape[:-1] if reduction == "none" else (), dtype=torch.float32)
     lse2 = hidden.new_empty(max(1, a.outer * a.inner), dtype=torch.float32) if for_backward else None
     a.want, a.loss, a.lse2 = _WANT_LOSS, loss.data_ptr(), lse2.data_ptr() if for_backward else None
     if loss.numel():
@@ -132,10 +130,8 @@ def _loss(hidden, weight, ids, logits, valid, temperature, reduction, for_backwa
     return loss, lse2
 
 
-def _grads(hidden, weight, ids, logits, valid, temperature, reduction, grad_loss, lse2, want_hidden=True, want_weight=True,
-           for_backward=False):
+def _grads(a, hidden, weight, reduction, grad_loss, lse2, want_hidden=True, want_weight=True, for_backward=False):
     """(loss or None, grad_hidden or None, grad_weight or None, lse2 or None); without ``lse2`` the loss is made, too."""
-    a = _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
     shape, loss = hidden.shape[:-1], None
     if grad_loss is not None:
         if not isinstance(grad_loss, torch.Tensor):
@@ -157,9 +153,9 @@ def _grads(hidden, weight, ids, logits, valid, temperature, reduction, grad_loss
         if for_backward:
             lse2 = hidden.new_empty(max(1, a.outer * a.inner), dtype=torch.float32)
         # (a tensor without elements has no address, and nothing is written to where it would be)
-        a.want, a.loss = _WANT_LOSS | _WANT_GRADS, (loss if loss.numel() else gw if gw is not None else weight).data_ptr()
+        a.want, a.loss = _WANT_LOSS | _WANT_GRADS, loss.data_ptr() or weight.data_ptr()
     a.lse2 = lse2.data_ptr() if lse2 is not None else None
-    a.grad_hidden = gh.data_ptr() if want_hidden and gh.numel() else None
+    a.grad_hidden = gh.data_ptr() or None if want_hidden else None
     a.grad_weight = gw.data_ptr() if want_weight else None
     if loss is not None or a.grad_hidden or a.grad_weight:
         _run(a, hidden.device)
@@ -173,36 +169,40 @@ class _VocabLoss(torch.autograd.Function):
     and for a second backward pass, the gradients are made from the saved sums."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, ids, logits, valid, temperature, reduction):
-        ctx.temperature, ctx.reduction, ctx.grads = temperature, reduction, None
+    def forward(ctx, hidden, weight, ids, logits, valid, a, temperature, reduction):
+        ctx.how, ctx.grads = (temperature, reduction), None
         if hidden.dtype == torch.bfloat16 and reduction != "none":
-            loss, gh, gw, lse2 = _grads(hidden, weight, ids, logits, valid, temperature, reduction, None, None,
-                                        ctx.needs_input_grad[0], ctx.needs_input_grad[1], for_backward=True)
+            wanted = ctx.needs_input_grad
+            loss, gh, gw, lse2 = _grads(a, hidden, weight, reduction, None, None, wanted[0], wanted[1], for_backward=True)
             ctx.grads = gh, gw
         else:
-            loss, lse2 = _loss(hidden, weight, ids, logits, valid, temperature, reduction, for_backward=True)
+            loss, lse2 = _loss(a, hidden, reduction, for_backward=True)
         ctx.save_for_backward(hidden, weight, ids, logits, valid, lse2)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        hidden, weight, ids, logits, valid, lse2 = ctx.saved_tensors
-        _refuse_capture(hidden.device)
+        _refuse_capture(grad_loss.device)
         if ctx.grads is not None:
             (gh, gw), ctx.grads = ctx.grads, None  # they are given away: a second pass makes its own
             _scale(gh, gw, grad_loss)
         else:
-            _, gh, gw, _ = _grads(hidden, weight, ids, logits, valid, ctx.temperature, ctx.reduction, grad_loss, lse2,
-                                  ctx.needs_input_grad[0], ctx.needs_input_grad[1])
-        return gh, gw, None, None, None, None, None
+            hidden, weight, ids, logits, valid, lse2 = ctx.saved_tensors
+            temperature, reduction = ctx.how
+            a = _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
+            _, gh, gw, _ = _grads(a, hidden, weight, reduction, grad_loss, lse2, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return gh, gw, None, None, None, None, None, None
 
 
 def _scale(gh: Optional[torch.Tensor], gw: Optional[torch.Tensor], by: torch.Tensor) -> None:
-    with torch.cuda.device(by.device):
-        st = L.load().stbpe_scale_gradients(gh.data_ptr() if gh is not None else None, gh.numel() if gh is not None else 0,
-                                            gw.data_ptr() if gw is not None else None, gw.numel() if gw is not None else 0,
-                                            by.data_ptr(), torch.cuda.current_stream(by.device).cuda_stream)
+    index = by.device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _scale(gh, gw, by)
+    st = L.load().stbpe_scale_gradients(gh.data_ptr() if gh is not None else None, gh.numel() if gh is not None else 0,
+                                        gw.data_ptr() if gw is not None else None, gw.numel() if gw is not None else 0,
+                                        by.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
     if st != L.OK:
         _raise(st, f"stbpe_scale_gradients failed with status {st}")
 
@@ -210,18 +210,20 @@ def _scale(gh: Optional[torch.Tensor], gw: Optional[torch.Tensor], by: torch.Ten
 def _refuse_capture(device: torch.device) -> None:
     """torch adds a leaf's gradient on the stream that the leaf was first used on.  A captured backward pass reaches out
     of its capture there when an eager graph of the same leaf is alive, which torch answers by ending the process."""
-    with torch.cuda.device(device):
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a loss with autograd cannot be captured: capture the call that returns the gradients "
-                               "(vocab_cross_entropy_grads, vocab_distillation_grads)")
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _refuse_capture(device)
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a loss with autograd cannot be captured: capture the call that returns the gradients "
+                           "(vocab_cross_entropy_grads, vocab_distillation_grads)")
 
 
 def _differentiable(hidden, weight, ids, logits, valid, temperature, reduction):
-    if torch.is_grad_enabled() and (getattr(hidden, "requires_grad", False) or getattr(weight, "requires_grad", False)):
-        _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
+    a = _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
+    if (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
         _refuse_capture(hidden.device)
-        return _VocabLoss.apply(hidden, weight, ids, logits, valid, temperature, reduction)
-    return _loss(hidden, weight, ids, logits, valid, temperature, reduction)[0]
+        return _VocabLoss.apply(hidden, weight, ids, logits, valid, a, temperature, reduction)
+    return _loss(a, hidden, reduction)[0]
 
 
 def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
@@ -238,8 +240,7 @@ def vocab_cross_entropy_grads(hidden: torch.Tensor, weight: torch.Tensor, target
     """``(loss, grad_hidden, grad_weight)`` in one call without autograd, which can be captured into a graph.  The
     gradients are contiguous, in the inputs' type, and times ``grad_loss``: a number, a float32 tensor of one element (a loss
     scale), or with ``reduction="none"`` one of the loss's shape."""
-    with torch.no_grad():
-        return _grads(hidden, weight, targets, None, valid, 1.0, reduction, grad_loss, None)[:3]
+    return _grads(_arguments(hidden, weight, targets, None, valid, 1.0, reduction), hidden, weight, reduction, grad_loss, None)[:3]
 
 
 def vocab_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor,
@@ -260,5 +261,5 @@ def vocab_distillation_grads(hidden: torch.Tensor, weight: torch.Tensor, teacher
     """``(loss, grad_hidden, grad_weight)`` of ``vocab_distillation``, as ``vocab_cross_entropy_grads`` gives them."""
     if teacher_logits is None:
         raise TypeError("teacher_logits must be a tensor")
-    with torch.no_grad():
-        return _grads(hidden, weight, teacher_ids, teacher_logits, valid, float(temperature), reduction, grad_loss, None)[:3]
+    a = _arguments(hidden, weight, teacher_ids, teacher_logits, valid, float(temperature), reduction)
+    return _grads(a, hidden, weight, reduction, grad_loss, None)[:3]
