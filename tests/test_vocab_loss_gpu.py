@@ -515,3 +515,35 @@ def test_a_few_rows_are_scored(rows, D, V, dtype):
     if rows > 1:
         targets[0, 1] = V
         assert ops.vocab_cross_entropy(hidden, weight, targets, valid, reduction="none").isnan().nonzero().tolist() == [[0, 1]]
+
+
+@pytest.mark.parametrize("N,V,D", [(300, 530_003, 4096), (2048, 1_100_003, 64)])
+def test_offsets_beyond_31_bits(N, V, D):
+    """More than 2^31 numbers in the weight and its gradient, or in what is held of the exponentials; checked by columns."""
+    hidden, weight, targets = make(1, N, D, V)
+    targets[0, -3:] = torch.tensor([V - 1, V - 2, 0], device="cuda")
+    loss, gh, gw = ops.vocab_cross_entropy_grads(hidden, weight, targets, grad_loss=float(N))
+    h, t = hidden[0].double(), targets[0].long()
+    spans = [(v, min(v + 65536, V)) for v in range(0, V, 65536)]
+    logits = lambda a, b: h @ weight[a:b].double().T  # noqa: E731
+    dz = lambda a, b: (D + 4) * E32 * (h.abs() @ weight[a:b].double().abs().T)  # noqa: E731
+    lse = torch.logsumexp(torch.stack([torch.logsumexp(logits(a, b), 1) for a, b in spans]), 0)
+    off = torch.stack([dz(a, b).amax(1) for a, b in spans]).amax(0)
+    zt = (h * weight[t].double()).sum(1)
+    tol = 2 * off + 16 * E32 * (1 + lse.abs() + zt.abs())
+    assert abs(float(loss) - float((lse - zt).mean())) <= float(tol.mean()) + (N / 32 + 64) * E32 * float((lse - zt).abs().mean())
+    u, full, full_tol = 2.0 ** -8, torch.zeros_like(h), torch.zeros_like(h)
+    for a, b in spans:
+        w = weight[a:b].double()
+        q = (logits(a, b) - lse[:, None]).exp()
+        aim = torch.zeros_like(q)
+        inside = (t >= a) & (t < b)
+        aim[inside, t[inside] - a] = 1.0
+        G = q - aim
+        dG = u * G.abs() + (q + aim) * (2 * off + 16 * E32 * (1 + lse.abs()))[:, None] * (1 + u)
+        full += G @ w
+        full_tol += dG @ w.abs() + (V + 4) * E32 * (G.abs() @ w.abs())
+        want = G.T @ h
+        bound = (dG + (u + u * u) * G.abs()).T @ h.abs() + (N + 4) * E32 * (G.abs().T @ h.abs())
+        assert bool(((gw[a:b].double() - want).abs() <= bound + u * (want.abs() + bound) + 2.0 ** -133).all())
+    assert bool(((gh[0].double() - full).abs() <= full_tol + u * (full.abs() + full_tol) + 2.0 ** -133).all())
