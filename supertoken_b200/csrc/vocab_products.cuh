@@ -36,9 +36,8 @@ constexpr int SPLITS = 8;
 constexpr int PRODUCT_THREADS = 384;
 constexpr int PRODUCT_SMEM = STAGES * STAGE_BYTES + 1024 + 256 + 8 * 2048;
 
-// How the tiles of one or two results are dealt out: whole ones in rounds of all clusters, first those of the first result, and those
-// that are left behind the full rounds split in depth, up to SPLITS units per tile of SPLIT_STEPS steps at least, so that the last
-// round is shorter, too.  Joining the units of a tile costs about as much as JOIN_STEPS steps.
+// How the tiles of one or two results are dealt out: whole ones in rounds of all clusters, and those that are left behind a result's full
+// rounds split in depth, up to SPLITS units per tile of SPLIT_STEPS steps at least, so that the last round is shorter, too.  Joining the units of a tile costs about as much as JOIN_STEPS steps.
 constexpr int SPLIT_STEPS = 16, JOIN_STEPS = 14;
 struct Deal {
     unsigned whole[2], left[2], splits[2], units;
@@ -336,17 +335,16 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
     };
     auto unit_at = [&](unsigned u) {  // (32-bit divisions: this stands between two tiles)
         Unit t;
-        const unsigned whole = dealt.whole[0] + dealt.whole[1], first = dealt.left[0] * dealt.splits[0];
-        unsigned tile;
+        // dH, whose tiles go deeper as a rule, and what is left of it, then dW
+        const unsigned first = dealt.left[0] * dealt.splits[0];
+        t.result = u >= dealt.whole[0] + first;
+        unsigned x = t.result ? u - dealt.whole[0] - first : u, tile = x;
+        const unsigned whole = t.result ? dealt.whole[1] : dealt.whole[0], left = t.result ? dealt.left[1] : dealt.left[0];
         t.split = -1, t.splits = 1, t.sums = t.done = 0;
-        if (u < whole) {
-            t.result = u >= dealt.whole[0];
-            tile = t.result ? u - dealt.whole[0] : u;
-        } else {
-            t.result = u - whole >= first;
-            const unsigned x = t.result ? u - whole - first : u - whole, left = t.result ? dealt.left[1] : dealt.left[0];
+        if (x >= whole) {
+            x -= whole;
             const unsigned split = x / left, index = x - split * left;
-            tile = (t.result ? dealt.whole[1] : dealt.whole[0]) + index;
+            tile = whole + index;
             t.splits = (int)(t.result ? dealt.splits[1] : dealt.splits[0]);
             if (t.splits > 1) {
                 t.split = (int)split;
