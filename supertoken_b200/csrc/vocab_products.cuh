@@ -32,7 +32,7 @@ enum { STATS, MAKE_E, MAKE_G, GRADS };
 constexpr int STAGES = 6;
 constexpr int OPERAND_BYTES = 128 * 64 * 2;  // what a CTA loads of one operand per step of 64 terms
 constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
-constexpr int SPLITS = 8;
+constexpr int SPLITS = 4;  // (8: nothing gained where 129 steps are split, and more registers)
 constexpr int PRODUCT_THREADS = 384;
 constexpr int PRODUCT_SMEM = STAGES * STAGE_BYTES + 1024 + 256 + 8 * 2048;
 
@@ -51,8 +51,8 @@ __host__ __device__ inline Deal deal(const unsigned (&tiles)[2], const unsigned 
         rounds += d.whole[r] / clusters * steps[r];
     }
     unsigned best = UINT_MAX;
-    for (unsigned a = 1; a <= (may_split[0] && d.left[0] ? SPLITS : 1); a *= 2)
-        for (unsigned b = 1; b <= (may_split[1] && d.left[1] ? SPLITS : 1); b *= 2) {
+    for (unsigned a = 1; a <= (may_split[0] && d.left[0] ? SPLITS : 1); ++a)
+        for (unsigned b = 1; b <= (may_split[1] && d.left[1] ? SPLITS : 1); ++b) {
             if ((a > 1 && (steps[0] < a * SPLIT_STEPS || d.left[0] * a > clusters)) || (b > 1 && (steps[1] < b * SPLIT_STEPS || d.left[1] * b > clusters)))
                 continue;
             const unsigned x = d.left[0] ? steps[0] / a + (a > 1 ? JOIN_STEPS : 0) : 0, y = d.left[1] ? steps[1] / b + (b > 1 ? JOIN_STEPS : 0) : 0;
