@@ -163,8 +163,8 @@ __device__ __forceinline__ void copy_row(T *to, const T *from, i64 inside, i64 a
 }
 
 // Which rows count, in their order (row_of, slot_of); the entry of a cross entropy row; what each counted row's dlogits are
-// multiplied by.  Every block goes through all rows by itself, 8 192 at a time, so that no launch lies between their numbers and
-// what follows; the first one writes them down.
+// multiplied by.  Every block has a range of the rows and counts by itself those that count before it, and all of them, eight loads
+// of a thread on their way at a time, so that no launch lies between the rows' numbers and what follows.
 // Then counted rows of `hidden` go one behind another, zeros up to the end of the last tile, a warp to a row: products then do no
 // work for padding, never multiply what a masked row holds (it may be NaN), and may read rows of any stride or alignment.  The
 // rows of dH that do not count get their zeros here.
@@ -181,90 +181,78 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
             copy_row((T *)p.weight_rows + j * p.dim_padded, (const T *)p.weight + j * p.weight_stride, p.dim, p.dim_padded, threadIdx.x & 31);
         return;
     }
-    constexpr int EACH = 8;  // rows of a thread, 1024 apart: their loads are in flight together
-    __shared__ int in_warp[EACH * 32], slots[EACH * 1024];
-    __shared__ int base;
-    __shared__ float part[32];
+    __shared__ int befores[32], alls[32], in_warp[32], slots[1024];
+    __shared__ float mosts[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const i64 each_block = (p.rows + p.row_blocks - 1) / p.row_blocks;
+    const i64 start = blockIdx.x * each_block, end = start + each_block < p.rows ? start + each_block : p.rows;
+    const bool last = blockIdx.x == p.row_blocks - 1;
     const bool each = p.want_grads && p.reduction == STBPE_REDUCE_NONE && p.grad_loss;
     const float one = p.want_grads && p.grad_loss && !each && p.rows > 0 ? p.grad_loss[0] : 1.f;
-    float most = fabsf(one);
-    if (each) most = 0.f;
-    if (threadIdx.x == 0) base = 0;
-    const bool first = blockIdx.x == 0;
-    if (first && p.split_done)
-        for (int x = threadIdx.x; x < 2 * SMS * 8; x += 1024) p.split_done[x] = 0;
-    for (i64 r0 = 0; r0 < p.rows; r0 += EACH * 1024) {
-        bool counted[EACH];
-        unsigned votes[EACH];
-        float nan[EACH], up[EACH];
-#pragma unroll
-        for (int x = 0; x < EACH; ++x) {
-            const i64 row = r0 + x * 1024 + threadIdx.x;
-            counted[x] = false, up[x] = 1.f, nan[x] = 0.f;
-            if (row < p.rows) {
-                const i64 o = (unsigned)row / (unsigned)p.inner, i = row - o * p.inner;
-                counted[x] = !p.valid || p.valid[o * p.valid_outer + i * p.valid_inner];
-                if (each) up[x] = p.grad_loss[o * p.grad_outer + i * p.grad_inner];
-                if (p.k) {
-                    counted[x] = counted[x] && p.has_entries[row];
-                    nan[x] = p.plogp[row] * 0.f;
-                } else {
-                    const i64 id = load_id(p.ids, p.ids_bytes, o * p.ids_outer + i * p.ids_inner);
-                    counted[x] = counted[x] && id >= 0;
-                    nan[x] = id >= p.vocab ? NAN : 0.f;
-                    if (first) p.entries[row] = make_int2(id >= p.vocab || id < 0 ? INT_MAX : (int)id, __float_as_int(1.f));
-                    if (first) p.plogp[row] = nan[x];
-                }
+    auto counts = [&](i64 row, i64 &id) {
+        const i64 o = (unsigned)row / (unsigned)p.inner, i = row - o * p.inner;
+        const bool there = !p.valid || p.valid[o * p.valid_outer + i * p.valid_inner];
+        if (p.k) return there && p.has_entries[row];
+        id = load_id(p.ids, p.ids_bytes, o * p.ids_outer + i * p.ids_inner);
+        return there && id >= 0;
+    };
+    auto grad_of = [&](i64 row) {
+        const i64 o = (unsigned)row / (unsigned)p.inner, i = row - o * p.inner;
+        return p.grad_loss[o * p.grad_outer + i * p.grad_inner];
+    };
+    int before = 0, all = 0;
+    float most = each ? 0.f : fabsf(one);
+#pragma unroll 8
+    for (i64 row = threadIdx.x; row < p.rows; row += 1024) {
+        i64 id;
+        const bool counted = counts(row, id);
+        all += counted, before += counted && row < start;
+        if (each && last && counted) most = fmaxf(most, fabsf(grad_of(row)));
+    }
+    for (int d = 16; d; d >>= 1) {
+        before += __shfl_xor_sync(~0u, before, d), all += __shfl_xor_sync(~0u, all, d);
+        most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+    }
+    if (lane == 0) befores[warp] = before, alls[warp] = all, mosts[warp] = most;
+    __syncthreads();
+    before = befores[lane], all = alls[lane], most = mosts[lane];
+    for (int d = 16; d; d >>= 1) {
+        before += __shfl_xor_sync(~0u, before, d), all += __shfl_xor_sync(~0u, all, d);
+        most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+    }
+    const i64 n = all, until = (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS;
+    for (i64 r0 = start; r0 < end; r0 += 1024) {
+        const i64 row = r0 + threadIdx.x;
+        i64 id = -1;
+        const bool there = row < end, counted = there && counts(row, id);
+        const unsigned votes = __ballot_sync(~0u, counted);
+        if (lane == 0) in_warp[warp] = __popc(votes);
+        __syncthreads();
+        int slot = lane < warp ? in_warp[lane] : 0, whole = in_warp[lane];
+        for (int d = 16; d; d >>= 1) slot += __shfl_xor_sync(~0u, slot, d), whole += __shfl_xor_sync(~0u, whole, d);
+        slot += before + __popc(votes & ((1u << lane) - 1));
+        before += whole;
+        slots[threadIdx.x] = counted ? slot : -1;
+        if (there) {
+            p.slot_of[row] = counted ? slot : -1;
+            const bool outside = !p.k && id >= p.vocab;
+            float nan = outside ? NAN : 0.f;
+            if (p.k) {
+                nan = p.plogp[row] * 0.f;
+            } else {
+                p.entries[row] = make_int2(outside || id < 0 ? INT_MAX : (int)id, __float_as_int(1.f));
+                p.plogp[row] = nan;
+            }
+            if (counted) {
+                p.row_of[slot] = (int)row;
+                if (p.want_grads) p.coef[slot] = (each ? grad_of(row) : 1.f) + nan;
+            } else if (p.want_loss) {
+                p.row_loss[row] = p.lse2[row] = 0.f;
             }
         }
         __syncthreads();
-#pragma unroll
-        for (int x = 0; x < EACH; ++x) {
-            votes[x] = __ballot_sync(~0u, counted[x]);
-            if (lane == 0) in_warp[x * 32 + warp] = __popc(votes[x]);
-        }
-        __syncthreads();
-        if (warp == 0) {  // counts to places
-            int mine = 0;
-#pragma unroll
-            for (int x = 0; x < EACH; ++x) mine += in_warp[lane * EACH + x];
-            int upto = mine;
-            for (int d = 1; d < 32; d <<= 1) {
-                const int y = __shfl_up_sync(~0u, upto, d);
-                if (lane >= d) upto += y;
-            }
-            int at = base + upto - mine;
-            __syncwarp();
-#pragma unroll
-            for (int x = 0; x < EACH; ++x) {
-                const int y = in_warp[lane * EACH + x];
-                in_warp[lane * EACH + x] = at;
-                at += y;
-            }
-            if (lane == 31) base = at;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int x = 0; x < EACH; ++x) {
-            const i64 row = r0 + x * 1024 + threadIdx.x;
-            const int slot = in_warp[x * 32 + warp] + __popc(votes[x] & ((1u << lane) - 1));
-            if (row < p.rows && first) {
-                p.slot_of[row] = counted[x] ? slot : -1;
-                if (counted[x]) {
-                    p.row_of[slot] = (int)row;
-                    if (p.want_grads) p.coef[slot] = up[x] + nan[x];
-                    if (each) most = fmaxf(most, fabsf(up[x]));
-                } else if (p.want_loss) {
-                    p.row_loss[row] = p.lse2[row] = 0.f;
-                }
-            }
-            slots[x * 1024 + threadIdx.x] = counted[x] ? slot : -1;
-        }
-        __syncthreads();
-        // every p.row_blocks-th row is this block's, one at a time to a warp
-        const i64 end = p.rows - r0 < EACH * 1024 ? p.rows - r0 : EACH * 1024;
-        for (i64 y = blockIdx.x + (i64)warp * p.row_blocks; y < end; y += (i64)p.row_blocks * 32) {
+        const i64 here = end - r0 < 1024 ? end - r0 : 1024;
+        for (i64 y = warp; y < here; y += 32) {
             const i64 its = r0 + y;
             const int to = slots[y];
             if (to >= 0) {
@@ -279,31 +267,26 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
                     for (int d = lane; d < p.dim; d += 32) at[d] = T(0.f);
             }
         }
-    }
-    __syncthreads();
-    const int n = base;
-    const i64 until = (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS;
-    for (i64 c = n + blockIdx.x * 32 + warp; c < until; c += p.row_blocks * 32)
-        for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)((T *)p.packed + c * p.dim_padded + d) = make_uint4(0, 0, 0, 0);
-    if (!first) return;
-    for (i64 c = n + threadIdx.x; c < p.rows_padded; c += 1024) p.row_of[c] = -1;
-    if (p.keep) {
-        for (i64 c = threadIdx.x; c < p.rows_padded; c += 1024) p.reference[c] = 0.f;
-        for (i64 c = threadIdx.x; c < p.rows_padded / TILE_ROWS; c += 1024) p.again[c] = 0;
-    }
-    if (each) {
-        for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
-        if (lane == 0) part[warp] = most;
         __syncthreads();
-        for (int w = 0; w < 32; ++w) most = fmaxf(most, part[w]);
     }
+    for (i64 c = n + blockIdx.x + warp * p.row_blocks; c < until; c += p.row_blocks * 32)
+        for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)((T *)p.packed + c * p.dim_padded + d) = make_uint4(0, 0, 0, 0);
+    const i64 step = (i64)p.row_blocks * 1024;
+    for (i64 c = n + blockIdx.x * 1024 + threadIdx.x; c < p.rows_padded; c += step) p.row_of[c] = -1;
+    if (p.keep) {
+        for (i64 c = blockIdx.x * 1024 + threadIdx.x; c < p.rows_padded; c += step) p.reference[c] = 0.f;
+        for (i64 c = blockIdx.x * 1024 + threadIdx.x; c < p.rows_padded / TILE_ROWS; c += step) p.again[c] = 0;
+    }
+    if (!last) return;
+    if (p.split_done)
+        for (int x = threadIdx.x; x < 2 * SMS * 8; x += 1024) p.split_done[x] = 0;
     if (threadIdx.x == 0) {
         const float factor = p.temperature / (p.reduction == STBPE_REDUCE_MEAN ? (float)(n > 0 ? n : 1) : 1.f);
         most *= factor;
         int up = 0;  // the next power of two, both sides kept within what 32 bits hold as normal numbers
         if (most > 0.f && most < INFINITY) frexpf(most, &up);
         up = max(-100, min(100, up));
-        p.meta->counted = n, p.meta->tickets = 0, p.meta->again = 0;
+        p.meta->counted = (int)n, p.meta->tickets = 0, p.meta->again = 0;
         p.meta->in_scale = (each ? 1.f : one) * factor * ldexpf(1.f, 14 - up);
         p.meta->out_scale = ldexpf(1.f, up - 14);
     }
@@ -447,6 +430,12 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
             sum = p.keep ? sum + x : sum * exp2f(top - both) + x * exp2f(m - both);
             top = both;
         };
+        // the row of this warp; the sum of its target's logit needs nothing of the parts
+        const i64 m = m0 + warp, slot = r0 + m;
+        const int row = m < n ? p.row_of[slot] : 0;
+        const int2 *e = p.entries + (i64)row * entries_of_row;
+        const bool refined = m < n && !p.k && !p.few && p.dim > REFINED_DIM && e[0].x != INT_MAX;
+        float sum_z = 0.f;
         if (m0 + (lane & 7) < n) {
             const float *from_max = p.part_max + m0 + (lane & 7), *from_sum = p.part_sum + m0 + (lane & 7);
 #pragma unroll 4
@@ -455,6 +444,17 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
         for (int d = 8; d < 32; d <<= 1) {
             const float m = __shfl_xor_sync(~0u, top, d), x = __shfl_xor_sync(~0u, sum, d);
             add(m, x);
+        }
+        if (refined) {
+            const T *w = (const T *)p.weight_rows + e[0].x * p.weight_rows_stride, *h = (const T *)p.packed + slot * p.dim_padded;
+#pragma unroll 4
+            for (int d = lane * 8; d < p.dim_padded; d += 256) {
+                const uint4 x = *(const uint4 *)(h + d), y = *(const uint4 *)(w + d);
+                const T *u = (const T *)&x, *v = (const T *)&y;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum_z = fmaf((float)u[i], (float)v[i], sum_z);
+            }
+            for (int d = 16; d; d >>= 1) sum_z += __shfl_xor_sync(~0u, sum_z, d);
         }
         if (lane < 8) tops[warp][lane] = top, sums[warp][lane] = sum;
         __syncthreads();
@@ -472,25 +472,12 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
             refs[lane] = ref, lse2s[lane] = ref + log2f(sum);
         }
         __syncthreads();
-        const i64 m = m0 + warp, slot = r0 + m;
         T *scaled = (T *)p.scaled + m * p.dim_padded;
         if (m < n) {
-            const int row = p.row_of[slot];
             float lse2 = lse2s[warp];
             const float ref = refs[warp];
-            const int2 *e = p.entries + (i64)row * entries_of_row;
             float *z = p.entry_z + slot * entries_of_row;
-            if (!p.k && !p.few && p.dim > REFINED_DIM && e[0].x != INT_MAX) {
-                const T *w = (const T *)p.weight_rows + e[0].x * p.weight_rows_stride, *h = (const T *)p.packed + slot * p.dim_padded;
-                float sum_z = 0.f;
-#pragma unroll 4
-                for (int d = lane * 8; d < p.dim_padded; d += 256) {
-                    const uint4 x = *(const uint4 *)(h + d), y = *(const uint4 *)(w + d);
-                    const T *u = (const T *)&x, *v = (const T *)&y;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sum_z = fmaf((float)u[i], (float)v[i], sum_z);
-                }
-                for (int d = 16; d; d >>= 1) sum_z += __shfl_xor_sync(~0u, sum_z, d);
+            if (refined) {
                 const float before = z[0], share = exp2f(fmaf(before, scale, -lse2));
                 lse2 += log1pf(share * expm1f((sum_z - before) * p.inv_temperature)) * 1.4426950408889634f;
                 __syncwarp();
