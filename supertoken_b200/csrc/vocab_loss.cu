@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
     for (i64 c = n + blockIdx.x * 1024 + threadIdx.x; c < p.rows_padded; c += step) p.row_of[c] = -1;
     if (p.keep) {
         for (i64 c = blockIdx.x * 1024 + threadIdx.x; c < p.rows_padded; c += step) p.reference[c] = 0.f;
-        for (i64 c = blockIdx.x * 1024 + threadIdx.x; c < p.rows_padded / TILE_ROWS; c += step) p.again[c] = 0;
+        for (i64 c = blockIdx.x * 1024 + threadIdx.x; c < 2 * p.rows_padded / TILE_ROWS; c += step) p.again[c] = 0;
     }
     if (!last) return;
     if (p.split_done)
@@ -403,14 +403,8 @@ __global__ void __launch_bounds__(256) few_kernel(Plan p) {
 // ---------------------------------------------------------------------------------------------- after the products
 // Eight rows of a chunk to a block: joins what the parts of the columns left, in a fixed order (eight threads read a sector, 32 parts
 // at a time), to lse and the loss of a row; then a warp has a row.  Where E is kept, the row's E gets its entries and the packed row its factor.
-// `again`: the tiles that were made a second time.
-//
-// The tensor cores cut their sums off at each step of 16 terms, always towards 0, so a sum that grows all along, as the logit of a token
-// that the row points to does, comes out short by 1e-8 to 1e-7 of itself a step (measured; 5e-6 in bf16 and 1e-5 in fp16 at
-// a width of 4 096).  Against that the target's logit is summed once more in rounded 32 bits, in the loss and in lse.
-constexpr int REFINED_DIM = 512;
 template <class T>
-__global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, bool again, unsigned int all_tickets) {
+__global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows) {
     next_may_come();
     before_is_done();
     __shared__ float tops[8][8], sums[8][8], lse2s[8], refs[8];
@@ -418,11 +412,8 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const i64 counted = p.meta->counted;
     const i64 n = counted - r0 < 0 ? 0 : counted - r0 < rows ? counted - r0 : rows;
-    const i64 until = again && !p.meta->again ? 0 : p.keep ? (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS : n;
-    const int entries_of_row = p.k ? p.k : 1;
-    const float scale = p.inv_temperature * 1.4426950408889634f;
+    const i64 until = p.keep ? (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS : n;
     for (i64 m0 = (i64)blockIdx.x * 8; m0 < until; m0 += (i64)gridDim.x * 8) {
-        if (again && !p.again[(r0 + m0) / TILE_ROWS]) continue;
         float top = LOWEST, sum = 0.f;
         auto add = [&](float m, float x) {
             const float both = fmaxf(top, m);
@@ -433,8 +424,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
         // the row of this warp; the sum of its target's logit needs nothing of the parts
         const i64 m = m0 + warp, slot = r0 + m;
         const int row = m < n ? p.row_of[slot] : 0;
-        const int2 *e = p.entries + (i64)row * entries_of_row;
-        const bool refined = m < n && !p.k && !p.few && p.dim > REFINED_DIM && e[0].x != INT_MAX;
+        const bool refined = m < n && is_refined(p, row);
         float sum_z = 0.f;
         if (m0 + (lane & 7) < n) {
             const float *from_max = p.part_max + m0 + (lane & 7), *from_sum = p.part_sum + m0 + (lane & 7);
@@ -445,17 +435,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
             const float m = __shfl_xor_sync(~0u, top, d), x = __shfl_xor_sync(~0u, sum, d);
             add(m, x);
         }
-        if (refined) {
-            const T *w = (const T *)p.weight_rows + e[0].x * p.weight_rows_stride, *h = (const T *)p.packed + slot * p.dim_padded;
-#pragma unroll 4
-            for (int d = lane * 8; d < p.dim_padded; d += 256) {
-                const uint4 x = *(const uint4 *)(h + d), y = *(const uint4 *)(w + d);
-                const T *u = (const T *)&x, *v = (const T *)&y;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum_z = fmaf((float)u[i], (float)v[i], sum_z);
-            }
-            for (int d = 16; d; d >>= 1) sum_z += __shfl_xor_sync(~0u, sum_z, d);
-        }
+        if (refined) sum_z = target_logit<T>(p, slot, row, lane);
         if (lane < 8) tops[warp][lane] = top, sums[warp][lane] = sum;
         __syncthreads();
         if (threadIdx.x < 8) {
@@ -464,7 +444,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
             float ref = top;
             if (p.keep && m0 + lane < n) {
                 ref = p.reference[r0 + m0 + lane];
-                if (!again && fabsf(top - ref) > 96.f && fabsf(top) < INFINITY) {
+                if (fabsf(top - ref) > 96.f && fabsf(top) < INFINITY) {
                     p.reference[r0 + m0 + lane] = top;
                     p.again[(r0 + m0) / TILE_ROWS] = p.meta->again = 1;
                 }
@@ -474,57 +454,17 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, boo
         __syncthreads();
         T *scaled = (T *)p.scaled + m * p.dim_padded;
         if (m < n) {
-            float lse2 = lse2s[warp];
-            const float ref = refs[warp];
-            float *z = p.entry_z + slot * entries_of_row;
-            if (refined) {
-                const float before = z[0], share = exp2f(fmaf(before, scale, -lse2));
-                lse2 += log1pf(share * expm1f((sum_z - before) * p.inv_temperature)) * 1.4426950408889634f;
-                __syncwarp();
-                if (lane == 0) z[0] = sum_z;
-                __syncwarp();
-            }
-            const float less = exp2f(lse2 - ref);  // keep: a share in the units of E
-            float pz = 0.f;
-            for (int k = lane; k < entries_of_row; k += 32) {
-                const int2 it = e[k];
-                if (it.x == INT_MAX) break;
-                pz += __int_as_float(it.y) * z[k];
-                if (p.keep && (k == 0 || e[k - 1].x != it.x)) {  // (the same id again: its first entry takes them all)
-                    float share = __int_as_float(it.y);
-                    for (int l = k + 1; l < entries_of_row && e[l].x == it.x; ++l) share += __int_as_float(e[l].y);
-                    ((T *)p.g)[m * p.g_stride + it.x] = T(exp2f(fmaf(z[k], scale, -ref)) - share * less);
-                }
-            }
-            for (int d = 16; d; d >>= 1) pz += __shfl_xor_sync(~0u, pz, d);
-            if (lane == 0) {
-                const float tau = p.temperature;
-                p.lse2[row] = lse2;
-                p.row_loss[row] = tau * tau * (lse2 * 0.69314718055994531f + p.plogp[row] - pz * p.inv_temperature);
-            }
-            if (p.keep) {
-                const float a = p.coef[slot] * p.meta->in_scale * exp2f(ref - lse2);
-                if (lane == 0) p.out_row[slot] = a * p.meta->out_scale;
-                const T *from = (const T *)p.packed + slot * p.dim_padded;
-#pragma unroll 4
-                for (int d = lane * 8; d < p.dim_padded; d += 256) {
-                    uint4 x = *(const uint4 *)(from + d);
-                    T *v = (T *)&x;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = T((float)v[i] * a);
-                    *(uint4 *)(scaled + d) = x;
-                }
-            }
+            finish_row<T>(p, m, slot, row, lse2s[warp], refs[warp], refined, sum_z, lane);
         } else if (p.keep && m < until) {  // zeros behind the last row
             for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)(scaled + d) = make_uint4(0, 0, 0, 0);
         }
         __syncthreads();
     }
-    if (p.reduction == STBPE_REDUCE_NONE || !all_tickets) return;
+    if (p.reduction == STBPE_REDUCE_NONE || p.keep) return;  // (keep: a row may be made again, the launch for the gradients adds up)
     // the block that is through last adds the losses up, in the order of the rows
     __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(&p.meta->tickets, 1u) == all_tickets - 1;
+    if (threadIdx.x == 0) last = atomicAdd(&p.meta->tickets, 1u) == gridDim.x - 1;
     __syncthreads();
     if (!last) return;
     __threadfence();
@@ -701,7 +641,7 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
         if (p.keep) {
             p.reference = (float *)take(p.rows_padded * 4);
             p.out_row = (float *)take(p.rows_padded * 4);
-            p.again = (int *)take(p.rows_padded / TILE_ROWS * 4);
+            p.again = (int *)take(2 * p.rows_padded / TILE_ROWS * 4);
             p.scaled = take(p.chunk_rows * p.dim_padded * 2);
             if (p.chunk_rows < p.rows_padded) p.weight_acc = (float *)take(p.vocab * p.acc_stride * 4);
         } else if (p.g_stride < all) {
@@ -770,7 +710,9 @@ int product(const Plan &p, const Job &job, const Maps &maps, cudaStream_t s, cha
         one.grad_weight = nullptr;
         VTRY((product<T, KIND>(one, job, maps, s, err, err_len)));
         one.grad_weight = p.grad_weight, one.grad_hidden = nullptr;
-        return product<T, KIND>(one, job, maps, s, err, err_len);
+        Job rest = job;
+        rest.add_up = false;
+        return product<T, KIND>(one, rest, maps, s, err, err_len);
     }
     const int group = group_of(tall, p.dim, wide, p.dim, job.width, rows, !p.acc, !p.weight_acc);
     return group == 1 ? launch<T, KIND, 1>(p, job, maps, SMS, s, err, err_len) : launch<T, KIND, 2>(p, job, maps, SMS, s, err, err_len);
@@ -786,7 +728,7 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
     if (p.few) {
         auto *few = p.rows == 1 ? few_kernel<T, 1> : p.rows == 2 ? few_kernel<T, 2> : p.rows <= 4 ? few_kernel<T, 4> : few_kernel<T, 8>;
         VCK(start(few, p.parts, 256, 0, 1, s, p));
-        VCK(start(join_kernel<T>, 1, 256, 0, 1, s, p, 0, p.rows_padded, false, 1));
+        VCK(start(join_kernel<T>, 1, 256, 0, 1, s, p, 0, p.rows_padded));
         return STBPE_OK;
     }
     if (p.k) {
@@ -804,28 +746,27 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
         VTRY(map(&grads.map[2], p.g, p.chunk_rows, p.g_stride, p.g_stride, 64));
         VTRY(map(&grads.map[3], p.keep ? p.scaled : p.packed, p.keep ? p.chunk_rows : p.rows_padded, p.dim, p.dim_padded, 64));
     }
-    const unsigned joins = blocks(p.chunk_rows, 8), few = joins < SMS ? joins : (unsigned)SMS;  // (few: mostly they find nothing made again)
+    const unsigned joins = blocks(p.chunk_rows, 8);
     if (p.keep) {
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-            const unsigned tickets = few * (unsigned)((p.rows_padded + p.chunk_rows - 1) / p.chunk_rows);
             for (i64 r0 = 0; r0 < p.rows_padded; r0 += p.chunk_rows) {
-                Job job{0, p.vocab, r0, p.chunk_rows, false};
+                Job job{0, p.vocab, r0, p.chunk_rows, false, false};
                 VTRY((product<T, MAKE_E>(p, job, logits, s, err, err_len)));
-                VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, r0, p.chunk_rows, false, 0));
+                VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, r0, p.chunk_rows));
                 job.again = true;
                 VTRY((product<T, MAKE_E>(p, job, logits, s, err, err_len)));
-                VCK(start(join_kernel<T>, few, 256, 0, 1, s, p, r0, p.chunk_rows, true, tickets));
+                job.again = false, job.add_up = p.reduction != STBPE_REDUCE_NONE && r0 + p.chunk_rows >= p.rows_padded;
                 VTRY((product<T, GRADS>(p, job, grads, s, err, err_len)));
             }
         }
     } else {
         if (p.want_loss) {
-            VTRY((product<T, STATS>(p, Job{0, p.vocab, 0, p.rows_padded, false}, logits, s, err, err_len)));
-            VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, 0, p.rows_padded, false, joins));
+            VTRY((product<T, STATS>(p, Job{0, p.vocab, 0, p.rows_padded, false, false}, logits, s, err, err_len)));
+            VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, 0, p.rows_padded));
         }
         if (p.want_grads) {
             for (i64 v0 = 0; v0 < p.vocab; v0 += p.g_stride) {
-                const Job job{v0, p.vocab - v0 < p.g_stride ? p.vocab - v0 : p.g_stride, 0, p.rows_padded, false};
+                const Job job{v0, p.vocab - v0 < p.g_stride ? p.vocab - v0 : p.g_stride, 0, p.rows_padded, false, false};
                 VTRY((product<T, MAKE_G>(p, job, logits, s, err, err_len)));
                 VTRY((product<T, GRADS>(p, job, grads, s, err, err_len)));
             }

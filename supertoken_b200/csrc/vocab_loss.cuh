@@ -1,7 +1,11 @@
 // What the kernels of the losses over a large vocabulary share (vocab_loss.cu, vocab_products.cuh).
 #pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <limits.h>
 #include <stdint.h>
+
+#include "../../include/stbpe.h"
 
 namespace vloss {
 
@@ -22,7 +26,7 @@ __device__ __forceinline__ void before_is_done() { asm volatile("griddepcontrol.
 
 struct Meta {
     int counted;          // rows that count
-    unsigned int tickets; // blocks that are through with their rows' losses
+    unsigned int tickets; // blocks of the join that are through with their rows
     float in_scale;       // what coef is multiplied by in the end
     float out_scale;      // what both gradients are multiplied by in the end
     int again;            // keep: a reference was too far from its row's maximum
@@ -63,7 +67,8 @@ struct Plan {
     void *g;
     i64 g_stride, chunk_rows;
     float *reference;        // keep: per packed row
-    int *again;              // keep: [packed row / TILE_ROWS] a reference was too far from the row's maximum
+    int *again;              // keep: [packed row / TILE_ROWS] a reference was too far from the row's maximum; then, per TILE_ROWS rows,
+                             // parts that are made again
     float *out_row;          // keep: what a packed row of dH is multiplied by
     void *scaled;            // keep: packed rows of the chunk, times coef exp2(reference - lse2)
     float *acc;              // several pieces: dH of packed rows in 32 bits, [packed row][acc_stride]
@@ -73,5 +78,104 @@ struct Plan {
     float *split_sums;       // sums of tiles whose depth is split
     unsigned int *split_done;
 };
+
+// ---------------------------------------------------------------------------------------------- one row, by one warp
+// The tensor cores cut their sums off at each step of 16 terms, always towards 0, so a sum that grows all along, as the logit of a token
+// that the row points to does, comes out short by 1e-8 to 1e-7 of itself a step (measured; 5e-6 in bf16 and 1e-5 in fp16 at
+// a width of 4 096).  Against that the target's logit is summed once more in rounded 32 bits, in the loss and in lse.
+constexpr int REFINED_DIM = 512;
+
+__device__ __forceinline__ bool is_refined(const Plan &p, int row) {
+    return !p.k && !p.few && p.dim > REFINED_DIM && p.entries[row].x != INT_MAX;
+}
+
+template <class T>
+__device__ __forceinline__ float target_logit(const Plan &p, i64 slot, int row, int lane) {
+    const T *w = (const T *)p.weight_rows + p.entries[row].x * p.weight_rows_stride, *h = (const T *)p.packed + slot * p.dim_padded;
+    float z = 0.f;
+#pragma unroll 4
+    for (int d = lane * 8; d < p.dim_padded; d += 256) {
+        const uint4 x = *(const uint4 *)(h + d), y = *(const uint4 *)(w + d);
+        const T *u = (const T *)&x, *v = (const T *)&y;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z = fmaf((float)u[i], (float)v[i], z);
+    }
+    for (int d = 16; d; d >>= 1) z += __shfl_xor_sync(~0u, z, d);
+    return z;
+}
+
+// What follows from a row's lse2: its loss, and where E is kept the entries in E (from their logits in 32 bits, once rounded), the factor of its
+// dH and the packed row times it for dW.  m: its place in the chunk.
+template <class T>
+__device__ __forceinline__ void finish_row(const Plan &p, i64 m, i64 slot, int row, float lse2, float ref, bool refined, float target, int lane) {
+    const int entries_of_row = p.k ? p.k : 1;
+    const float scale = p.inv_temperature * 1.4426950408889634f;
+    const int2 *e = p.entries + (i64)row * entries_of_row;
+    float *z = p.entry_z + slot * entries_of_row;
+    if (refined) {
+        const float before = z[0], share = exp2f(fmaf(before, scale, -lse2));
+        lse2 += log1pf(share * expm1f((target - before) * p.inv_temperature)) * 1.4426950408889634f;
+        __syncwarp();
+        if (lane == 0) z[0] = target;
+        __syncwarp();
+    }
+    const float less = exp2f(lse2 - ref);  // a share in the units of E
+    float pz = 0.f;
+    for (int k = lane; k < entries_of_row; k += 32) {
+        const int2 it = e[k];
+        if (it.x == INT_MAX) break;
+        pz += __int_as_float(it.y) * z[k];
+        if (p.keep && (k == 0 || e[k - 1].x != it.x)) {  // (the same id again: its first entry takes them all)
+            float share = __int_as_float(it.y);
+            for (int l = k + 1; l < entries_of_row && e[l].x == it.x; ++l) share += __int_as_float(e[l].y);
+            ((T *)p.g)[m * p.g_stride + it.x] = T(exp2f(fmaf(z[k], scale, -ref)) - share * less);
+        }
+    }
+    for (int d = 16; d; d >>= 1) pz += __shfl_xor_sync(~0u, pz, d);
+    if (lane == 0) {
+        const float tau = p.temperature;
+        p.lse2[row] = lse2;
+        p.row_loss[row] = tau * tau * (lse2 * 0.69314718055994531f + p.plogp[row] - pz * p.inv_temperature);
+    }
+    if (p.keep) {
+        const float a = p.coef[slot] * p.meta->in_scale * exp2f(ref - lse2);
+        if (lane == 0) p.out_row[slot] = a * p.meta->out_scale;
+        const T *from = (const T *)p.packed + slot * p.dim_padded;
+        T *scaled = (T *)p.scaled + m * p.dim_padded;
+#pragma unroll 4
+        for (int d = lane * 8; d < p.dim_padded; d += 256) {
+            uint4 x = *(const uint4 *)(from + d);
+            T *v = (T *)&x;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = T((float)v[i] * a);
+            *(uint4 *)(scaled + d) = x;
+        }
+    }
+}
+
+// Joins the rows of TILE_ROWS that were made again, one after another.
+template <class T>
+__device__ __noinline__ void join_again(const Plan &p, i64 r0, i64 m0, i64 n, int lane) {
+    for (i64 m = m0; m < m0 + TILE_ROWS && m < n; ++m) {
+        const i64 slot = r0 + m;
+        const int row = p.row_of[slot];
+        float sum = 0.f;
+        for (int t = lane; t < p.parts; t += 32) sum += __ldcg(p.part_sum + t * p.part_stride + m);
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        const float ref = p.reference[slot];
+        const bool refined = is_refined(p, row);
+        finish_row<T>(p, m, slot, row, ref + log2f(sum), ref, refined, refined ? target_logit<T>(p, slot, row, lane) : 0.f, lane);
+    }
+}
+
+// The losses of all rows, in their order, by one warp.
+__device__ __forceinline__ void add_up(const Plan &p, int lane) {
+    float sum = 0.f;
+#pragma unroll 16
+    for (i64 r = lane; r < p.rows; r += 32) sum += p.row_loss[r];
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+    const int n = p.meta->counted;
+    if (lane == 0) p.loss[0] = p.reduction == STBPE_REDUCE_MEAN ? sum / (float)(n > 0 ? n : 1) : sum;
+}
 
 }  // namespace vloss

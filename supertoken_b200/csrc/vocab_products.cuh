@@ -72,6 +72,7 @@ struct Job {
     i64 v0, width;  // the piece of the vocabulary
     i64 r0, rows;   // the chunk of the packed rows
     bool again;     // MAKE_E: only where a reference was too far off
+    bool add_up;    // GRADS: the losses are added up beside the products
 };
 
 // ---------------------------------------------------------------------------------------------- instructions
@@ -454,6 +455,8 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             }
         }
         __syncwarp();
+    } else if (warp == 3) {
+        if (!LOGITS && job.add_up && blockIdx.x == 0) add_up(p, lane);
     } else if (warp >= 4) {
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const float scale = p.inv_temperature * 1.4426950408889634f;
@@ -616,6 +619,19 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             if ((KIND == STATS || KIND == MAKE_E) && row >= 0 && job.v0 + c0 < p.vocab) {
                 const i64 to = (job.v0 + c0) / COLUMNS * p.part_stride + m;
                 p.part_max[to] = top, p.part_sum[to] = sum;
+            }
+            if (KIND == MAKE_E && job.again) {
+                // the warp that is through last with the parts of these rows joins them
+                __threadfence();
+                __syncwarp();
+                const i64 m0 = t.m0 / TILE_ROWS * TILE_ROWS, high = n - m0 < TILE_ROWS ? n - m0 : TILE_ROWS;
+                const int parts = (int)((high + TILE - 1) / TILE * tiles_n[0]) * GROUP * 8;
+                int before = 0;
+                if (lane == 0) before = atomicAdd(p.again + (p.rows_padded + job.r0 + m0) / TILE_ROWS, 1);
+                if (__shfl_sync(~0u, before, 0) == parts - 1) {
+                    __threadfence();
+                    join_again<T>(p, job.r0, m0, n, lane);
+                }
             }
             if (!LOGITS && t.split >= 0) {
                 // the last of the splits to get here adds them up, in their order
