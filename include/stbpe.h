@@ -333,7 +333,7 @@ int stbpe_rows_count_pairs_noalloc(const int32_t *tokens, const uint8_t *valid, 
  *   STBPE_WANT_GRADS : grad_hidden[rows][dim] and grad_weight[vocab][dim] in the inputs' type (NULL: not wanted), times
  *                      grad_loss (one value, or one per row without a reduction; NULL: 1).  Alone, lse2 comes from a
  *                      call with the same inputs.
- * The call reads nothing back and does not synchronise: it can be captured.  workspace: device memory on a 1024-byte
+ * The call runs on the current device, reads nothing back and does not synchronise: it can be captured.  workspace: device memory on a 1024-byte
  * boundary, of the size that stbpe_vocab_loss_workspace gives for the same arguments; nothing in it outlasts the call.
  * err may be NULL. */
 #define STBPE_REAL_BF16 0

@@ -6,16 +6,20 @@
 //   MAKE_G       Z again, of one piece of the vocabulary, and G = dlogits from it in 16 bits
 //   GRADS        dH = E W or G W        (k over the columns: W is read with the other dimension contiguous) and
 //                dW = E^T H' or G^T H   (k over the rows: both are read with the other dimension contiguous),
-//                which wait for the same and fill each other's last round: a step over 2 048 x 1 256 x 512 takes 42 us with
+//                which wait for the same and fill each other's last round: a step over 2 048 x 1 256 x 512 took 42 us with
 //                both in one launch and 51 with one each
 //
 // A group of GROUP CTAs makes a tile of 128 GROUP x 128 GROUP: with GROUP = 2 the two CTAs of a cluster share one
 // 256 x 256 tile (cta_group::2), each holding its half of both operands, so that a byte brought into shared memory serves twice as
 // many products.  A CTA loads 128 x 64 of each operand per step in either case: 64 bytes per SM and clock at the full rate
-// with GROUP = 2, 128 with GROUP = 1, which L2 does not deliver (0.93 to 0.98 PFLOP/s against 1.24 to 1.59 at
-// 8 188 x 32 256 x 2 048).  Persistent: the tiles are dealt out
-// to the clusters in turn, and the sums of one tile are looked at while the next one is being made (two buffers in TMEM).
-// Warp 0 loads, warp 1 of the group's first CTA multiplies, warp 2 owns the TMEM, warps 4 to 11 take the sums.
+// with GROUP = 2, 128 with GROUP = 1, which L2 does not deliver (1.5 to 1.6 PFLOP/s against 0.93 to 0.98 at
+// 8 188 x 32 256 x 2 048).  Persistent: the tiles are dealt out to the clusters in turn, and the sums of one tile are looked at
+// while the next one is being made (two buffers in TMEM).
+// Warp 0 loads, warp 1 of the group's first CTA multiplies, warp 2 owns the TMEM, warps 4 to 11 take the sums, warp 3 has
+// the losses to add up.
+//
+// What bounds them at that size: the tensor pipe, active 92 to 95 % of the cycles, and the board's power, which holds the clock at
+// 1.35 to 1.45 GHz.  At depths of 16 steps, or where the tiles are few, what begins and ends a tile.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -37,7 +41,8 @@ constexpr int PRODUCT_THREADS = 384;
 constexpr int PRODUCT_SMEM = STAGES * STAGE_BYTES + 1024 + 256 + 8 * 2048;
 
 // How the tiles of one or two results are dealt out: whole ones in rounds of all clusters, and those that are left behind a result's full
-// rounds split in depth, up to SPLITS units per tile of SPLIT_STEPS steps at least, so that the last round is shorter, too.  Joining the units of a tile costs about as much as JOIN_STEPS steps.
+// rounds split in depth, up to SPLITS units per tile of SPLIT_STEPS steps at least, so that the last round is shorter, too.  Joining
+// the units of a tile costs about as much as JOIN_STEPS steps.
 constexpr int SPLIT_STEPS = 16, JOIN_STEPS = 14;
 struct Deal {
     unsigned whole[2], left[2], splits[2], units;

@@ -257,6 +257,9 @@ def test_strides_and_alignment(K):
     flat = [x.reshape(B * L, *x.shape[2:]) for x in ((state, ids, logits) if K else (state, tokens))]
     flat = [x[::2] for x in ([flat[0][:, :D], flat[1][:, :K], flat[2][:, :K]] if K else [flat[0][:, :D], flat[1]])]
     check(flat[0], table[:V, :D], *flat[1:])
+    rest = (ids[..., :K], logits[..., :K]) if K else (tokens,)
+    check(state[..., :D].contiguous(), table[:1, :D].expand(V, D), *rest)       # one row for all ids,
+    check(state[..., :D].contiguous(), table[:, :8].as_strided((V, D), (8, 1)), *rest)  # rows that overlap
     one = state[:1, :1, :D].expand(B, L, D)  # one state for all rows
     check(one, table[:V, :D], *((ids[..., :K], logits[..., :K]) if K else (tokens,)))
 
