@@ -170,9 +170,9 @@ __device__ __forceinline__ void copy_row(T *to, const T *from, i64 inside, i64 a
 // Then counted rows of `hidden` go one behind another, zeros up to the end of the last tile, a warp to a row: products then do no
 // work for padding, never multiply what a masked row holds (it may be NaN), and may read rows of any stride or alignment.  The
 // rows of dH that do not count get their zeros here.
-// dlogits are held in the inputs' 16-bit type, so they are brought into that type's range: the largest |g_i T|
-// becomes up to 2^14 (by a power of two, so bf16 loses nothing; fp16 keeps shares down to 2^-28 at full precision and its
-// entries stay below 2^15), and both gradients are scaled back in 32 bits.
+// dlogits are held in the inputs' 16-bit type, so they are brought into that type's range: the largest |g_i T| becomes 16376 (fp16
+// keeps shares down to 2^-28 at full precision and its entries stay below 2^15; just below a power of two, a target's
+// dlogit, -g T (1 - q), loses half as much to its rounding as just above one), and both gradients are scaled back in 32 bits.
 template <class T>
 __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
     next_may_come();
@@ -284,13 +284,10 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
         for (int x = threadIdx.x; x < 2 * SMS * 8; x += 1024) p.split_done[x] = 0;
     if (threadIdx.x == 0) {
         const float factor = p.temperature / (p.reduction == STBPE_REDUCE_MEAN ? (float)(n > 0 ? n : 1) : 1.f);
-        most *= factor;
-        int up = 0;  // the next power of two, both sides kept within what 32 bits hold as normal numbers
-        if (most > 0.f && most < INFINITY) frexpf(most, &up);
-        up = max(-100, min(100, up));
+        const float in = 16376.f / fminf(fmaxf(most * factor, 1e-30f), 1e30f);
         p.meta->counted = (int)n, p.meta->tickets = 0, p.meta->again = 0;
-        p.meta->in_scale = (each ? 1.f : one) * factor * ldexpf(1.f, 14 - up);
-        p.meta->out_scale = ldexpf(1.f, up - 14);
+        p.meta->in_scale = (each ? 1.f : one) * factor * in;
+        p.meta->out_scale = 1.f / in;
     }
 }
 
