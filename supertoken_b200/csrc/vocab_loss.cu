@@ -5,15 +5,18 @@
 //   loss_i = T^2 (lse_i + sum_k p_ik (log p_ik - s z_i,t_ik))
 //   G_ij = g_i T (exp(s z_ij - lse_i) - sum_k p_ik [j = t_ik])       dH = G W        dW = G^T H
 // The N x V logits are never stored.  Two ways to the gradients:
-//   keep    (loss and gradients at once, bf16): E_ij = exp2(z_ij s log2 e - c_i) goes to memory in 16 bits, for at most 1 GiB of
-//           rows at a time, with a reference c_i known before the product, and the sums that make lse_i (lse2_i in
-//           powers of 2) beside it.  Then E - p exp2(lse2_i - c_i) at the entries, from z in 32 bits, and with
-//           a_i = g_i T exp2(c_i - lse2_i), dH = a (E W) and dW = E^T (a H).  Three products; three roundings to 16 bits
-//           reach dW (E, a H, the result) and two dH, 0.0028 and 0.0024 off in the 2-norm where the result's own is 0.0017.
-//           c_i is 0; a row whose largest logit lies further than a factor of 2^96 from that gets it as its reference and its
-//           tile is made again, which logits below 66 in size never need.  fp16 has not the range for it.
-//   anew    (fp16, or gradients after the loss): z is made a second time, and G from it for up to 1 GiB of the vocabulary
-//           at a time.  Four products, or three behind a loss; two roundings.
+//   keep    (loss and gradients at once): E_ij = exp2(z_ij s log2 e - c_i) goes to memory in 16 bits, for at most 1 GiB of rows at
+//           a time, and the sums that make lse_i (lse2_i in powers of 2) beside it.  Three products.
+//           With each part's own maximum (of 64 or 128 columns, less 14) as c, E has the range that fp16 needs, and becomes G
+//           where it lies once lse_i is known, the entries from z in 32 bits: E is read and written once more (0.2 ms for 4 336 rows of
+//           50 257), and G is rounded twice but for the entries, from which most of the gradients come.
+//           With c_i = 0 for a row (bf16, where E is above 48 MB and that pass would cost 3 to 6 % of a step) E stays, but for the entries,
+//           and a_i = g_i T exp2(c_i - lse2_i) goes to the other factors: dH = a (E W), dW = E^T (a H).  One rounding more
+//           reaches dW, 0.0028 off in the 2-norm against 0.0022, where the result's own rounding is 0.0017.  A row whose
+//           largest logit lies further than a factor of 2^96 from c_i gets it as its reference and its tile is made again, which logits
+//           below 66 in size never need.
+//   anew    (gradients after the loss, as fp16 and losses per row need them through autograd): z is made a second time,
+//           and G from it for up to 1 GiB of the vocabulary at a time.  Three products behind the loss's one.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
         for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)((T *)p.packed + c * p.dim_padded + d) = make_uint4(0, 0, 0, 0);
     const i64 step = (i64)p.row_blocks * 1024;
     for (i64 c = n + blockIdx.x * 1024 + threadIdx.x; c < p.rows_padded; c += step) p.row_of[c] = -1;
-    if (p.keep) {
+    if (p.fixed) {
         for (i64 c = blockIdx.x * 1024 + threadIdx.x; c < p.rows_padded; c += step) p.reference[c] = 0.f;
         for (i64 c = blockIdx.x * 1024 + threadIdx.x; c < 2 * p.rows_padded / TILE_ROWS; c += step) p.again[c] = 0;
     }
@@ -400,10 +403,10 @@ __global__ void __launch_bounds__(256) few_kernel(Plan p) {
 }
 
 // ---------------------------------------------------------------------------------------------- after the products
-// Eight rows of a chunk to a block: joins what the parts of the columns left, in a fixed order (eight threads read a sector, 32 parts
+// Eight rows of a chunk (and a slice of their columns, where few rows are turned into G) to a block: joins what the parts of the columns left, in a fixed order (eight threads read a sector, 32 parts
 // at a time), to lse and the loss of a row; then a warp has a row.  Where E is kept, the row's E gets its entries and the packed row its factor.
 template <class T>
-__global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows) {
+__global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int slices) {
     next_may_come();
     before_is_done();
     __shared__ float tops[8][8], sums[8][8], lse2s[8], refs[8];
@@ -411,13 +414,14 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const i64 counted = p.meta->counted;
     const i64 n = counted - r0 < 0 ? 0 : counted - r0 < rows ? counted - r0 : rows;
-    const i64 until = p.keep ? (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS : n;
-    for (i64 m0 = (i64)blockIdx.x * 8; m0 < until; m0 += (i64)gridDim.x * 8) {
+    const i64 until = p.fixed ? (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS : n;
+    const int slice = blockIdx.x % slices;
+    for (i64 m0 = (i64)(blockIdx.x / slices) * 8; m0 < until; m0 += (i64)(gridDim.x / slices) * 8) {
         float top = LOWEST, sum = 0.f;
         auto add = [&](float m, float x) {
             const float both = fmaxf(top, m);
-            // (all parts of a row of E have the row's reference)
-            sum = p.keep ? sum + x : sum * exp2f(top - both) + x * exp2f(m - both);
+            // (with a fixed reference all parts of a row have it)
+            sum = p.fixed ? sum + x : sum * exp2f(top - both) + x * exp2f(m - both);
             top = both;
         };
         // the row of this warp; the sum of its target's logit needs nothing of the parts
@@ -441,7 +445,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows) {
             top = tops[0][lane], sum = sums[0][lane];
             for (int w = 1; w < 8; ++w) add(tops[w][lane], sums[w][lane]);
             float ref = top;
-            if (p.keep && m0 + lane < n) {
+            if (p.fixed && m0 + lane < n) {
                 ref = p.reference[r0 + m0 + lane];
                 if (fabsf(top - ref) > 96.f && fabsf(top) < INFINITY) {
                     p.reference[r0 + m0 + lane] = top;
@@ -453,8 +457,8 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows) {
         __syncthreads();
         T *scaled = (T *)p.scaled + m * p.dim_padded;
         if (m < n) {
-            finish_row<T>(p, m, slot, row, lse2s[warp], refs[warp], refined, sum_z, lane);
-        } else if (p.keep && m < until) {  // zeros behind the last row
+            finish_row<T>(p, m, slot, row, lse2s[warp], refs[warp], refined, sum_z, lane, slice, slices);
+        } else if (p.fixed && m < until) {  // zeros behind the last row
             for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)(scaled + d) = make_uint4(0, 0, 0, 0);
         }
         __syncthreads();
@@ -589,10 +593,11 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     p.loss = a->loss, p.lse2 = a->lse2, p.grad_hidden = a->grad_hidden, p.grad_weight = a->grad_weight;
     const bool aligned = (uintptr_t)a->weight % 16 == 0 && a->weight_stride % 8 == 0 && a->weight_stride >= a->dim && a->dim % 8 == 0;
     p.weight_rows_stride = aligned ? a->weight_stride : p.dim_padded;
+    if (!aligned && p.row_blocks > SMS / 4) p.row_blocks = SMS / 4;  // (the others align the weight: a block of either kind has an SM)
     // at most KEPT bytes of E or G at a time (for large vocabularies 2048 rows of E, for many rows 2048 columns of G)
-    constexpr i64 KEPT = 1ll << 30;
+    constexpr i64 KEPT = 1ll << 30, FIXED_BYTES = 48ll << 20;
     const i64 all = up_to(a->vocab, PIECE);
-    p.keep = p.want_loss && p.want_grads && a->type == STBPE_REAL_BF16;
+    p.keep = p.want_loss && p.want_grads;
     p.chunk_rows = p.rows_padded, p.g_stride = all;
     if (p.keep) {
         const i64 most = KEPT / (2 * all) / TILE_ROWS * TILE_ROWS;
@@ -601,6 +606,7 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
         const i64 most = KEPT / (2 * p.rows_padded) / PIECE * PIECE;
         p.g_stride = all <= most ? all : most > 2048 ? most : all < 2048 ? all : 2048;
     }
+    p.fixed = p.keep && a->type == STBPE_REAL_BF16 && p.rows * a->vocab * 2 > FIXED_BYTES;
     p.group = group_of(p.keep && p.chunk_rows < p.rows ? p.chunk_rows : p.rows, a->vocab, 0, 0, a->dim, 0, false, false);
     p.parts = (int)((a->vocab + 64 * p.group - 1) / (64 * p.group));
     p.part_stride = p.chunk_rows;
@@ -637,13 +643,14 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
         p.g = take(p.chunk_rows * p.g_stride * 2);
         p.split_sums = (float *)take((i64)2 * SMS * 8 * 64 * 2 * 32 * 4);
         p.split_done = (unsigned int *)take(2 * SMS * 8 * 4);
-        if (p.keep) {
+        if (p.fixed) {
             p.reference = (float *)take(p.rows_padded * 4);
             p.out_row = (float *)take(p.rows_padded * 4);
             p.again = (int *)take(2 * p.rows_padded / TILE_ROWS * 4);
             p.scaled = take(p.chunk_rows * p.dim_padded * 2);
-            if (p.chunk_rows < p.rows_padded) p.weight_acc = (float *)take(p.vocab * p.acc_stride * 4);
-        } else if (p.g_stride < all) {
+        }
+        if (p.chunk_rows < p.rows_padded) p.weight_acc = (float *)take(p.vocab * p.acc_stride * 4);
+        if (p.g_stride < all) {
             p.acc = (float *)take(p.rows_padded * p.acc_stride * 4);
         }
     }
@@ -727,14 +734,14 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
     if (p.few) {
         auto *few = p.rows == 1 ? few_kernel<T, 1> : p.rows == 2 ? few_kernel<T, 2> : p.rows <= 4 ? few_kernel<T, 4> : few_kernel<T, 8>;
         VCK(start(few, p.parts, 256, 0, 1, s, p));
-        VCK(start(join_kernel<T>, 1, 256, 0, 1, s, p, 0, p.rows_padded));
+        VCK(start(join_kernel<T>, 1, 256, 0, 1, s, p, 0, p.rows_padded, 1));
         return STBPE_OK;
     }
     if (p.k) {
         auto *teacher = p.k <= 32 ? teacher_kernel<1> : p.k <= 64 ? teacher_kernel<2> : p.k <= 128 ? teacher_kernel<4> : teacher_kernel<8>;
         VCK(start(teacher, blocks(p.rows, 4), 128, 0, 1, s, p));
     }
-    VCK(start(rows_kernel<T>, p.row_blocks + (p.weight_rows != p.weight ? SMS : 0), 1024, 0, 1, s, p));
+    VCK(start(rows_kernel<T>, p.weight_rows != p.weight ? SMS : p.row_blocks, 1024, 0, 1, s, p));
     Maps logits, grads;
     VTRY(map(&logits.map[0], p.packed, p.rows_padded, p.dim, p.dim_padded, 128));
     VTRY(map(&logits.map[1], p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 128));
@@ -743,25 +750,30 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
         VTRY(map(&grads.map[0], p.g, p.chunk_rows, p.g_stride, p.g_stride, 128));
         VTRY(map(&grads.map[1], p.weight_rows, p.vocab, p.dim, p.weight_rows_stride, 64));
         VTRY(map(&grads.map[2], p.g, p.chunk_rows, p.g_stride, p.g_stride, 64));
-        VTRY(map(&grads.map[3], p.keep ? p.scaled : p.packed, p.keep ? p.chunk_rows : p.rows_padded, p.dim, p.dim_padded, 64));
+        VTRY(map(&grads.map[3], p.fixed ? p.scaled : p.packed, p.fixed ? p.chunk_rows : p.rows_padded, p.dim, p.dim_padded, 64));
     }
-    const unsigned joins = blocks(p.chunk_rows, 8);
+    const unsigned joins = blocks(p.chunk_rows < p.rows ? p.chunk_rows : p.rows, 8);
+    const int slices = p.keep && !p.fixed && joins <= SMS / 2 ? 8 : 1;  // (two slices of 1 665 rows cost 8 us, eight of 256 save 4)
     if (p.keep) {
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-            for (i64 r0 = 0; r0 < p.rows_padded; r0 += p.chunk_rows) {
-                Job job{0, p.vocab, r0, p.chunk_rows, false, false};
-                VTRY((product<T, MAKE_E>(p, job, logits, s, err, err_len)));
-                VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, r0, p.chunk_rows));
-                job.again = true;
-                VTRY((product<T, MAKE_E>(p, job, logits, s, err, err_len)));
-                job.again = false, job.add_up = p.reduction != STBPE_REDUCE_NONE && r0 + p.chunk_rows >= p.rows_padded;
-                VTRY((product<T, GRADS>(p, job, grads, s, err, err_len)));
+        for (i64 r0 = 0; r0 < p.rows_padded; r0 += p.chunk_rows) {
+            Job job{0, p.vocab, r0, p.chunk_rows, false, false};
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                if (p.fixed) VTRY((product<T, MAKE_E>(p, job, logits, s, err, err_len)));
             }
+            if (!p.fixed) VTRY((product<T, MAKE_R>(p, job, logits, s, err, err_len)));
+            VCK(start(join_kernel<T>, joins * slices, 256, 0, 1, s, p, r0, p.chunk_rows, slices));
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                job.again = true;
+                if (p.fixed) VTRY((product<T, MAKE_E>(p, job, logits, s, err, err_len)));
+                job.again = false;
+            }
+            job.add_up = p.reduction != STBPE_REDUCE_NONE && r0 + p.chunk_rows >= p.rows_padded;
+            VTRY((product<T, GRADS>(p, job, grads, s, err, err_len)));
         }
     } else {
         if (p.want_loss) {
             VTRY((product<T, STATS>(p, Job{0, p.vocab, 0, p.rows_padded, false, false}, logits, s, err, err_len)));
-            VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, 0, p.rows_padded));
+            VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, 0, p.rows_padded, 1));
         }
         if (p.want_grads) {
             for (i64 v0 = 0; v0 < p.vocab; v0 += p.g_stride) {

@@ -29,7 +29,7 @@ struct Meta {
     unsigned int tickets; // blocks of the join that are through with their rows
     float in_scale;       // what coef is multiplied by in the end
     float out_scale;      // what both gradients are multiplied by in the end
-    int again;            // keep: a reference was too far from its row's maximum
+    int again;            // fixed: a reference was too far from its row's maximum
 };
 
 struct Plan {
@@ -61,16 +61,16 @@ struct Plan {
     float *part_max, *part_sum, *row_loss;  // [part][packed row of the chunk]; per row
     i64 part_stride;
     float *coef;             // what a packed row of dlogits is multiplied by, and in_scale
-    // G (16 bits) of one piece of the vocabulary and all packed rows; or E = exp2(logits - reference) of the whole
-    // vocabulary and a chunk of the packed rows (keep)
-    bool keep;
+    // G (16 bits) of one piece of the vocabulary and all packed rows; or (keep) E = exp2(logits - reference) of the whole
+    // vocabulary and a chunk of the packed rows, the reference known before (fixed), or each part's own and E to become G
+    bool keep, fixed;
     void *g;
     i64 g_stride, chunk_rows;
-    float *reference;        // keep: per packed row
-    int *again;              // keep: [packed row / TILE_ROWS] a reference was too far from the row's maximum; then, per TILE_ROWS rows,
+    float *reference;        // fixed: per packed row
+    int *again;              // fixed: [packed row / TILE_ROWS] a reference was too far from the row's maximum; then, per TILE_ROWS rows,
                              // parts that are made again
-    float *out_row;          // keep: what a packed row of dH is multiplied by
-    void *scaled;            // keep: packed rows of the chunk, times coef exp2(reference - lse2)
+    float *out_row;          // fixed: what a packed row of dH is multiplied by
+    void *scaled;            // fixed: packed rows of the chunk, times coef exp2(reference - lse2)
     float *acc;              // several pieces: dH of packed rows in 32 bits, [packed row][acc_stride]
     float *weight_acc;       // several chunks: dW in 32 bits, [vocab][acc_stride]
     i64 acc_stride;
@@ -104,40 +104,65 @@ __device__ __forceinline__ float target_logit(const Plan &p, i64 slot, int row, 
     return z;
 }
 
-// What follows from a row's lse2: its loss, and where E is kept the entries in E (from their logits in 32 bits, once rounded), the factor of its
-// dH and the packed row times it for dW.  m: its place in the chunk.
+// What follows from a row's lse2: its loss.  Where E has a fixed reference, the entries in E (from their logits in 32 bits, once
+// rounded), the factor of the row's dH and the packed row times it for dW; where each part has its own, G in the place of E.
+// m: the row's place in the chunk; slice: which of the row's slices of columns this warp turns into G.
 template <class T>
-__device__ __forceinline__ void finish_row(const Plan &p, i64 m, i64 slot, int row, float lse2, float ref, bool refined, float target, int lane) {
+__device__ __forceinline__ void finish_row(const Plan &p, i64 m, i64 slot, int row, float lse2, float ref, bool refined, float target, int lane,
+                                           int slice = 0, int slices = 1) {
     const int entries_of_row = p.k ? p.k : 1;
     const float scale = p.inv_temperature * 1.4426950408889634f;
     const int2 *e = p.entries + (i64)row * entries_of_row;
-    float *z = p.entry_z + slot * entries_of_row;
+    const float *z = p.entry_z + slot * entries_of_row;
     if (refined) {
         const float before = z[0], share = exp2f(fmaf(before, scale, -lse2));
         lse2 += log1pf(share * expm1f((target - before) * p.inv_temperature)) * 1.4426950408889634f;
-        __syncwarp();
-        if (lane == 0) z[0] = target;
+    }
+    float unit = exp2f(lse2 - ref), minus = ref, times = 1.f;  // a share, the logits and a factor in the units of E
+    const i64 from_j = slice == 0 ? 0 : p.vocab * slice / slices / 8 * 8, to_j = slice + 1 == slices ? p.vocab : p.vocab * (slice + 1) / slices / 8 * 8;
+    if (p.keep && !p.fixed) {
+        unit = 1.f, minus = lse2, times = p.coef[slot] * p.meta->in_scale;
+        T *g = (T *)p.g + m * p.g_stride;
+        const int shift = 5 + p.group;  // 64 columns to a part, or 128
+        constexpr int MANY = 4;  // loads of a lane on their way at a time
+        for (i64 j0 = from_j + lane * 8; j0 < to_j; j0 += MANY * 256) {
+            uint4 x[MANY];
+            float f[MANY];
+#pragma unroll
+            for (int y = 0; y < MANY; ++y) {
+                const i64 j = j0 + y * 256 < to_j ? j0 + y * 256 : j0;
+                x[y] = __ldcs((const uint4 *)(g + j)), f[y] = p.part_max[(j >> shift) * p.part_stride + m];
+            }
+#pragma unroll
+            for (int y = 0; y < MANY; ++y) {
+                const float by = times * exp2f(f[y] - lse2);
+                T *v = (T *)&x[y];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = T((float)v[i] * by);
+                if (j0 + y * 256 < to_j) *(uint4 *)(g + j0 + y * 256) = x[y];
+            }
+        }
         __syncwarp();
     }
-    const float less = exp2f(lse2 - ref);  // a share in the units of E
     float pz = 0.f;
     for (int k = lane; k < entries_of_row; k += 32) {
         const int2 it = e[k];
         if (it.x == INT_MAX) break;
-        pz += __int_as_float(it.y) * z[k];
-        if (p.keep && (k == 0 || e[k - 1].x != it.x)) {  // (the same id again: its first entry takes them all)
+        const float its = refined ? target : z[k];
+        pz += __int_as_float(it.y) * its;
+        if (p.keep && it.x >= from_j && it.x < to_j && (k == 0 || e[k - 1].x != it.x)) {  // (the same id again: its first entry takes them all)
             float share = __int_as_float(it.y);
             for (int l = k + 1; l < entries_of_row && e[l].x == it.x; ++l) share += __int_as_float(e[l].y);
-            ((T *)p.g)[m * p.g_stride + it.x] = T(exp2f(fmaf(z[k], scale, -ref)) - share * less);
+            ((T *)p.g)[m * p.g_stride + it.x] = T(times * (exp2f(fmaf(its, scale, -minus)) - share * unit));
         }
     }
     for (int d = 16; d; d >>= 1) pz += __shfl_xor_sync(~0u, pz, d);
-    if (lane == 0) {
+    if (lane == 0 && slice == 0) {
         const float tau = p.temperature;
         p.lse2[row] = lse2;
         p.row_loss[row] = tau * tau * (lse2 * 0.69314718055994531f + p.plogp[row] - pz * p.inv_temperature);
     }
-    if (p.keep) {
+    if (p.fixed) {
         const float a = p.coef[slot] * p.meta->in_scale * exp2f(ref - lse2);
         if (lane == 0) p.out_row[slot] = a * p.meta->out_scale;
         const T *from = (const T *)p.packed + slot * p.dim_padded;

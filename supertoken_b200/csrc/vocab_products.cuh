@@ -3,6 +3,7 @@
 //
 //   STATS        Z = H W^T; per row and part of the columns the maximum and the sum of exp, the logits at the entries
 //   MAKE_E       the same, and E = exp2(Z - reference) in 16 bits
+//   MAKE_R       the same with each part's maximum, less 14, as the reference: E is below 2^14
 //   MAKE_G       Z again, of one piece of the vocabulary, and G = dlogits from it in 16 bits
 //   GRADS        dH = E W or G W        (k over the columns: W is read with the other dimension contiguous) and
 //                dW = E^T H' or G^T H   (k over the rows: both are read with the other dimension contiguous),
@@ -31,7 +32,7 @@
 
 namespace vloss {
 
-enum { STATS, MAKE_E, MAKE_G, GRADS };
+enum { STATS, MAKE_E, MAKE_R, MAKE_G, GRADS };
 
 constexpr int STAGES = 6;
 constexpr int OPERAND_BYTES = 128 * 64 * 2;  // what a CTA loads of one operand per step of 64 terms
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             for (unsigned u = cluster; u < units && alive; u += clusters) {
                 const Unit t = unit_at(u);
                 if (skipped(t)) continue;
-                const int am = (int)(t.m0 + rank * 128), bn = (int)(t.n0 + rank * 128);
+                const int am = (int)(t.m0 + rank * 128), bn = (int)(t.n0 + rank * 128), h0 = p.fixed ? 0 : (int)job.r0;
                 // (a loop of its own for each result: what differs is known when it is compiled)
                 auto load = [&](auto which) {
                     constexpr int RESULT = decltype(which)::value;
@@ -400,8 +401,8 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                         } else {
                             tma_load<GROUP>(a, &maps.map[2], am, k * 64, bar);
                             tma_load<GROUP>(a + 8192, &maps.map[2], am + 64, k * 64, bar);
-                            tma_load<GROUP>(b, &maps.map[3], bn, k * 64, bar);
-                            tma_load<GROUP>(b + 8192, &maps.map[3], bn + 64, k * 64, bar);
+                            tma_load<GROUP>(b, &maps.map[3], bn, h0 + k * 64, bar);
+                            tma_load<GROUP>(b + 8192, &maps.map[3], bn + 64, h0 + k * 64, bar);
                         }
                         ++issued;
                         if (++s == STAGES) s = 0, phase ^= 1;
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                 coef = p.meta->out_scale;
                 if (t.result == 0 && m < n) {
                     row = p.row_of[slot];
-                    if (p.keep) coef = p.out_row[slot];
+                    if (p.fixed) coef = p.out_row[slot];
                 }
             }
             // 32 sums of dH or dW, at column c of this thread's columns
@@ -541,6 +542,22 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             const uint32_t from = tmem + buffer * TILE + half * COLUMNS + ((uint32_t)(quarter * 32) << 16);
             // [unit of a split tile][CTA][warp][column][lane]
             float *sums = p.split_sums + (((i64)(t.sums + (t.split < 0 ? 0 : t.split)) * GROUP + rank) * 8 + warp - 4) * (COLUMNS * 32) + lane;
+            if (KIND == MAKE_R) {  // the maximum first, the sums are read twice
+#pragma unroll 1
+                for (int c = 0; c < COLUMNS && alive; c += 32) {
+                    uint32_t bits[32];
+                    __syncwarp();
+                    tmem_load(from + c, bits);
+                    const i64 inside = p.vocab - (job.v0 + c0 + c);
+                    float most = -INFINITY;
+#pragma unroll
+                    for (int x = 0; x < 32; ++x)
+                        if (x < inside) most = fmaxf(most, __uint_as_float(bits[x]));
+                    top = fmaxf(top, most * scale);
+                }
+                top -= 14.f;
+                if (row >= 0) shift = top;
+            }
 #pragma unroll 1
             for (int c = 0; c < COLUMNS; c += 32) {
                 float v[32];
@@ -569,7 +586,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     continue;
                 }
                 const i64 j = job.v0 + c0 + c;  // first column, as a token id
-                if (KIND == STATS || KIND == MAKE_E) {
+                if (KIND != MAKE_G) {
                     while (walk.next.x < j + 32) {
                         const int x0 = walk.next.x - (int)j;
                         float z = 0.f;
@@ -584,20 +601,18 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                         for (int x = 0; x < 32; ++x)
                             if (j + x >= p.vocab) v[x] = -INFINITY;
                     }
-                    float most = v[0];
+                    if (KIND != MAKE_R) {
+                        float most = v[0];
 #pragma unroll
-                    for (int x = 1; x < 32; ++x) most = fmaxf(most, v[x]);
-                    if (KIND == STATS) {
-                        shift = fmaxf(top, most * scale);
-                        sum *= exp2_fast(top - shift);
-                        top = shift;
-                    } else {
-                        top = fmaxf(top, most * scale);
+                        for (int x = 1; x < 32; ++x) most = fmaxf(most, v[x]);
+                        const float now = fmaxf(top, most * scale);
+                        if (KIND == STATS) sum *= exp2_fast(top - now), shift = now;
+                        top = now;
                     }
                 }
 #pragma unroll
                 for (int x = 0; x < 32; ++x) v[x] = exp2_fast(fmaf(v[x], scale, -shift));
-                if (KIND == STATS || KIND == MAKE_E) {
+                if (KIND != MAKE_G) {
 #pragma unroll
                     for (int x = 0; x < 32; ++x) sum += v[x];
                 }
@@ -617,11 +632,11 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                             if (j + x >= p.vocab) v[x] = 0.f;
                     }
                 }
-                if (KIND == MAKE_E || KIND == MAKE_G) {
+                if (KIND != STATS) {
                     if (c0 + c < p.g_stride) store_rows((T *)p.g + m * p.g_stride + c0 + c, v, 32, 8, stage, lane);
                 }
             }
-            if ((KIND == STATS || KIND == MAKE_E) && row >= 0 && job.v0 + c0 < p.vocab) {
+            if (LOGITS && KIND != MAKE_G && row >= 0 && job.v0 + c0 < p.vocab) {
                 const i64 to = (job.v0 + c0) / COLUMNS * p.part_stride + m;
                 p.part_max[to] = top, p.part_sum[to] = sum;
             }

@@ -479,6 +479,7 @@ def test_more_rows_and_ids_than_are_held_at_a_time(K, dtype):
     """2 300 rows over 300 001 ids are two chunks of rows (or two pieces of the vocabulary); fewer rows than a chunk count, too."""
     args = make(1, 2300, 64, 300_001, K, dtype=dtype)
     check(*args, grad=64.0)
+    check(*args, grad=64.0, reduction="none")
     valid = torch.arange(2300, device="cuda")[None] % 3 == 0
     check(*args, valid=valid, grad=64.0)
 
@@ -492,6 +493,13 @@ def test_rows_of_any_height(K):
     hidden[0, 17, 0], hidden[0, 18, 0], hidden[1, 150:, 0], hidden[2, :2, 0] = 90.0, -90.0, 250.0, -3000.0
     check(hidden, weight, *rest)
     check(hidden, weight, *rest, reduction="none")
+    # as much of it as exponentials about a fixed reference are kept of
+    hidden, weight, *rest = make(3, 900, 64, 10_000, K)
+    weight[:, 0] = 1.0
+    hidden[..., 0] = 0.0
+    hidden[0, 17, 0], hidden[0, 18, 0], hidden[1, 850:, 0], hidden[2, :2, 0] = 90.0, -90.0, 250.0, -3000.0
+    check(hidden, weight, *rest)
+    check(hidden, weight, *rest, reduction="sum", grad=0.5)
 
 
 def test_splits_of_the_depth():
