@@ -37,31 +37,32 @@ enum { STATS, MAKE_E, MAKE_R, MAKE_G, GRADS };
 constexpr int STAGES = 6;
 constexpr int OPERAND_BYTES = 128 * 64 * 2;  // what a CTA loads of one operand per step of 64 terms
 constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
-constexpr int SPLITS = 4;  // (8: nothing gained where 129 steps are split, and more registers)
+constexpr int SPLITS = 8;
 constexpr int PRODUCT_THREADS = 384;
 constexpr int PRODUCT_SMEM = STAGES * STAGE_BYTES + 1024 + 256 + 8 * 2048;
 
 // How the tiles of one or two results are dealt out: whole ones in rounds of all clusters, and those that are left behind a result's full
 // rounds split in depth, up to SPLITS units per tile of SPLIT_STEPS steps at least, so that the last round is shorter, too.  Joining
-// the units of a tile costs about as much as JOIN_STEPS steps.
-constexpr int SPLIT_STEPS = 16, JOIN_STEPS = 14;
+// a units of a tile costs about as much as JOIN_STEPS + 2 a steps.
+constexpr int SPLIT_STEPS = 16, JOIN_STEPS = 8;
 struct Deal {
     unsigned whole[2], left[2], splits[2], units;
     unsigned steps;  // what the busiest cluster goes through, about
 };
 __host__ __device__ inline Deal deal(const unsigned (&tiles)[2], const unsigned (&steps)[2], const bool (&may_split)[2], unsigned clusters) {
     Deal d;
-    unsigned rounds = 0;
+    unsigned rounds = 0, most[2];
     for (int r = 0; r < 2; ++r) {
         d.left[r] = tiles[r] % clusters, d.whole[r] = tiles[r] - d.left[r], d.splits[r] = 1;
         rounds += d.whole[r] / clusters * steps[r];
+        most[r] = may_split[r] && d.left[r] ? SPLITS : 1;
+        while (most[r] > 1 && (steps[r] < most[r] * SPLIT_STEPS || d.left[r] * most[r] > clusters)) most[r] >>= 1;
     }
     unsigned best = UINT_MAX;
-    for (unsigned a = 1; a <= (may_split[0] && d.left[0] ? SPLITS : 1); ++a)
-        for (unsigned b = 1; b <= (may_split[1] && d.left[1] ? SPLITS : 1); ++b) {
-            if ((a > 1 && (steps[0] < a * SPLIT_STEPS || d.left[0] * a > clusters)) || (b > 1 && (steps[1] < b * SPLIT_STEPS || d.left[1] * b > clusters)))
-                continue;
-            const unsigned x = d.left[0] ? steps[0] / a + (a > 1 ? JOIN_STEPS : 0) : 0, y = d.left[1] ? steps[1] / b + (b > 1 ? JOIN_STEPS : 0) : 0;
+    for (unsigned a = 1; a <= most[0]; a *= 2)
+        for (unsigned b = 1; b <= most[1]; b *= 2) {
+            const unsigned x = d.left[0] ? steps[0] / a + (a > 1 ? JOIN_STEPS + 2 * a : 0) : 0;
+            const unsigned y = d.left[1] ? steps[1] / b + (b > 1 ? JOIN_STEPS + 2 * b : 0) : 0;
             const unsigned cost = d.left[0] * a + d.left[1] * b <= clusters ? (x > y ? x : y) : x + y;
             if (cost < best) best = cost, d.splits[0] = a, d.splits[1] = b;
         }
@@ -540,8 +541,8 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             if (alive) alive = __all_sync(~0u, barrier_wait(sums_full + 8 * buffer, sums_phase));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t from = tmem + buffer * TILE + half * COLUMNS + ((uint32_t)(quarter * 32) << 16);
-            // [unit of a split tile][CTA][warp][column][lane]
-            float *sums = p.split_sums + (((i64)(t.sums + (t.split < 0 ? 0 : t.split)) * GROUP + rank) * 8 + warp - 4) * (COLUMNS * 32) + lane;
+            // [unit of a split tile][CTA][warp][column / 4][lane], four columns each
+            float4 *sums = (float4 *)p.split_sums + (((i64)(t.sums + (t.split < 0 ? 0 : t.split)) * GROUP + rank) * 8 + warp - 4) * (COLUMNS * 8) + lane;
             if (KIND == MAKE_R) {  // the maximum first, the sums are read twice
 #pragma unroll 1
                 for (int c = 0; c < COLUMNS && alive; c += 32) {
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                         emit(c, v);
                     } else {
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) __stcg(sums + (c + x) * 32, v[x]);
+                        for (int x = 0; x < 32; x += 4) __stcg(sums + (c + x) * 8, make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]));
                     }
                     continue;
                 }
@@ -664,24 +665,26 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                 if (before == t.splits - 1) {
                     __threadfence();
                     if (lane == 0) *done = 0;
-                    const i64 next = (i64)GROUP * 8 * COLUMNS * 32;
-                    sums -= t.split * next;
+                    constexpr int next = GROUP * 8 * COLUMNS * 8;
+                    sums -= (i64)t.split * next;
 #pragma unroll 1
                     for (int c = 0; c < COLUMNS; c += 32) {
                         float v[32];
 #pragma unroll
-                        for (int x0 = 0; x0 < 32; x0 += 8) {  // eight columns of all splits on their way at a time
-                            float y[SPLITS][8];
+                        for (int x = 0; x < 32; ++x) v[x] = 0.f;
+#pragma unroll 1
+                        for (int s = 0; s < t.splits; s += 2) {  // two units on their way at a time
+                            float4 y[2][8];
 #pragma unroll
-                            for (int s = 0; s < SPLITS; ++s)
+                            for (int z = 0; z < 2; ++z)
 #pragma unroll
-                                for (int x = 0; x < 8; ++x) y[s][x] = s < t.splits ? __ldcg(sums + s * next + (c + x0 + x) * 32) : 0.f;
+                                for (int x = 0; x < 8; ++x)
+                                    y[z][x] = s + z < t.splits ? __ldcg(sums + (s + z) * next + (c + 4 * x) * 8) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                            for (int x = 0; x < 8; ++x) {
-                                v[x0 + x] = y[0][x];
+                            for (int z = 0; z < 2; ++z)
 #pragma unroll
-                                for (int s = 1; s < SPLITS; ++s) v[x0 + x] += y[s][x];
-                            }
+                                for (int x = 0; x < 8; ++x)
+                                    v[4 * x] += y[z][x].x, v[4 * x + 1] += y[z][x].y, v[4 * x + 2] += y[z][x].z, v[4 * x + 3] += y[z][x].w;
                         }
                         emit(c, v);
                     }
