@@ -710,8 +710,8 @@ int product(const Plan &p, const Job &job, const Maps &maps, cudaStream_t s, cha
         return p.group == 1 ? launch<T, KIND, 1>(p, job, maps, tiles, s, err, err_len) : launch<T, KIND, 2>(p, job, maps, tiles, s, err, err_len);
     }
     const i64 tall = p.grad_hidden ? rows : 0, wide = p.grad_weight ? job.width : 0;
-    auto tiles = [&](i64 x) { return ((x + 255) / 256) * ((p.dim + 255) / 256); };
-    if (tall && wide && tiles(tall) + tiles(wide) > 4 * SMS / 2) {  // a launch each
+    auto work = [&](i64 x, i64 deep) { return ((x + 255) / 256) * ((p.dim + 255) / 256) * ((deep + 63) / 64); };
+    if (tall && wide && work(tall, job.width) + work(wide, rows) > 1000 * SMS / 2) {  // above 1000 steps of a cluster, 0.4 ms, a launch each
         Plan one = p;
         one.grad_weight = nullptr;
         VTRY((product<T, KIND>(one, job, maps, s, err, err_len)));
