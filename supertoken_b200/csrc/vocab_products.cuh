@@ -253,22 +253,24 @@ __device__ __forceinline__ void store_rows(T *to, const float (&v)[32], i64 insi
     }
 }
 
-// The entries of one row in ascending order: what falls into each 32 columns.
+// The entries of one row in ascending order: what falls into each 32 columns.  The one behind the next is on its way already.
 struct Walk {
     const int2 *entries;
     int at, all;
-    int2 next;
+    int2 next, then;
 
+    __device__ __forceinline__ int2 entry(int which) const { return which < all ? entries[which] : make_int2(INT_MAX, 0); }
     __device__ __forceinline__ void start(const Plan &p, i64 row, i64 column) {
         all = p.k ? p.k : 1;
         entries = p.entries + row * all;
         at = p.k ? p.first[row * p.pieces + column / PIECE] : 0;
-        next = at < all ? entries[at] : make_int2(INT_MAX, 0);
+        next = entry(at), then = entry(at + 1);
         while (next.x < column) advance();
     }
     __device__ __forceinline__ void advance() {
         ++at;
-        next = at < all ? entries[at] : make_int2(INT_MAX, 0);
+        next = then;
+        then = entry(at + 1);
     }
 };
 
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             if (LOGITS) {
                 row = slot < p.rows_padded ? p.row_of[slot] : -1;
                 if (row >= 0 && job.v0 + c0 < p.vocab) walk.start(p, row, job.v0 + c0);
-                else walk.next.x = INT_MAX, walk.at = walk.all = 0;
+                else walk.next.x = walk.then.x = INT_MAX, walk.at = walk.all = 0;
                 if (KIND == MAKE_E && row >= 0) shift = p.reference[slot];
                 if (KIND == MAKE_G && row >= 0) shift = p.lse2[row], coef = p.coef[slot] * p.meta->in_scale;
             }
@@ -550,11 +552,16 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     __syncwarp();
                     tmem_load(from + c, bits);
                     const i64 inside = p.vocab - (job.v0 + c0 + c);
-                    float most = -INFINITY;
+                    float highest[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    if (inside >= 32) {
 #pragma unroll
-                    for (int x = 0; x < 32; ++x)
-                        if (x < inside) most = fmaxf(most, __uint_as_float(bits[x]));
-                    top = fmaxf(top, most * scale);
+                        for (int x = 0; x < 32; ++x) highest[x & 3] = fmaxf(highest[x & 3], __uint_as_float(bits[x]));
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x)
+                            if (x < inside) highest[x & 3] = fmaxf(highest[x & 3], __uint_as_float(bits[x]));
+                    }
+                    top = fmaxf(top, fmaxf(fmaxf(highest[0], highest[1]), fmaxf(highest[2], highest[3])) * scale);
                 }
                 top -= 14.f;
                 if (row >= 0) shift = top;
@@ -603,9 +610,10 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                             if (j + x >= p.vocab) v[x] = -INFINITY;
                     }
                     if (KIND != MAKE_R) {
-                        float most = v[0];
+                        float highest[4] = {v[0], v[1], v[2], v[3]};  // (four chains of operations side by side)
 #pragma unroll
-                        for (int x = 1; x < 32; ++x) most = fmaxf(most, v[x]);
+                        for (int x = 4; x < 32; ++x) highest[x & 3] = fmaxf(highest[x & 3], v[x]);
+                        const float most = fmaxf(fmaxf(highest[0], highest[1]), fmaxf(highest[2], highest[3]));
                         const float now = fmaxf(top, most * scale);
                         if (KIND == STATS) sum *= exp2_fast(top - now), shift = now;
                         top = now;
@@ -614,8 +622,10 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
 #pragma unroll
                 for (int x = 0; x < 32; ++x) v[x] = exp2_fast(fmaf(v[x], scale, -shift));
                 if (KIND != MAKE_G) {
+                    float part[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) sum += v[x];
+                    for (int x = 4; x < 32; ++x) part[x & 3] += v[x];
+                    sum += (part[0] + part[1]) + (part[2] + part[3]);
                 }
                 if (KIND == MAKE_G) {
                     while (walk.next.x < j + 32) {
