@@ -20,7 +20,8 @@
 // the losses to add up.
 //
 // What bounds them at that size: the tensor pipe, active 92 to 95 % of the cycles, and the board's power, which holds the clock at
-// 1.35 to 1.45 GHz.  At depths of 16 steps, or where the tiles are few, what begins and ends a tile.
+// 1.35 to 1.45 GHz.  At depths of 12 steps or fewer the instructions and latencies of the exponentials, two warps to a scheduler (4 500 x
+// 32 494 x 128 scored in 107 us, of which the exponentials' pipe is busy 41); where the tiles are few, what begins and ends one.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -176,10 +177,64 @@ __device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[32]) {
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[64]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(at)
+        : "memory");
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// two numbers by one instruction
+__device__ __forceinline__ u64 two(float a, float b) {
+    u64 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void fma_two(float &a, float &b, u64 times, u64 plus) {
+    u64 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(two(a, b)), "l"(times), "l"(plus));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ u64 add_two(u64 a, u64 b) {
+    u64 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// (NaN is left out, as by fmaxf)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// the largest of N, in four chains of operations side by side
+template <int N>
+__device__ __forceinline__ float largest(const float (&v)[N]) {
+    float m[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int x = 4; x < N; x += 8)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) m[y] = x + 4 + y < N ? max3(m[y], v[x + y], v[x + 4 + y]) : fmaxf(m[y], v[x + y]);
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
 __device__ __forceinline__ void cluster_sync() {
@@ -211,14 +266,14 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
 // 32 columns of a warp's 32 rows in 16 bits, a row to a lane, by way of shared memory (2 KB of the warp's own), so that lanes side by side
 // store to one row: 16 bytes by 4 lanes, 4 by 16 or 2 by 32 (`unit` numbers at a time), where a lane that stores its own row
 // touches a sector of its own each time.  `to`: where the lane's row goes, null: nowhere; `inside`: how many of the columns there are.
-template <class T>
-__device__ __forceinline__ void store_rows(T *to, const float (&v)[32], i64 inside, int unit, uint32_t stage, int lane) {
+template <class T, int N>
+__device__ __forceinline__ void store_rows(T *to, const float (&w)[N], i64 inside, int unit, uint32_t stage, int lane) {
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < 4; ++c)  // units of 16 bytes change places so that eight rows fall into different banks
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + (c ^ ((lane >> 1) & 3)) * 16),
-                     "r"(pack2<T>(v[8 * c], v[8 * c + 1])), "r"(pack2<T>(v[8 * c + 2], v[8 * c + 3])),
-                     "r"(pack2<T>(v[8 * c + 4], v[8 * c + 5])), "r"(pack2<T>(v[8 * c + 6], v[8 * c + 7]))
+                     "r"(pack2<T>(w[8 * c], w[8 * c + 1])), "r"(pack2<T>(w[8 * c + 2], w[8 * c + 3])),
+                     "r"(pack2<T>(w[8 * c + 4], w[8 * c + 5])), "r"(pack2<T>(w[8 * c + 6], w[8 * c + 7]))
                      : "memory");
     __syncwarp();
     if (unit == 8 && inside >= 32) {
@@ -253,7 +308,7 @@ __device__ __forceinline__ void store_rows(T *to, const float (&v)[32], i64 insi
     }
 }
 
-// The entries of one row in ascending order: what falls into each 32 columns.  The one behind the next is on its way already.
+// The entries of one row in ascending order: what falls into the columns at hand.  The one behind the next is on its way already.
 struct Walk {
     const int2 *entries;
     int at, all;
@@ -280,7 +335,8 @@ template <class T, int KIND, int GROUP>
 __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
     product_kernel(const __grid_constant__ Plan p, const __grid_constant__ Job job, const __grid_constant__ Maps maps) {
     constexpr bool LOGITS = KIND != GRADS;
-    constexpr int TILE = 128 * GROUP, COLUMNS = TILE / 2;  // columns that one epilogue thread takes of its row
+    constexpr int TILE = 128 * GROUP, COLUMNS = TILE / 2;  // columns that one epilogue thread takes of its row,
+    constexpr int W = KIND == STATS ? 64 : 32;             // and how many at a time
     // sums in 32 bits, the operands' type, TILE x TILE; dH has only its second operand across, dW both
     constexpr uint32_t WHAT = 1u << 4 | (std::is_same<T, __nv_bfloat16>::value ? 1u << 7 | 1u << 10 : 0u) | (LOGITS ? 0u : 1u << 16) |
                               (uint32_t)(TILE >> 3) << 17 | (uint32_t)(TILE >> 4) << 24;
@@ -547,104 +603,106 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             float4 *sums = (float4 *)p.split_sums + (((i64)(t.sums + (t.split < 0 ? 0 : t.split)) * GROUP + rank) * 8 + warp - 4) * (COLUMNS * 8) + lane;
             if (KIND == MAKE_R) {  // the maximum first, the sums are read twice
 #pragma unroll 1
-                for (int c = 0; c < COLUMNS && alive; c += 32) {
-                    uint32_t bits[32];
+                for (int c = 0; c < COLUMNS && alive; c += W) {
+                    uint32_t bits[W];
                     __syncwarp();
                     tmem_load(from + c, bits);
                     const i64 inside = p.vocab - (job.v0 + c0 + c);
-                    float highest[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    if (inside >= 32) {
+                    float v[W];
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) highest[x & 3] = fmaxf(highest[x & 3], __uint_as_float(bits[x]));
-                    } else {
+                    for (int x = 0; x < W; ++x) v[x] = __uint_as_float(bits[x]);
+                    if (inside < W) {
 #pragma unroll
-                        for (int x = 0; x < 32; ++x)
-                            if (x < inside) highest[x & 3] = fmaxf(highest[x & 3], __uint_as_float(bits[x]));
+                        for (int x = 0; x < W; ++x)
+                            if (x >= inside) v[x] = -INFINITY;
                     }
-                    top = fmaxf(top, fmaxf(fmaxf(highest[0], highest[1]), fmaxf(highest[2], highest[3])) * scale);
+                    top = fmaxf(top, largest(v) * scale);
                 }
                 top -= 14.f;
                 if (row >= 0) shift = top;
             }
 #pragma unroll 1
-            for (int c = 0; c < COLUMNS; c += 32) {
-                float v[32];
+            for (int c = 0; c < COLUMNS; c += W) {
+                float v[W];
                 __syncwarp();
                 if (alive) {
-                    uint32_t bits[32];
+                    uint32_t bits[W];
                     tmem_load(from + c, bits);
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) v[x] = t.k1 > t.k0 ? __uint_as_float(bits[x]) : 0.f;  // (no rows: nothing was summed)
-                    if (c + 32 == COLUMNS) {  // the buffer is free
+                    for (int x = 0; x < W; ++x) v[x] = LOGITS || t.k1 > t.k0 ? __uint_as_float(bits[x]) : 0.f;  // (no rows: nothing was summed)
+                    if (c + W == COLUMNS) {  // the buffer is free
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) barrier_arrive_cluster(GROUP == 2 ? in_cta(sums_empty + 8 * buffer, 0) : sums_empty + 8 * buffer);
                     }
                 } else {
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) v[x] = NAN;
+                    for (int x = 0; x < W; ++x) v[x] = NAN;
                 }
-                if (!LOGITS) {
+                if constexpr (!LOGITS) {
                     if (t.split < 0) {
                         emit(c, v);
                     } else {
 #pragma unroll
-                        for (int x = 0; x < 32; x += 4) __stcg(sums + (c + x) * 8, make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]));
+                        for (int x = 0; x < W; x += 4) __stcg(sums + (c + x) * 8, make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]));
                     }
                     continue;
                 }
                 const i64 j = job.v0 + c0 + c;  // first column, as a token id
                 if (KIND != MAKE_G) {
-                    while (walk.next.x < j + 32) {
+                    while (walk.next.x < j + W) {
                         const int x0 = walk.next.x - (int)j;
                         float z = 0.f;
 #pragma unroll
-                        for (int x = 0; x < 32; ++x)
+                        for (int x = 0; x < W; ++x)
                             if (x == x0) z = v[x];
                         p.entry_z[slot * entries_of_row + walk.at] = z;
                         walk.advance();
                     }
-                    if (j + 32 > p.vocab) {
+                    if (j + W > p.vocab) {
 #pragma unroll
-                        for (int x = 0; x < 32; ++x)
+                        for (int x = 0; x < W; ++x)
                             if (j + x >= p.vocab) v[x] = -INFINITY;
                     }
                     if (KIND != MAKE_R) {
-                        float highest[4] = {v[0], v[1], v[2], v[3]};  // (four chains of operations side by side)
-#pragma unroll
-                        for (int x = 4; x < 32; ++x) highest[x & 3] = fmaxf(highest[x & 3], v[x]);
-                        const float most = fmaxf(fmaxf(highest[0], highest[1]), fmaxf(highest[2], highest[3]));
-                        const float now = fmaxf(top, most * scale);
+                        const float now = fmaxf(top, largest(v) * scale);
                         if (KIND == STATS) sum *= exp2_fast(top - now), shift = now;
                         top = now;
                     }
                 }
+                const u64 scales = two(scale, scale), shifts = two(-shift, -shift);
 #pragma unroll
-                for (int x = 0; x < 32; ++x) v[x] = exp2_fast(fmaf(v[x], scale, -shift));
+                for (int x = 0; x < W; x += 2) {
+                    fma_two(v[x], v[x + 1], scales, shifts);
+                    v[x] = exp2_fast(v[x]), v[x + 1] = exp2_fast(v[x + 1]);
+                }
                 if (KIND != MAKE_G) {
-                    float part[4] = {v[0], v[1], v[2], v[3]};
+                    u64 part[2] = {two(v[0], v[1]), two(v[2], v[3])};
 #pragma unroll
-                    for (int x = 4; x < 32; ++x) part[x & 3] += v[x];
-                    sum += (part[0] + part[1]) + (part[2] + part[3]);
+                    for (int x = 4; x < W; x += 2) part[x / 2 & 1] = add_two(part[x / 2 & 1], two(v[x], v[x + 1]));
+                    float a, b;
+                    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(add_two(part[0], part[1])));
+                    sum += a + b;
                 }
                 if (KIND == MAKE_G) {
-                    while (walk.next.x < j + 32) {
+                    while (walk.next.x < j + W) {
                         const int x0 = walk.next.x - (int)j;
 #pragma unroll
-                        for (int x = 0; x < 32; ++x)
+                        for (int x = 0; x < W; ++x)
                             if (x == x0) v[x] -= __int_as_float(walk.next.y);
                         walk.advance();
                     }
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) v[x] *= coef;
-                    if (j + 32 > p.vocab) {
+                    for (int x = 0; x < W; ++x) v[x] *= coef;
+                    if (j + W > p.vocab) {
 #pragma unroll
-                        for (int x = 0; x < 32; ++x)
+                        for (int x = 0; x < W; ++x)
                             if (j + x >= p.vocab) v[x] = 0.f;
                     }
                 }
                 if (KIND != STATS) {
-                    if (c0 + c < p.g_stride) store_rows((T *)p.g + m * p.g_stride + c0 + c, v, 32, 8, stage, lane);
+                    T *to = (T *)p.g + m * p.g_stride + c0 + c;
+                    if (c0 + c < p.g_stride) store_rows(to, v, 32, 8, stage, lane);
                 }
             }
             if (LOGITS && KIND != MAKE_G && row >= 0 && job.v0 + c0 < p.vocab) {
