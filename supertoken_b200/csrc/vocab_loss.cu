@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
         // the row of this warp; the sum of its target's logit needs nothing of the parts
         const i64 m = m0 + warp, slot = r0 + m;
         const int row = m < n ? p.row_of[slot] : 0;
-        const bool refined = m < n && is_refined(p, row);
+        const int refined = m < n ? refined_entry(p, row, lane) : -1;
         float sum_z = 0.f;
         if (m0 + (lane & 7) < n) {
             const float *from_max = p.part_max + m0 + (lane & 7), *from_sum = p.part_sum + m0 + (lane & 7);
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
             const float m = __shfl_xor_sync(~0u, top, d), x = __shfl_xor_sync(~0u, sum, d);
             add(m, x);
         }
-        if (refined) sum_z = target_logit<T>(p, slot, row, lane);
+        if (refined >= 0) sum_z = entry_logit<T>(p, slot, row, refined, lane);
         if (lane < 8) tops[warp][lane] = top, sums[warp][lane] = sum;
         __syncthreads();
         if (threadIdx.x < 8) {

@@ -82,16 +82,25 @@ struct Plan {
 // ---------------------------------------------------------------------------------------------- one row, by one warp
 // The tensor cores cut their sums off at each step of 16 terms, always towards 0, so a sum that grows all along, as the logit of a token
 // that the row points to does, comes out short by 1e-8 to 1e-7 of itself a step (measured; 5e-6 in bf16 and 1e-5 in fp16 at
-// a width of 4 096).  Against that the target's logit is summed once more in rounded 32 bits, in the loss and in lse.
+// a width of 4 096).  Against that the target's logit, or that of an entry with more than half of the row's share, is summed once
+// more in rounded 32 bits, in the loss and in lse.
 constexpr int REFINED_DIM = 512;
 
-__device__ __forceinline__ bool is_refined(const Plan &p, int row) {
-    return !p.k && !p.few && p.dim > REFINED_DIM && p.entries[row].x != INT_MAX;
+// which entry of the row that is, -1: none
+__device__ __forceinline__ int refined_entry(const Plan &p, int row, int lane) {
+    if (p.few || p.dim <= REFINED_DIM) return -1;
+    if (!p.k) return p.entries[row].x != INT_MAX ? 0 : -1;
+    int found = -1;
+    for (int k = lane; k < p.k; k += 32) {
+        const int2 it = p.entries[(i64)row * p.k + k];
+        if (it.x != INT_MAX && __int_as_float(it.y) > 0.5f) found = k;
+    }
+    return __reduce_max_sync(~0u, found);
 }
 
 template <class T>
-__device__ __forceinline__ float target_logit(const Plan &p, i64 slot, int row, int lane) {
-    const T *w = (const T *)p.weight_rows + p.entries[row].x * p.weight_rows_stride, *h = (const T *)p.packed + slot * p.dim_padded;
+__device__ __forceinline__ float entry_logit(const Plan &p, i64 slot, int row, int k, int lane) {
+    const T *w = (const T *)p.weight_rows + p.entries[(i64)row * (p.k ? p.k : 1) + k].x * p.weight_rows_stride, *h = (const T *)p.packed + slot * p.dim_padded;
     float z = 0.f;
 #pragma unroll 4
     for (int d = lane * 8; d < p.dim_padded; d += 256) {
@@ -108,14 +117,14 @@ __device__ __forceinline__ float target_logit(const Plan &p, i64 slot, int row, 
 // rounded), the factor of the row's dH and the packed row times it for dW; where each part has its own, G in the place of E.
 // m: the row's place in the chunk; slice: which of the row's slices of columns this warp turns into G.
 template <class T>
-__device__ __forceinline__ void finish_row(const Plan &p, i64 m, i64 slot, int row, float lse2, float ref, bool refined, float target, int lane,
+__device__ __forceinline__ void finish_row(const Plan &p, i64 m, i64 slot, int row, float lse2, float ref, int refined, float target, int lane,
                                            int slice = 0, int slices = 1) {
     const int entries_of_row = p.k ? p.k : 1;
     const float scale = p.inv_temperature * 1.4426950408889634f;
     const int2 *e = p.entries + (i64)row * entries_of_row;
     const float *z = p.entry_z + slot * entries_of_row;
-    if (refined) {
-        const float before = z[0], share = exp2f(fmaf(before, scale, -lse2));
+    if (refined >= 0) {
+        const float before = z[refined], share = exp2f(fmaf(before, scale, -lse2));
         lse2 += log1pf(share * expm1f((target - before) * p.inv_temperature)) * 1.4426950408889634f;
     }
     float unit = exp2f(lse2 - ref), minus = ref, times = 1.f;  // a share, the logits and a factor in the units of E
@@ -148,7 +157,7 @@ __device__ __forceinline__ void finish_row(const Plan &p, i64 m, i64 slot, int r
     for (int k = lane; k < entries_of_row; k += 32) {
         const int2 it = e[k];
         if (it.x == INT_MAX) break;
-        const float its = refined ? target : z[k];
+        const float its = k == refined ? target : z[k];
         pz += __int_as_float(it.y) * its;
         if (p.keep && it.x >= from_j && it.x < to_j && (k == 0 || e[k - 1].x != it.x)) {  // (the same id again: its first entry takes them all)
             float share = __int_as_float(it.y);
@@ -188,8 +197,8 @@ __device__ __noinline__ void join_again(const Plan &p, i64 r0, i64 m0, i64 n, in
         for (int t = lane; t < p.parts; t += 32) sum += __ldcg(p.part_sum + t * p.part_stride + m);
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
         const float ref = p.reference[slot];
-        const bool refined = is_refined(p, row);
-        finish_row<T>(p, m, slot, row, ref + log2f(sum), ref, refined, refined ? target_logit<T>(p, slot, row, lane) : 0.f, lane);
+        const int refined = refined_entry(p, row, lane);
+        finish_row<T>(p, m, slot, row, ref + log2f(sum), ref, refined, refined >= 0 ? entry_logit<T>(p, slot, row, refined, lane) : 0.f, lane);
     }
 }
 

@@ -192,6 +192,8 @@ def test_teachers_entries():
     for T in (1.0, 2.5):
         check(hidden, weight, ids, logits, T=T)
         check(hidden, weight, ids.long(), logits, T=T, reduction="none")
+        wide = make(4, 30, 1040, 500)[:2]  # wide enough for an entry with most of the share to be summed once more
+        check(*wide, ids, logits, T=T, reduction="none")
     order = torch.randperm(24, device="cuda")
     a = ops.vocab_distillation(hidden, weight, ids, logits, reduction="none")
     b = ops.vocab_distillation(hidden, weight, ids[..., order].contiguous(), logits[..., order].contiguous(), reduction="none")
