@@ -125,7 +125,8 @@ __device__ __forceinline__ void finish_row(const Plan &p, i64 m, i64 slot, int r
     const float *z = p.entry_z + slot * entries_of_row;
     if (refined >= 0) {
         const float before = z[refined], share = exp2f(fmaf(before, scale, -lse2));
-        lse2 += log1pf(share * expm1f((target - before) * p.inv_temperature)) * 1.4426950408889634f;
+        // (a logit of -inf has no share, and no difference to itself)
+        if (share > 0.f) lse2 += log1pf(share * expm1f((target - before) * p.inv_temperature)) * 1.4426950408889634f;
     }
     float unit = exp2f(lse2 - ref), minus = ref, times = 1.f;  // a share, the logits and a factor in the units of E
     const i64 from_j = slice == 0 ? 0 : p.vocab * slice / slices / 8 * 8, to_j = slice + 1 == slices ? p.vocab : p.vocab * (slice + 1) / slices / 8 * 8;
