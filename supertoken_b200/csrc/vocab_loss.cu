@@ -63,8 +63,7 @@ __global__ void __launch_bounds__(128) teacher_kernel(Plan p) {
         for (int x = 0; x < ITEMS; ++x) {
             const int k = x * 32 + lane;
             id[x] = k < p.k ? load_id(p.ids, p.ids_bytes, id_at + k) : -1;
-            // rounded before anything is taken from it: the maximum less itself has to be 0 at the type's lowest value, too
-            t[x] = k < p.k ? __fmul_rn(load_real(p.logits, p.logits_type, real_at + k), p.inv_temperature) : 0.f;
+            t[x] = k < p.k ? load_real(p.logits, p.logits_type, real_at + k) : 0.f;
         }
         float top = -INFINITY, sum = 0.f, plogp = 0.f;
         bool bad = false;
@@ -80,9 +79,12 @@ __global__ void __launch_bounds__(128) teacher_kernel(Plan p) {
         for (int x = 0; x < ITEMS; ++x) nan |= id[x] >= 0 && isnan(t[x]);
         bad = __any_sync(~0u, bad), nan = __any_sync(~0u, nan);
         const bool counted = top > -INFINITY || nan;
+        // the difference first: a logit times 1 / temperature may leave the range of 32 bits, and the maximum less itself is 0
 #pragma unroll
-        for (int x = 0; x < ITEMS; ++x)
-            if (id[x] >= 0 && counted) sum += expf(t[x] - top);
+        for (int x = 0; x < ITEMS; ++x) {
+            t[x] = (t[x] - top) * p.inv_temperature;
+            if (id[x] >= 0 && counted) sum += expf(t[x]);
+        }
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
         const float inv = 1.f / sum, log_sum = logf(sum);
         u64 word[ITEMS];
@@ -90,9 +92,9 @@ __global__ void __launch_bounds__(128) teacher_kernel(Plan p) {
         for (int x = 0; x < ITEMS; ++x) {
             word[x] = ~0ull;  // no entry: behind all others
             if (id[x] < 0 || !counted || bad) continue;
-            const float share = expf(t[x] - top) * inv;
+            const float share = expf(t[x]) * inv;
             if (share > 0.f) {
-                plogp += share * (t[x] - top - log_sum);
+                plogp += share * (t[x] - log_sum);
                 word[x] = ((u64)id[x] << 32) | __float_as_uint(share);
             }
         }

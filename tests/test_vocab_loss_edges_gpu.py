@@ -38,3 +38,20 @@ def test_a_target_of_minus_infinity(rows, V, D, K):
         near(torch.where(others, loss, 0.0), want, "loss")
     gw = grads_of(hidden, weight, *rest, reduction="none")[2]
     assert not bool(gw[:V - 50].isnan().any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [0.01, 0.7, 1.0, 2.5])
+def test_a_teachers_lowest_and_largest_numbers(T, dtype):
+    """A logit above -inf is an entry, whatever the temperature: rows of the type's lowest and largest numbers are uniform."""
+    hidden, weight, ids, logits = make(2, 40, 64, 500, 40)
+    logits = logits.to(dtype)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    logits[0, 1], logits[0, 2], logits[0, 3], logits[0, 4, 1:] = low, high, low, low
+    logits[0, 3, 5], logits[0, 5, ::2], logits[0, 6, 1::2] = high, -math.inf, high
+    want = formula(hidden, weight, ids, logits, T=T, reduction="none")
+    assert not bool(want["loss"].isnan().any())
+    loss, gh, gw = ops.vocab_distillation_grads(hidden, weight, ids, logits, temperature=T, reduction="none")
+    near(loss, want, "loss"), near(gh, want, "gh"), near(gw, want, "gw")
+    mean = ops.vocab_distillation(hidden, weight, ids, logits, temperature=T)
+    near(mean, formula(hidden, weight, ids, logits, T=T), "loss")
