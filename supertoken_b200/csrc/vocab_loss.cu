@@ -486,6 +486,24 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
     }
 }
 
+// Gradients after the loss: the refined entry of a packed row and its share, a warp to a row.  Among entries of the same id it is the first, where G
+// takes the whole share.  Bound by the memory that the rows and their targets' rows of the weight come from.
+template <class T>
+__global__ void __launch_bounds__(256) refine_kernel(Plan p) {
+    next_may_come();
+    before_is_done();
+    const int lane = threadIdx.x & 31, n = p.meta->counted;
+    const float scale = p.inv_temperature * 1.4426950408889634f;
+    for (i64 slot = (i64)blockIdx.x * 8 + (threadIdx.x >> 5); slot < n; slot += (i64)gridDim.x * 8) {
+        const int row = p.row_of[slot];
+        int k = refined_entry(p, row, lane);
+        const float z = k >= 0 ? entry_logit<T>(p, slot, row, k, lane) : 0.f;
+        const int2 *e = p.entries + (i64)row * (p.k ? p.k : 1);
+        while (k > 0 && e[k - 1].x == e[k].x) --k;
+        if (lane == 0) p.refined[slot] = make_int2(k, __float_as_int(exp2f(fmaf(z, scale, -p.lse2[row]))));
+    }
+}
+
 // What comes down to the loss, onto gradients that were made with it.
 __global__ void __launch_bounds__(256) scale_kernel(__nv_bfloat16 *a, i64 n_a, __nv_bfloat16 *b, i64 n_b, const float *by) {
     next_may_come();
@@ -645,6 +663,7 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
         p.g = take(p.chunk_rows * p.g_stride * 2);
         p.split_sums = (float *)take((i64)2 * SMS * 8 * 64 * 2 * 32 * 4);
         p.split_done = (unsigned int *)take(2 * SMS * 8 * 4);
+        if (!p.keep && p.dim > REFINED_DIM) p.refined = (int2 *)take(p.rows_padded * 8);
         if (p.fixed) {
             p.reference = (float *)take(p.rows_padded * 4);
             p.out_row = (float *)take(p.rows_padded * 4);
@@ -778,6 +797,7 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
             VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, 0, p.rows_padded, 1));
         }
         if (p.want_grads) {
+            if (p.refined) VCK(start(refine_kernel<T>, blocks(p.rows, 8), 256, 0, 1, s, p));
             for (i64 v0 = 0; v0 < p.vocab; v0 += p.g_stride) {
                 const Job job{v0, p.vocab - v0 < p.g_stride ? p.vocab - v0 : p.g_stride, 0, p.rows_padded, false, false};
                 VTRY((product<T, MAKE_G>(p, job, logits, s, err, err_len)));

@@ -55,6 +55,7 @@ struct Plan {
     unsigned short *first;   // first entry of a row at or behind a piece's first column
     unsigned char *has_entries;
     float *entry_z;          // logits at the entries of a packed row
+    int2 *refined;           // anew: of a packed row, the entry whose logit is summed once more (-1: none), and its share of the row
     void *packed;            // counted rows of hidden, one behind another
     const void *weight_rows; // weight, or its copy with rows on 16-byte boundaries
     i64 weight_rows_stride;
@@ -83,7 +84,8 @@ struct Plan {
 // The tensor cores cut their sums off at each step of 16 terms, always towards 0, so a sum that grows all along, as the logit of a token
 // that the row points to does, comes out short by 1e-8 to 1e-7 of itself a step (measured; 5e-6 in bf16 and 1e-5 in fp16 at
 // a width of 4 096).  Against that the target's logit, or that of an entry with more than half of the row's share, is summed once
-// more in rounded 32 bits, in the loss and in lse.
+// more in rounded 32 bits, in the loss, in lse and in dlogits, which are small differences of two shares where the model is sure of its
+// token (a share about e^-7 below 1 at a width of 4 096 in fp16: dH and dW would be off by 28 % in the 2-norm, and are by 0.1 %).
 constexpr int REFINED_DIM = 512;
 
 // which entry of the row that is, -1: none

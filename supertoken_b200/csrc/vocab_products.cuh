@@ -540,13 +540,17 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
             int row = -1;
             // exp2(0 - inf) = 0 in the rows that fill the last tile up
             float shift = INFINITY, coef = 0.f, top = LOWEST, sum = 0.f;
+            int2 refined = make_int2(-1, 0);
             Walk walk;
             if (LOGITS) {
                 row = slot < p.rows_padded ? p.row_of[slot] : -1;
                 if (row >= 0 && job.v0 + c0 < p.vocab) walk.start(p, row, job.v0 + c0);
                 else walk.next.x = walk.then.x = INT_MAX, walk.at = walk.all = 0;
                 if (KIND == MAKE_E && row >= 0) shift = p.reference[slot];
-                if (KIND == MAKE_G && row >= 0) shift = p.lse2[row], coef = p.coef[slot] * p.meta->in_scale;
+                if (KIND == MAKE_G && row >= 0) {
+                    shift = p.lse2[row], coef = p.coef[slot] * p.meta->in_scale;
+                    if (p.refined) refined = p.refined[slot];
+                }
             }
             if (!LOGITS) {
                 coef = p.meta->out_scale;
@@ -689,7 +693,7 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                         const int x0 = walk.next.x - (int)j;
 #pragma unroll
                         for (int x = 0; x < W; ++x)
-                            if (x == x0) v[x] -= __int_as_float(walk.next.y);
+                            if (x == x0) v[x] = (walk.at == refined.x ? __int_as_float(refined.y) : v[x]) - __int_as_float(walk.next.y);
                         walk.advance();
                     }
 #pragma unroll

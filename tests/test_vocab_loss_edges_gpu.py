@@ -55,3 +55,78 @@ def test_a_teachers_lowest_and_largest_numbers(T, dtype):
     near(loss, want, "loss"), near(gh, want, "gh"), near(gw, want, "gw")
     mean = ops.vocab_distillation(hidden, weight, ids, logits, temperature=T)
     near(mean, formula(hidden, weight, ids, logits, T=T), "loss")
+
+
+def sure(rows, D, V, lean, dtype, K=0, twice=False):
+    """Rows that point to their target: losses far below 1.  A teacher has most of its share there, ``twice``: in two entries."""
+    hidden, weight, targets = make(1, rows, D, V, dtype=dtype)
+    hidden = (0.3 * hidden.float() + 40 * lean * weight[targets.long()].float()).to(dtype)
+    if not K:
+        return hidden, weight, targets
+    ids = torch.randint(0, V, (1, rows, K), device="cuda", generator=torch.Generator("cuda").manual_seed(0), dtype=torch.int32)
+    logits = torch.full((1, rows, K), -9.0, device="cuda")
+    ids[..., K // 2], logits[..., K // 2] = targets, 0.0
+    if twice:
+        ids[..., 0], logits[..., 0] = targets, -2.0
+    return hidden, weight, ids, logits
+
+
+def norms(hidden, weight, args, want, T, up):
+    """Bounds of the loss of a row and of the gradients' 2-norms.
+    A share q is off by 8 roundings of 32 bits of an exponent of |lse| / ln 2 + 1 at the most (the logit that is summed in 32 bits, its scaling, lse and its
+    logarithm, the difference, exp2, and what lse is saved in), and that is what the target's dlogit, a difference of shares, is off by beside
+    its own rounding.  Logits that are summed by the tensor cores are off by (D / 16 + 4) 2^-23 of the largest of a row: D / 16 steps, cut off at 32 bits, and
+    that is what the other shares are off by, of themselves.  In both gradients up to three roundings to 16 bits (E, G or a H, the result) count,
+    each of at most u / sqrt(3) in the 2-norm as errors are spread evenly over a step, together u."""
+    u = torch.finfo(hidden.dtype).eps / 2
+    n, D = hidden.shape[1], hidden.shape[2]
+    h, w, ids = hidden[0].double(), weight.double(), args[0].reshape(n, -1).long()
+    z = h @ w.T / T
+    lse = torch.logsumexp(z, 1)
+    off = 8 * 2.0 ** -24 * (lse.abs() / math.log(2) + 1)
+    cut = (D / 16 + 4) * E32 * z.abs().amax(1)
+    t = ids[:, -1] if len(args) == 1 else ids[:, ids.shape[1] // 2]
+    rest = -torch.expm1(z.gather(1, t[:, None])[:, 0] - lse)  # shares of all but the target
+    loss_tol = T * T * (off + cut * rest + 16 * E32)
+    f = up.double() * T
+    dG = f * (off + cut * rest)
+    gh = (dG[:, None] * w[t]).norm()
+    gw = torch.zeros_like(w).index_add_(0, t, dG[:, None] * h).norm()
+    # (a teacher's other entries are not summed again)
+    if len(args) == 2:
+        gh, gw = 2 * gh, 2 * gw
+    return loss_tol, u, float(gh / want["gh"].norm()), float(gw / want["gw"].norm())
+
+
+def near_in_norm(got, want, u, extra, name):
+    got, want = got.double().flatten(), want.flatten()
+    off, along = float((got - want).norm() / want.norm()), float(got @ want / (want @ want)) - 1
+    assert off <= u + extra, f"{name}: {off:.3g} off in the 2-norm, {u + extra:.3g} allowed"
+    # a value rounds to 16 bits with all of its likes, but by less than half of u where it lies just below a power of two as a target's dlogit does
+    assert abs(along) <= u / 2 + extra, f"{name}: too large by {along:.3g}, {u / 2 + extra:.3g} allowed"
+
+
+@pytest.mark.parametrize("K,twice", [(0, False), (6, False)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,D,V,lean", [(300, 2048, 5000, 0.3), (300, 4096, 5000, 0.3), (300, 4096, 5000, 0.4), (1000, 2056, 30_000, 0.3)])
+def test_rows_that_are_sure_of_their_target(rows, D, V, lean, dtype, K, twice):
+    """Losses and dlogits are small differences there, for which the target's logit is summed in 32 bits, in every way to the gradients."""
+    hidden, weight, *args = sure(rows, D, V, lean, dtype, K, twice)
+    loss_of, grads_of = (ops.vocab_distillation, ops.vocab_distillation_grads) if K else (ops.vocab_cross_entropy, ops.vocab_cross_entropy_grads)
+    for reduction, up in (("mean", torch.full((rows,), 4096.0 / rows, device="cuda")),
+                          ("none", torch.linspace(256.0, 4096.0, rows, device="cuda"))):
+        grad = 4096.0 if reduction == "mean" else up[None]
+        want = formula(hidden, weight, *args, reduction=reduction, grad=grad)
+        each = formula(hidden, weight, *args, reduction="none")["loss"][0]
+        loss_tol, u, gh_extra, gw_extra = norms(hidden, weight, args, want, 1.0, up)
+        loss, gh, gw = grads_of(hidden, weight, *args, None, grad, reduction=reduction)
+        h, w = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+        auto = loss_of(h, w, *args, reduction=reduction)
+        ah, aw = torch.autograd.grad(auto, (h, w), torch.as_tensor(grad, device="cuda").expand_as(auto))
+        for x in (loss, auto.detach(), loss_of(hidden, weight, *args, reduction=reduction)):
+            if reduction == "none":
+                assert bool(((x[0].double() - each).abs() <= loss_tol).all())
+            else:
+                assert abs(float(x) - float(each.mean())) <= float(loss_tol.mean()) + 64 * E32 * float(each.abs().mean())
+        for name, x in (("gh", gh), ("gh", ah), ("gw", gw), ("gw", aw)):
+            near_in_norm(x, want[name], u, gh_extra if name == "gh" else gw_extra, f"{name}, {reduction}")
