@@ -130,6 +130,7 @@ __device__ __forceinline__ void finish_row(const Plan &p, i64 m, i64 slot, int r
         // (a logit of -inf has no share, and no difference to itself)
         if (share > 0.f) lse2 += log1pf(share * expm1f((target - before) * p.inv_temperature)) * 1.4426950408889634f;
     }
+    const int refined_id = refined >= 0 ? e[refined].x : -1;  // (in more than one entry, if a teacher gives it twice)
     float unit = exp2f(lse2 - ref), minus = ref, times = 1.f;  // a share, the logits and a factor in the units of E
     const i64 from_j = slice == 0 ? 0 : p.vocab * slice / slices / 8 * 8, to_j = slice + 1 == slices ? p.vocab : p.vocab * (slice + 1) / slices / 8 * 8;
     if (p.keep && !p.fixed) {
@@ -160,7 +161,7 @@ __device__ __forceinline__ void finish_row(const Plan &p, i64 m, i64 slot, int r
     for (int k = lane; k < entries_of_row; k += 32) {
         const int2 it = e[k];
         if (it.x == INT_MAX) break;
-        const float its = k == refined ? target : z[k];
+        const float its = it.x == refined_id ? target : z[k];
         pz += __int_as_float(it.y) * its;
         if (p.keep && it.x >= from_j && it.x < to_j && (k == 0 || e[k - 1].x != it.x)) {  // (the same id again: its first entry takes them all)
             float share = __int_as_float(it.y);

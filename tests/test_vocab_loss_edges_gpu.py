@@ -106,7 +106,7 @@ def near_in_norm(got, want, u, extra, name):
     assert abs(along) <= u / 2 + extra, f"{name}: too large by {along:.3g}, {u / 2 + extra:.3g} allowed"
 
 
-@pytest.mark.parametrize("K,twice", [(0, False), (6, False)])
+@pytest.mark.parametrize("K,twice", [(0, False), (6, False), (6, True)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,D,V,lean", [(300, 2048, 5000, 0.3), (300, 4096, 5000, 0.3), (300, 4096, 5000, 0.4), (1000, 2056, 30_000, 0.3)])
 def test_rows_that_are_sure_of_their_target(rows, D, V, lean, dtype, K, twice):
