@@ -447,6 +447,8 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
             top = tops[0][lane], sum = sums[0][lane];
             for (int w = 1; w < 8; ++w) add(tops[w][lane], sums[w][lane]);
             float ref = top;
+            // a logit of +inf makes the sum NaN about a maximum, and has to about a fixed reference
+            if (p.fixed && top == INFINITY) sum = NAN;
             if (p.fixed && m0 + lane < n) {
                 ref = p.reference[r0 + m0 + lane];
                 if (fabsf(top - ref) > 96.f && fabsf(top) < INFINITY) {

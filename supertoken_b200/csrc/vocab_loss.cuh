@@ -200,6 +200,7 @@ __device__ __noinline__ void join_again(const Plan &p, i64 r0, i64 m0, i64 n, in
         float sum = 0.f;
         for (int t = lane; t < p.parts; t += 32) sum += __ldcg(p.part_sum + t * p.part_stride + m);
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        if (sum == INFINITY) sum = NAN;  // a logit of +inf: no other is that far from its reference by now
         const float ref = p.reference[slot];
         const int refined = refined_entry(p, row, lane);
         finish_row<T>(p, m, slot, row, ref + log2f(sum), ref, refined, refined >= 0 ? entry_logit<T>(p, slot, row, refined, lane) : 0.f, lane);

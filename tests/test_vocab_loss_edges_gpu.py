@@ -130,3 +130,24 @@ def test_rows_that_are_sure_of_their_target(rows, D, V, lean, dtype, K, twice):
                 assert abs(float(x) - float(each.mean())) <= float(loss_tol.mean()) + 64 * E32 * float(each.abs().mean())
         for name, x in (("gh", gh), ("gh", ah), ("gw", gw), ("gw", aw)):
             near_in_norm(x, want[name], u, gh_extra if name == "gh" else gw_extra, f"{name}, {reduction}")
+
+
+@pytest.mark.parametrize("K", [0, 3])
+@pytest.mark.parametrize("far", [0.0, 200.0])  # (a row beside it that has the tile made again)
+@pytest.mark.parametrize("rows,V", BOTH_WAYS)
+def test_a_logit_of_plus_infinity(rows, V, far, K):
+    """There are no shares then: loss, the row's gradient and the weight's are NaN by every call, whichever the target is."""
+    hidden, weight, *rest = make(1, rows, 64, V, K)
+    hidden[..., 0], weight[:, 0] = 0.0, -1.0
+    hidden[0, 5, 0], hidden[0, 9, 0], weight[V // 2, 0] = math.inf, far, 1.0
+    loss_of, grads_of = (ops.vocab_distillation, ops.vocab_distillation_grads) if K else (ops.vocab_cross_entropy, ops.vocab_cross_entropy_grads)
+    for target in (V // 2, V // 2 + 1):
+        rest[0][0, 5] = target
+        loss, gh, gw = grads_of(hidden, weight, *rest, reduction="none")
+        assert loss.isnan().nonzero().tolist() == [[0, 5]] and bool(gh[0, 5].isnan().all()) and bool(gw.isnan().all())
+        assert not bool(gh[0, :5].isnan().any()) and not bool(gh[0, 6:].isnan().any())
+        assert loss_of(hidden, weight, *rest, reduction="none").isnan().nonzero().tolist() == [[0, 5]]
+        h, w = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+        for reduction in ("none", "mean"):
+            ah, aw = torch.autograd.grad(loss_of(h, w, *rest, reduction=reduction).sum(), (h, w))
+            assert ah[0].isnan().any(1).nonzero().tolist() == [[5]] and bool(ah[0, 5].isnan().all()) and bool(aw.isnan().all())
