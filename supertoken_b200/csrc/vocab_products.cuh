@@ -552,6 +552,8 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                     if (p.refined) refined = p.refined[slot];
                 }
             }
+            // E and G of the rows that fill the last tile up are 0 whatever the weight holds (0 times a weight of -inf is NaN)
+            const bool filled = LOGITS && KIND != STATS && __any_sync(~0u, row < 0);
             if (!LOGITS) {
                 coef = p.meta->out_scale;
                 if (t.result == 0 && m < n) {
@@ -651,6 +653,10 @@ __global__ void __launch_bounds__(PRODUCT_THREADS, 1)
                         for (int x = 0; x < W; x += 4) __stcg(sums + (c + x) * 8, make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]));
                     }
                     continue;
+                }
+                if (filled) {
+#pragma unroll
+                    for (int x = 0; x < W; ++x) v[x] = row < 0 ? 0.f : v[x];
                 }
                 const i64 j = job.v0 + c0 + c;  // first column, as a token id
                 if (KIND != MAKE_G) {

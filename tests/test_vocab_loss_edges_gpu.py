@@ -151,3 +151,22 @@ def test_a_logit_of_plus_infinity(rows, V, far, K):
         for reduction in ("none", "mean"):
             ah, aw = torch.autograd.grad(loss_of(h, w, *rest, reduction=reduction).sum(), (h, w))
             assert ah[0].isnan().any(1).nonzero().tolist() == [[5]] and bool(ah[0, 5].isnan().all()) and bool(aw.isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K", [0, 3])
+@pytest.mark.parametrize("rows,V", BOTH_WAYS + [(256, 300)])
+def test_ids_that_the_weight_rules_out(rows, V, K, dtype):
+    """Logits of -inf by way of the weight: those ids' rows of its gradient are 0, the others as if they were not there."""
+    hidden, weight, *rest = make(1, rows, 64, V, K, dtype=dtype)
+    hidden[..., 0] = 1.0
+    weight[V - 50:, 0] = -math.inf
+    rest[0].clamp_(max=V - 51)
+    want = formula(hidden, weight[:V - 50], *rest, reduction="sum", grad=64.0)
+    loss_of, grads_of = (ops.vocab_distillation, ops.vocab_distillation_grads) if K else (ops.vocab_cross_entropy, ops.vocab_cross_entropy_grads)
+    loss, _, gw = grads_of(hidden, weight, *rest, None, 64.0, reduction="sum")
+    near(loss, want, "loss"), near(gw[:V - 50], want, "gw")
+    w = weight.clone().requires_grad_(True)
+    aw, = torch.autograd.grad(loss_of(hidden, w, *rest, reduction="none").sum(), w, torch.tensor(64.0, device="cuda"))
+    near(aw[:V - 50], want, "gw")
+    assert not bool(gw[V - 50:].any()) and not bool(aw[V - 50:].any())
