@@ -13,8 +13,8 @@
 //           With c_i = 0 for a row (bf16, where E is above 48 MB and that pass would cost 3 to 6 % of a step) E stays, but for the entries,
 //           and a_i = g_i T exp2(c_i - lse2_i) goes to the other factors: dH = a (E W), dW = E^T (a H).  One rounding more
 //           reaches dW, 0.0028 off in the 2-norm against 0.0022, where the result's own rounding is 0.0017.  A row whose
-//           largest logit lies further than a factor of 2^96 from c_i gets it as its reference and its tile is made again, which logits
-//           below 66 in size never need.
+//           largest logit lies more than a factor of 2^96 above c_i or 2^80 below gets it as its reference and its tile is made again, which
+//           a largest logit between -55 and 66 never needs.
 //   anew    (gradients after the loss, as fp16 and losses per row need them through autograd): z is made a second time,
 //           and G from it for up to 1 GiB of the vocabulary at a time.  Three products behind the loss's one.
 #include <cuda_bf16.h>
@@ -451,7 +451,9 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
             if (p.fixed && top == INFINITY) sum = NAN;
             if (p.fixed && m0 + lane < n) {
                 ref = p.reference[r0 + m0 + lane];
-                if (fabsf(top - ref) > 96.f && fabsf(top) < INFINITY) {
+                // above, exp2 must not overflow; below, 2^-126 is the least that is kept, 2^-46 of the maximum then: 2^-25 of it for 2^21 ids
+                const float above = top - ref;
+                if ((above > 96.f || above < -80.f) && fabsf(top) < INFINITY) {
                     p.reference[r0 + m0 + lane] = top;
                     p.again[(r0 + m0) / TILE_ROWS] = p.meta->again = 1;
                 }

@@ -170,3 +170,24 @@ def test_ids_that_the_weight_rules_out(rows, V, K, dtype):
     aw, = torch.autograd.grad(loss_of(hidden, w, *rest, reduction="none").sum(), w, torch.tensor(64.0, device="cuda"))
     near(aw[:V - 50], want, "gw")
     assert not bool(gw[V - 50:].any()) and not bool(aw[V - 50:].any())
+
+
+@pytest.mark.parametrize("top,low", [(-66.0, -87.5), (-60.0, -80.0), (-56.0, -76.0), (-55.0, -75.0), (0.0, -20.0), (66.0, 46.0), (68.0, 48.0)])
+def test_small_shares_of_many_ids(top, low):
+    """One id far above 300 000 others, which together are a small part of the row wherever its logits lie.  One product a logit, exact in 32
+    bits; lse is off by 8 roundings of its exponent at the most, and by those of its sum: at most 128 columns of a part to the sum with the large one in
+    it, two at a time and four sums at the end, less than 70 additions, then every 32nd of 2 344 or 4 688 parts, 147 at most, and 10 to
+    bring those sums together; 227 times half a step of a sum of 1 to 2, 2^-24.  Gradients: three roundings to 16 bits and that."""
+    V, rows = 300_001, 100
+    hidden = torch.zeros(1, rows, 64, device="cuda", dtype=torch.bfloat16)
+    weight = torch.zeros(V, 64, device="cuda", dtype=torch.bfloat16)
+    hidden[..., 0], weight[:, 0], weight[77, 0] = 1.0, low, top
+    targets = torch.full((1, rows), 77, device="cuda")
+    rest = (V - 1) * math.exp(low - top)
+    off = 8 * 2.0 ** -24 * (abs(top) / math.log(2) + 1) + 227 * 2.0 ** -24
+    loss, gh, gw = ops.vocab_cross_entropy_grads(hidden, weight, targets)
+    for x in (loss, ops.vocab_cross_entropy(hidden, weight, targets)):
+        assert abs(float(x) - math.log1p(rest)) <= off
+    q = math.exp(low - top) / (1 + rest)
+    others = torch.cat([gw[:77, 0], gw[78:, 0]]).double() / q - 1
+    assert float(others.abs().max()) <= 3.1 * 2.0 ** -8 + 2 * off
