@@ -412,6 +412,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
     next_may_come();
     before_is_done();
     __shared__ float tops[8][8], sums[8][8], lse2s[8], refs[8];
+    __shared__ double losses[8];
     __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const i64 counted = p.meta->counted;
@@ -477,16 +478,16 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
     __syncthreads();
     if (!last) return;
     __threadfence();
-    float sum = 0.f;
+    double sum = 0.0;  // (as in add_up)
 #pragma unroll 8
     for (i64 r = threadIdx.x; r < p.rows; r += 256) sum += __ldcg(p.row_loss + r);
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-    if (lane == 0) sums[0][warp] = sum;
+    if (lane == 0) losses[warp] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
-        float all = 0.f;
-        for (int w = 0; w < 8; ++w) all += sums[0][w];
-        p.loss[0] = p.reduction == STBPE_REDUCE_MEAN ? all / (float)(counted > 0 ? counted : 1) : all;
+        double all = 0.0;
+        for (int w = 0; w < 8; ++w) all += losses[w];
+        p.loss[0] = (float)(p.reduction == STBPE_REDUCE_MEAN ? all / (counted > 0 ? counted : 1) : all);
     }
 }
 

@@ -207,14 +207,15 @@ __device__ __noinline__ void join_again(const Plan &p, i64 r0, i64 m0, i64 n, in
     }
 }
 
-// The losses of all rows, in their order, by one warp.
+// The losses of all rows, in their order, by one warp.  In 64 bits: a lane of 2^20 rows of the same loss rounds 32 768 times the same way in 32,
+// 2e-4 of the mean.
 __device__ __forceinline__ void add_up(const Plan &p, int lane) {
-    float sum = 0.f;
+    double sum = 0.0;
 #pragma unroll 16
     for (i64 r = lane; r < p.rows; r += 32) sum += p.row_loss[r];
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
     const int n = p.meta->counted;
-    if (lane == 0) p.loss[0] = p.reduction == STBPE_REDUCE_MEAN ? sum / (float)(n > 0 ? n : 1) : sum;
+    if (lane == 0) p.loss[0] = (float)(p.reduction == STBPE_REDUCE_MEAN ? sum / (n > 0 ? n : 1) : sum);
 }
 
 }  // namespace vloss

@@ -11,7 +11,7 @@ A row counts unless ``valid`` is 0 there or its target is negative (the padding 
 no entry with an id of 0 or more and a logit above ``-inf``.  Rows that do not count have a loss and a gradient of 0, and
 what ``hidden`` holds there is not looked at.  ``reduction="mean"`` divides by the rows that count (0 if none does).  Nothing is read back, so
 an id of ``V`` or more cannot raise: it makes the loss NaN, as a NaN among the inputs does.  Results are the same at every call with the same
-inputs; sums are held in 32 bits."""
+inputs; sums are held in 32 bits, those of the losses of rows in 64."""
 from __future__ import annotations
 
 import ctypes

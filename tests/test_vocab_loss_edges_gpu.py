@@ -191,3 +191,16 @@ def test_small_shares_of_many_ids(top, low):
     q = math.exp(low - top) / (1 + rest)
     others = torch.cat([gw[:77, 0], gw[78:, 0]]).double() / q - 1
     assert float(others.abs().max()) <= 3.1 * 2.0 ** -8 + 2 * off
+
+
+@pytest.mark.parametrize("V", [11, 1000])
+@pytest.mark.parametrize("rows", [300, 8192, 1 << 20])
+def test_the_mean_of_many_equal_losses(rows, V):
+    """Logits of 0: every row's loss is log V by four roundings of 32 bits at the most (log2 of the sum, its product with ln 2, ln 2 itself, the difference
+    to the target's 0), and so is their mean, with one rounding more."""
+    hidden = torch.zeros(rows, 8, device="cuda", dtype=torch.bfloat16)
+    weight, targets = torch.zeros(V, 8, device="cuda", dtype=torch.bfloat16), torch.zeros(rows, device="cuda", dtype=torch.int32)
+    for reduction, by in (("mean", 1), ("sum", rows)):
+        for loss in (ops.vocab_cross_entropy(hidden, weight, targets, reduction=reduction),
+                     ops.vocab_cross_entropy_grads(hidden, weight, targets, reduction=reduction)[0]):
+            assert abs(float(loss) / by / math.log(V) - 1) <= 5 * 2.0 ** -24
