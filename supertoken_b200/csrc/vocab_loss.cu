@@ -289,7 +289,8 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
         for (int x = threadIdx.x; x < 2 * SMS * 8; x += 1024) p.split_done[x] = 0;
     if (threadIdx.x == 0) {
         const float factor = p.temperature / (p.reduction == STBPE_REDUCE_MEAN ? (float)(n > 0 ? n : 1) : 1.f);
-        const float in = 16376.f / fminf(fmaxf(most * factor, 1e-30f), 1e30f);
+        // (in times factor is finite where all are 0, too, up to a temperature of 2e9)
+        const float in = 16376.f / fminf(fmaxf(most * factor, 1e-25f), 1e30f);
         p.meta->counted = (int)n, p.meta->tickets = 0, p.meta->again = 0;
         p.meta->in_scale = (each ? 1.f : one) * factor * in;
         p.meta->out_scale = 1.f / in;

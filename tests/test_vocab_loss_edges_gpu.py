@@ -204,3 +204,16 @@ def test_the_mean_of_many_equal_losses(rows, V):
         for loss in (ops.vocab_cross_entropy(hidden, weight, targets, reduction=reduction),
                      ops.vocab_cross_entropy_grads(hidden, weight, targets, reduction=reduction)[0]):
             assert abs(float(loss) / by / math.log(V) - 1) <= 5 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [1.0, 2.0 ** 15, 2.0 ** 16])
+def test_nothing_comes_down_to_the_loss(T, dtype):
+    hidden, weight, ids, logits = make(2, 70, 64, 500, 4, dtype=dtype)
+    for reduction, grad in (("none", torch.zeros(2, 70, device="cuda")), ("sum", 0.0), ("mean", 0.0)):
+        loss, gh, gw = ops.vocab_distillation_grads(hidden, weight, ids, logits, None, grad, temperature=T, reduction=reduction)
+        near(loss, formula(hidden, weight, ids, logits, T=T, reduction=reduction), "loss")
+        assert bool((gh == 0).all()) and bool((gw == 0).all())
+        h, w = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+        auto = ops.vocab_distillation(h, w, ids, logits, temperature=T, reduction=reduction)
+        assert all(bool((x == 0).all()) for x in torch.autograd.grad(auto, (h, w), torch.zeros_like(auto)))
