@@ -345,6 +345,8 @@ int stbpe_rows_count_pairs_noalloc(const int32_t *tokens, const uint8_t *valid, 
 #define STBPE_WANT_LOSS 1
 #define STBPE_WANT_GRADS 2
 #define STBPE_VOCAB_LOSS_MAX_K 256
+#define STBPE_MIN_TEMPERATURE (1.f / 65536.f)
+#define STBPE_MAX_TEMPERATURE 65536.f
 
 typedef struct stbpe_vocab_loss {
     int64_t outer, inner, vocab, dim;
@@ -354,7 +356,7 @@ typedef struct stbpe_vocab_loss {
     int32_t logits_type;         /* STBPE_REAL_* */
     int32_t reduction;           /* STBPE_REDUCE_* */
     int32_t want;                /* STBPE_WANT_* */
-    float temperature;           /* 1 where k is 0 */
+    float temperature;           /* STBPE_MIN_TEMPERATURE to _MAX_TEMPERATURE; 1 where k is 0 */
     int32_t reserved;
     const void *hidden;          /* [outer][inner][dim] */
     int64_t hidden_outer, hidden_inner;

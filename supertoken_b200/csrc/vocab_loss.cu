@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
         for (int x = threadIdx.x; x < 2 * SMS * 8; x += 1024) p.split_done[x] = 0;
     if (threadIdx.x == 0) {
         const float factor = p.temperature / (p.reduction == STBPE_REDUCE_MEAN ? (float)(n > 0 ? n : 1) : 1.f);
-        // (in times factor is finite where all are 0, too, up to a temperature of 2e9)
+        // (in times factor is finite where all are 0, too)
         const float in = 16376.f / fminf(fmaxf(most * factor, 1e-25f), 1e30f);
         p.meta->counted = (int)n, p.meta->tickets = 0, p.meta->again = 0;
         p.meta->in_scale = (each ? 1.f : one) * factor * in;
@@ -596,7 +596,8 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     if (a->k < 0 || a->k > STBPE_VOCAB_LOSS_MAX_K) return bad("number of teacher entries out of range");
     if (a->ids_bytes != 4 && a->ids_bytes != 8) return bad("ids have 4 or 8 bytes");
     if (a->k && (a->logits_type < STBPE_REAL_BF16 || a->logits_type > STBPE_REAL_FP32)) return bad("type of the teacher's logits");
-    if (!(a->temperature > 0.f) || !std::isfinite(a->temperature) || !std::isfinite(1.f / a->temperature)) return bad("temperature is positive and finite");
+    // below, logits over it leave the 24 bits that a difference of theirs is taken in; above, its square and the gradients' scale the exponents of 32
+    if (!(a->temperature >= STBPE_MIN_TEMPERATURE && a->temperature <= STBPE_MAX_TEMPERATURE)) return bad("temperature is between 2^-16 and 2^16");
     if (!a->k && a->temperature != 1.f) return bad("cross entropy has no temperature");
     if (a->reduction < STBPE_REDUCE_NONE || a->reduction > STBPE_REDUCE_MEAN) return bad("reduction");
     if (!(a->want & (STBPE_WANT_LOSS | STBPE_WANT_GRADS))) return bad("nothing is wanted");

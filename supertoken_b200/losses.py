@@ -25,6 +25,7 @@ _REAL = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _WANT_LOSS, _WANT_GRADS = 1, 2
 MAX_TEACHER_ENTRIES = 256
+MIN_TEMPERATURE, MAX_TEMPERATURE = 2.0 ** -16, 2.0 ** 16
 
 
 def _raise(status: int, msg: str) -> None:
@@ -81,8 +82,8 @@ def _arguments(hidden, weight, ids, logits, valid, temperature, reduction) -> L.
             raise ValueError(f"a teacher gives 1 to {MAX_TEACHER_ENTRIES} entries per row")
         if k > 1 and (ids.stride(-1) != 1 or logits.stride(-1) != 1):
             raise ValueError("the last dimension of teacher_ids and teacher_logits must be contiguous")
-        if not (0.0 < temperature < float("inf")):
-            raise ValueError("temperature must be positive and finite")
+        if not MIN_TEMPERATURE <= temperature <= MAX_TEMPERATURE:
+            raise ValueError("temperature must lie between 2^-16 and 2^16")
         a.logits, a.logits_type = logits.data_ptr(), _REAL[logits.dtype]
         a.logits_outer, a.logits_inner = _rows(logits, lead)
     if lead == 2:
@@ -247,7 +248,7 @@ def vocab_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: 
                        teacher_logits: torch.Tensor, valid: Optional[torch.Tensor] = None, *, temperature: float = 1.0,
                        reduction: str = "mean") -> torch.Tensor:
     """``T^2 KL(p || softmax(hidden @ weight.T / T))`` with ``p = softmax(teacher_logits / T)`` over the teacher's up to 256
-    entries of a row (in any order; an id below 0 is no entry, the same id twice counts twice).  Gradients and captures as with
+    entries of a row (in any order; an id below 0 is no entry, the same id twice counts twice); ``T`` between 2^-16 and 2^16.  Gradients and captures as with
     ``vocab_cross_entropy``."""
     if teacher_logits is None:
         raise TypeError("teacher_logits must be a tensor")

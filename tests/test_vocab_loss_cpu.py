@@ -72,3 +72,11 @@ def test_cpu_tensors_are_refused():
             call()
     with pytest.raises(TypeError):
         losses.vocab_distillation(h, w, t[:, None], None)
+
+
+def test_temperatures_that_32_bits_do_not_hold():
+    for t in (2.0 ** -16, 0.01, 2.0 ** 16):
+        assert _need(_args(k=4, logits_type=2, temperature=t))[0] == L.OK
+    for t in (1e-20, 1e-10, 1e-5, 65537.0, 1e20, -2.0):
+        st, n, text = _need(_args(k=4, logits_type=2, temperature=t))
+        assert st == L.E_BADARG and n == -1 and "temperature" in text

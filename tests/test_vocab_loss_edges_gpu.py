@@ -217,3 +217,24 @@ def test_nothing_comes_down_to_the_loss(T, dtype):
         h, w = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
         auto = ops.vocab_distillation(h, w, ids, logits, temperature=T, reduction=reduction)
         assert all(bool((x == 0).all()) for x in torch.autograd.grad(auto, (h, w), torch.zeros_like(auto)))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [2.0 ** -16, 2.0 ** -10, 2.0 ** 16])
+def test_the_range_of_temperatures(T, dtype):
+    args = make(2, 70, 64, 500, 4, dtype=dtype)
+    for reduction in ("none", "mean"):
+        want = formula(*args, T=T, reduction=reduction)
+        out = ops.vocab_distillation_grads(*args, temperature=T, reduction=reduction)
+        for name, x in zip(("loss", "gh", "gw"), out):
+            over = want[name].abs() > torch.finfo(x.dtype).max  # (65 536 times what a gradient is at a temperature of 1, in fp16: rounds to infinity)
+            assert bool((x[over] == want[name][over].sign() * math.inf).all())
+            want[name + "_tol"] = torch.where(over, math.inf, want[name + "_tol"])
+            near(torch.where(over, 0.0, x), want, name)
+    empty = [x[:, :0] for x in (args[0], args[2], args[3])]
+    for t in (2.0 ** -17, 1e-10, 2.0 ** 17, 1e20):
+        for h, ids, logits in ((args[0], *args[2:]), empty):
+            with pytest.raises(ValueError, match="temperature"):
+                ops.vocab_distillation(h, args[1], ids, logits, temperature=t, reduction="none")
+            with pytest.raises(ValueError, match="temperature"):
+                ops.vocab_distillation_grads(h, args[1], ids, logits, temperature=t, reduction="none")
