@@ -18,6 +18,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -39,6 +40,12 @@ def _rows(t: torch.Tensor, lead: int) -> Tuple[int, int]:
     return (t.stride(0), t.stride(1)) if lead == 2 else (0, t.stride(0))
 
 
+def _refuse_tangents(*tensors) -> None:
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the losses over a large vocabulary have no forward-mode derivative")
+
+
 def _arguments(hidden, weight, ids, logits, valid, temperature, reduction) -> L.VocabLoss:
     device, kd = getattr(hidden, "device", None), logits is not None
     for t in (hidden, weight, ids, logits if kd else ids, ids if valid is None else valid):
@@ -48,6 +55,7 @@ def _arguments(hidden, weight, ids, logits, valid, temperature, reduction) -> L.
             raise RuntimeError("supertoken_b200 operators need CUDA tensors; there is no CPU fallback")
         if t.device != device:
             raise ValueError("tensors must be on one device")
+    _refuse_tangents(hidden, weight, logits)
     dtype = hidden.dtype
     if (dtype != torch.bfloat16 and dtype != torch.float16) or weight.dtype != dtype:
         raise TypeError("hidden and weight must both be bfloat16 or both be float16")
@@ -137,6 +145,7 @@ def _grads(a, hidden, weight, reduction, grad_loss, lse2, want_hidden=True, want
     if grad_loss is not None:
         if not isinstance(grad_loss, torch.Tensor):
             grad_loss = torch.full((), float(grad_loss), dtype=torch.float32, device=hidden.device)
+        _refuse_tangents(grad_loss)
         if grad_loss.device != hidden.device:
             raise ValueError("tensors must be on one device")
         if grad_loss.dtype != torch.float32:
@@ -185,6 +194,7 @@ class _VocabLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
         _refuse_capture(grad_loss.device)
+        _refuse_tangents(grad_loss)
         if ctx.grads is not None:
             (gh, gw), ctx.grads = ctx.grads, None  # they are given away: a second pass makes its own
             _scale(gh, gw, grad_loss)
@@ -230,7 +240,7 @@ def _differentiable(hidden, weight, ids, logits, valid, temperature, reduction):
 def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
                         valid: Optional[torch.Tensor] = None, *, reduction: str = "mean") -> torch.Tensor:
     """``-log softmax(hidden @ weight.T)[targets]`` in float32: a scalar, or one per row with ``reduction="none"``.
-    Differentiable in ``hidden`` and ``weight``.  A reduced loss in bfloat16 makes its gradients at once, so score under
+    Differentiable in ``hidden`` and ``weight``, once and in reverse mode.  A reduced loss in bfloat16 makes its gradients at once, so score under
     ``torch.no_grad()``; without gradients wanted the call can be captured into a graph."""
     return _differentiable(hidden, weight, targets, None, valid, 1.0, reduction)
 

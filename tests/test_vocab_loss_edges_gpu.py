@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from supertoken_b200 import ops
 from test_vocab_loss_gpu import E32, formula, make, near
@@ -238,3 +239,29 @@ def test_the_range_of_temperatures(T, dtype):
                 ops.vocab_distillation(h, args[1], ids, logits, temperature=t, reduction="none")
             with pytest.raises(ValueError, match="temperature"):
                 ops.vocab_distillation_grads(h, args[1], ids, logits, temperature=t, reduction="none")
+
+
+@pytest.mark.parametrize("K", [0, 4])
+def test_forward_mode_is_refused(K):
+    """A tangent is not dropped: by the losses, by the calls for gradients, and on its way down to a loss."""
+    args = make(2, 20, 64, 500, K)
+    loss_of, grads_of = (ops.vocab_distillation, ops.vocab_distillation_grads) if K else (ops.vocab_cross_entropy, ops.vocab_cross_entropy_grads)
+    h = args[0].clone().requires_grad_(True)
+    eager = {r: loss_of(h, *args[1:], reduction=r) for r in ("sum", "none")}
+    with fw.dual_level():
+        for which in (0, 1, 3) if K else (0, 1):
+            dual = list(args)
+            dual[which] = fw.make_dual(args[which], torch.ones_like(args[which]))
+            for call in (loss_of, grads_of):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*dual)
+        for loss in eager.values():
+            up = fw.make_dual(torch.ones_like(loss), torch.ones_like(loss))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(loss, h, up, retain_graph=True)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                grads_of(*args, None, up, reduction="sum" if loss.dim() == 0 else "none")
+        plain = loss_of(*args)  # nothing has a tangent
+    assert torch.equal(plain, loss_of(*args))
+    for reduction, loss in eager.items():  # as good as before the refusals
+        near(torch.autograd.grad(loss.sum(), h)[0], formula(*args, reduction=reduction), "gh")
