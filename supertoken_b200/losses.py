@@ -231,6 +231,8 @@ def _refuse_capture(device: torch.device) -> None:
 
 def _differentiable(hidden, weight, ids, logits, valid, temperature, reduction):
     a = _arguments(hidden, weight, ids, logits, valid, temperature, reduction)
+    if logits is not None and logits.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("teacher_logits get no gradient: detach them")
     if (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
         _refuse_capture(hidden.device)
         return _VocabLoss.apply(hidden, weight, ids, logits, valid, a, temperature, reduction)
@@ -258,7 +260,8 @@ def vocab_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: 
                        teacher_logits: torch.Tensor, valid: Optional[torch.Tensor] = None, *, temperature: float = 1.0,
                        reduction: str = "mean") -> torch.Tensor:
     """``T^2 KL(p || softmax(hidden @ weight.T / T))`` with ``p = softmax(teacher_logits / T)`` over the teacher's up to 256
-    entries of a row (in any order; an id below 0 is no entry, the same id twice counts twice); ``T`` between 2^-16 and 2^16.  Gradients and captures as with
+    entries of a row (in any order; an id below 0 is no entry, the same id twice counts twice); ``T`` between 2^-16 and 2^16.  The
+    teacher's logits are constants: those that require a gradient are refused.  Gradients and captures as with
     ``vocab_cross_entropy``."""
     if teacher_logits is None:
         raise TypeError("teacher_logits must be a tensor")

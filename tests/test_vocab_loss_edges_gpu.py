@@ -265,3 +265,16 @@ def test_forward_mode_is_refused(K):
     assert torch.equal(plain, loss_of(*args))
     for reduction, loss in eager.items():  # as good as before the refusals
         near(torch.autograd.grad(loss.sum(), h)[0], formula(*args, reduction=reduction), "gh")
+
+
+def test_a_teacher_that_wants_a_gradient_is_refused():
+    hidden, weight, ids, logits = make(2, 20, 64, 500, 4)
+    plain = ops.vocab_distillation(hidden, weight, ids, logits)
+    logits.requires_grad_(True)
+    for h in (hidden, hidden.clone().requires_grad_(True)):
+        with pytest.raises(RuntimeError, match="detach"):
+            ops.vocab_distillation(h, weight, ids, logits)
+    assert torch.equal(ops.vocab_distillation(hidden, weight, ids, logits.detach()), plain)
+    with torch.no_grad():
+        assert torch.equal(ops.vocab_distillation(hidden, weight, ids, logits), plain)
+    assert ops.vocab_distillation_grads(hidden, weight, ids, logits)[1].shape == hidden.shape
