@@ -677,10 +677,8 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
             p.again = (int *)take(2 * p.rows_padded / TILE_ROWS * 4);
             p.scaled = take(p.chunk_rows * p.dim_padded * 2);
         }
-        if (p.chunk_rows < p.rows_padded) p.weight_acc = (float *)take(p.vocab * p.acc_stride * 4);
-        if (p.g_stride < all) {
-            p.acc = (float *)take(p.rows_padded * p.acc_stride * 4);
-        }
+        if (p.chunk_rows < p.rows_padded && p.grad_weight) p.weight_acc = (float *)take(p.vocab * p.acc_stride * 4);
+        if (p.g_stride < all && p.grad_hidden) p.acc = (float *)take(p.rows_padded * p.acc_stride * 4);
     }
     return STBPE_OK;
 }

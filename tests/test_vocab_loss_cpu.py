@@ -80,3 +80,10 @@ def test_temperatures_that_32_bits_do_not_hold():
     for t in (1e-20, 1e-10, 1e-5, 65537.0, 1e20, -2.0):
         st, n, text = _need(_args(k=4, logits_type=2, temperature=t))
         assert st == L.E_BADARG and n == -1 and "temperature" in text
+
+
+def test_no_workspace_for_a_gradient_that_is_not_wanted():
+    many = dict(outer=8, inner=2048, vocab=65536, dim=4096, hidden_outer=2048 * 4096, hidden_inner=4096, weight_stride=4096)
+    at_once, later = dict(many, want=3), dict(many, want=2, lse2=6 << 20)
+    assert _need(_args(**at_once))[1] - _need(_args(**at_once, grad_weight=0))[1] == 65536 * 4096 * 4
+    assert _need(_args(**later))[1] - _need(_args(**later, grad_hidden=0))[1] == 8 * 2048 * 4096 * 4

@@ -278,3 +278,19 @@ def test_a_teacher_that_wants_a_gradient_is_refused():
     with torch.no_grad():
         assert torch.equal(ops.vocab_distillation(hidden, weight, ids, logits), plain)
     assert ops.vocab_distillation_grads(hidden, weight, ids, logits)[1].shape == hidden.shape
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("frozen", [0, 1])
+def test_one_gradient_of_more_than_is_held_at_a_time(frozen, dtype):
+    """Two chunks of rows or two pieces of the vocabulary, one gradient wanted."""
+    hidden, weight, targets = make(1, 2300, 64, 300_001, dtype=dtype)
+    for reduction in ("mean", "none"):
+        want = formula(hidden, weight, targets, reduction=reduction, grad=64.0)
+        for name in ("gh_tol", "gw_tol"):  # what comes down is multiplied onto them once they are rounded
+            want[name] = want[name] * (1 + 2 ** -8) + torch.finfo(dtype).eps / 2 * want[name[:2]].abs()
+        h, w = hidden.clone().requires_grad_(frozen == 1), weight.clone().requires_grad_(frozen == 0)
+        loss = ops.vocab_cross_entropy(h, w, targets, reduction=reduction)
+        near(loss.detach(), want, "loss")
+        got, = torch.autograd.grad(loss, h if frozen else w, torch.tensor(64.0, device="cuda").expand_as(loss))
+        near(got, want, "gh" if frozen else "gw")
