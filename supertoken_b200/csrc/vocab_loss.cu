@@ -408,8 +408,9 @@ __global__ void __launch_bounds__(256) few_kernel(Plan p) {
 // ---------------------------------------------------------------------------------------------- after the products
 // Eight rows of a chunk (and a slice of their columns, where few rows are turned into G) to a block: joins what the parts of the columns left, in a fixed order (eight threads read a sector, 32 parts
 // at a time), to lse and the loss of a row; then a warp has a row.  Where E is kept, the row's E gets its entries and the packed row its factor.
+// all_blocks: of the joins of all chunks, the last of which adds up.
 template <class T>
-__global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int slices) {
+__global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int slices, unsigned all_blocks) {
     next_may_come();
     before_is_done();
     __shared__ float tops[8][8], sums[8][8], lse2s[8], refs[8];
@@ -475,7 +476,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
     // the block that is through last adds the losses up, in the order of the rows
     __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(&p.meta->tickets, 1u) == gridDim.x - 1;
+    if (threadIdx.x == 0) last = atomicAdd(&p.meta->tickets, 1u) == all_blocks - 1;
     __syncthreads();
     if (!last) return;
     __threadfence();
@@ -621,7 +622,7 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     const bool aligned = (uintptr_t)a->weight % 16 == 0 && a->weight_stride % 8 == 0 && a->weight_stride >= a->dim && a->dim % 8 == 0;
     p.weight_rows_stride = aligned ? a->weight_stride : p.dim_padded;
     if (!aligned && p.row_blocks > SMS / 4) p.row_blocks = SMS / 4;  // (the others align the weight: a block of either kind has an SM)
-    // at most KEPT bytes of E or G at a time (for large vocabularies 2048 rows of E, for many rows 2048 columns of G)
+    // at most KEPT bytes of E, G or parts' sums at a time (for large vocabularies 2048 rows of E or sums, for many rows 2048 columns of G)
     constexpr i64 KEPT = 1ll << 30, FIXED_BYTES = 48ll << 20;
     const i64 all = up_to(a->vocab, PIECE);
     p.keep = p.want_loss && p.want_grads;
@@ -629,12 +630,15 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
     if (p.keep) {
         const i64 most = KEPT / (2 * all) / TILE_ROWS * TILE_ROWS;
         p.chunk_rows = p.rows_padded <= most ? p.rows_padded : most > 2048 ? most : p.rows_padded < 2048 ? p.rows_padded : 2048;
+    } else if (!p.want_grads) {
+        const i64 most = KEPT / (8 * ((a->vocab + 63) / 64)) / TILE_ROWS * TILE_ROWS, least = most > 2048 ? most : 2048;
+        if (p.chunk_rows > least) p.chunk_rows = least;
     } else {
         const i64 most = KEPT / (2 * p.rows_padded) / PIECE * PIECE;
         p.g_stride = all <= most ? all : most > 2048 ? most : all < 2048 ? all : 2048;
     }
     p.fixed = p.keep && a->type == STBPE_REAL_BF16 && p.rows * a->vocab * 2 > FIXED_BYTES;
-    p.group = group_of(p.keep && p.chunk_rows < p.rows ? p.chunk_rows : p.rows, a->vocab, 0, 0, a->dim, 0, false, false);
+    p.group = group_of(p.chunk_rows < p.rows ? p.chunk_rows : p.rows, a->vocab, 0, 0, a->dim, 0, false, false);
     p.parts = (int)((a->vocab + 64 * p.group - 1) / (64 * p.group));
     p.part_stride = p.chunk_rows;
     p.few = !p.want_grads && !p.k && aligned && p.rows > 0 && p.rows <= FEW_ROWS && p.dim * (p.rows <= 2 ? p.rows : p.rows <= 4 ? 4 : 8) <= FEW_NUMBERS;
@@ -760,7 +764,7 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
     if (p.few) {
         auto *few = p.rows == 1 ? few_kernel<T, 1> : p.rows == 2 ? few_kernel<T, 2> : p.rows <= 4 ? few_kernel<T, 4> : few_kernel<T, 8>;
         VCK(start(few, p.parts, 256, 0, 1, s, p));
-        VCK(start(join_kernel<T>, 1, 256, 0, 1, s, p, 0, p.rows_padded, 1));
+        VCK(start(join_kernel<T>, 1, 256, 0, 1, s, p, 0, p.rows_padded, 1, 1));
         return STBPE_OK;
     }
     if (p.k) {
@@ -787,7 +791,7 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
                 if (p.fixed) VTRY((product<T, MAKE_E>(p, job, logits, s, err, err_len)));
             }
             if (!p.fixed) VTRY((product<T, MAKE_R>(p, job, logits, s, err, err_len)));
-            VCK(start(join_kernel<T>, joins * slices, 256, 0, 1, s, p, r0, p.chunk_rows, slices));
+            VCK(start(join_kernel<T>, joins * slices, 256, 0, 1, s, p, r0, p.chunk_rows, slices, 0));
             if constexpr (std::is_same<T, __nv_bfloat16>::value) {
                 job.again = true;
                 if (p.fixed) VTRY((product<T, MAKE_E>(p, job, logits, s, err, err_len)));
@@ -798,8 +802,11 @@ int run(const Plan &p, int type, cudaStream_t s, char *err, size_t err_len) {
         }
     } else {
         if (p.want_loss) {
-            VTRY((product<T, STATS>(p, Job{0, p.vocab, 0, p.rows_padded, false, false}, logits, s, err, err_len)));
-            VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, 0, p.rows_padded, 1));
+            const i64 chunks = (p.rows_padded + p.chunk_rows - 1) / p.chunk_rows;
+            for (i64 r0 = 0; r0 < p.rows_padded; r0 += p.chunk_rows) {
+                VTRY((product<T, STATS>(p, Job{0, p.vocab, r0, p.chunk_rows, false, false}, logits, s, err, err_len)));
+                VCK(start(join_kernel<T>, joins, 256, 0, 1, s, p, r0, p.chunk_rows, 1, joins * chunks));
+            }
         }
         if (p.want_grads) {
             if (p.refined) VCK(start(refine_kernel<T>, blocks(p.rows, 8), 256, 0, 1, s, p));

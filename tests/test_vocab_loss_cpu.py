@@ -87,3 +87,12 @@ def test_no_workspace_for_a_gradient_that_is_not_wanted():
     at_once, later = dict(many, want=3), dict(many, want=2, lse2=6 << 20)
     assert _need(_args(**at_once))[1] - _need(_args(**at_once, grad_weight=0))[1] == 65536 * 4096 * 4
     assert _need(_args(**later))[1] - _need(_args(**later, grad_hidden=0))[1] == 8 * 2048 * 4096 * 4
+
+
+def test_scoring_many_rows_takes_a_bounded_workspace():
+    """What follows from rows times vocabulary is held for a chunk of the rows: 2^20 rows of 262 144 ids have 2 GiB of sums and maxima per 131 072 rows."""
+    rows = dict(outer=1024, inner=1024, vocab=262144, dim=64, hidden_outer=1024 * 64, hidden_inner=64, weight_stride=64, want=1)
+    inputs = (1 << 20) * 64 * 2
+    assert _need(_args(**rows))[1] < (1 << 30) + 2 * inputs
+    # a teacher's rows have two bytes for every 256 ids, too
+    assert _need(_args(**rows, k=16, logits_type=2))[1] < (1 << 30) + 4 * inputs + (1 << 20) * 1024 * 2

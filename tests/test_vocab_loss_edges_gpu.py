@@ -294,3 +294,24 @@ def test_one_gradient_of_more_than_is_held_at_a_time(frozen, dtype):
         near(loss.detach(), want, "loss")
         got, = torch.autograd.grad(loss, h if frozen else w, torch.tensor(64.0, device="cuda").expand_as(loss))
         near(got, want, "gh" if frozen else "gw")
+
+
+@pytest.mark.parametrize("K", [0, 5])
+def test_more_rows_are_scored_than_are_held_at_a_time(K):
+    """Two chunks of rows; some of both by their formula, and their sum."""
+    rows, V = 9000, 1_000_003
+    args = list(make(1, rows, 8, V, K))
+    some = torch.tensor([0, 1, 255, 8191, 8447, 8448, 8449, 8703, 8704, 8999], device="cuda")
+    loss_of = ops.vocab_distillation if K else ops.vocab_cross_entropy
+    each = loss_of(*args, reduction="none")
+    for at in some:
+        one = [args[0][:, at:at + 1], args[1], *(x[:, at:at + 1] for x in args[2:])]
+        near(each[:, at:at + 1], formula(*one, reduction="none"), "loss")
+    mean = float(each.double().mean())
+    assert abs(float(loss_of(*args)) / mean - 1) <= 2.0 ** -24
+    few = torch.arange(rows, device="cuda")[None] % 3 == 0  # fewer than a chunk count
+    kept = loss_of(*args, few, reduction="none")
+    assert bool((kept[~few] == 0).all())
+    # (the rows have other places in their tiles, which changes no row's sums)
+    assert torch.equal(kept[few], each[few])
+    assert abs(float(loss_of(*args, few, reduction="sum")) / float(kept.double().sum()) - 1) <= 2.0 ** -24
