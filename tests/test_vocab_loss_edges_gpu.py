@@ -315,3 +315,74 @@ def test_more_rows_are_scored_than_are_held_at_a_time(K):
     # (the rows have other places in their tiles, which changes no row's sums)
     assert torch.equal(kept[few], each[few])
     assert abs(float(loss_of(*args, few, reduction="sum")) / float(kept.double().sum()) - 1) <= 2.0 ** -24
+
+
+def loss_bound(hidden, weight, args, T=1.0):
+    """Per row: the bounds of ``norms`` for any row, that is, cut sums of the tensor cores in the target's logit and in lse, and 16 e (1 + |log p|) for a
+    teacher's shares.  About 1e-5 of the loss, where the sum of |h w| that bounds any order of the terms allows a thousand times as much."""
+    n, D = math.prod(hidden.shape[:-1]), hidden.shape[-1]
+    z = hidden.reshape(n, D).double() @ weight.double().T / T
+    bound = 8 * 2.0 ** -24 * (torch.logsumexp(z, 1).abs() / math.log(2) + 1) + 2 * (D / 16 + 4) * E32 * z.abs().amax(1) + 16 * E32
+    if len(args) == 2:
+        logp = torch.log_softmax(args[1].reshape(n, -1).double() / T, 1)
+        bound = bound + 16 * E32 * (logp.exp() * logp.abs()).sum(1)
+    return T * T * bound
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,L,D,V,K,T", [(2, 300, 770, 4099, 0, 1.0), (8, 64, 1024, 8256, 0, 1.0), (3, 171, 136, 513, 7, 1.0), (1, 300, 520, 20_000, 3, 2.0),
+                                         (3, 900, 64, 10_000, 0, 1.0), (1, 1000, 1032, 30_000, 7, 1.5), (1, 1000, 771, 30_000, 0, 1.0)])
+def test_how_near_in_norms(B, L, D, V, K, T, dtype):
+    """Losses row by row at about 1e-5 of them, gradients at what three roundings to 16 bits leave, and no factor on them."""
+    hidden, weight, *args = make(B, L, D, V, K, dtype=dtype)
+    kd = {"temperature": T} if K else {}
+    loss_of, grads_of = (ops.vocab_distillation, ops.vocab_distillation_grads) if K else (ops.vocab_cross_entropy, ops.vocab_cross_entropy_grads)
+    bound, u = loss_bound(hidden, weight, args, T), torch.finfo(dtype).eps / 2
+    up = torch.linspace(1024.0, 4096.0, B * L, device="cuda").view(B, L)
+    for reduction, grad in (("mean", 4096.0), ("none", up)):
+        want = formula(hidden, weight, *args, T=T, reduction=reduction, grad=grad)
+        each = formula(hidden, weight, *args, T=T, reduction="none")["loss"].flatten()
+        loss, gh, gw = grads_of(hidden, weight, *args, None, grad, reduction=reduction, **kd)
+        h, w = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+        auto = loss_of(h, w, *args, reduction=reduction, **kd)
+        ah, aw = torch.autograd.grad(auto, (h, w), torch.as_tensor(grad, device="cuda").expand_as(auto))
+        for x in (loss, auto.detach(), loss_of(hidden, weight, *args, reduction=reduction, **kd)):
+            if reduction == "none":
+                assert bool(((x.flatten().double() - each).abs() <= bound).all())
+            else:
+                assert abs(float(x) - float(each.mean())) <= float(bound.mean())
+        for name, x in (("gh", gh), ("gh", ah), ("gw", gw), ("gw", aw)):
+            near_in_norm(x, want[name], u, 0.0, f"{name}, {reduction}")
+
+
+@pytest.mark.parametrize("K", [0, 7])
+@pytest.mark.parametrize("D", [770, 1032])
+def test_large_steps_with_rows_of_any_height(D, K):
+    """As much of E as has a fixed reference, at widths whose targets are summed again: rows above and below it that are made again, a teacher that is
+    sure, rows that do not count between them."""
+    hidden, weight, *args = make(1, 1000, D, 30_000, K)
+    weight[:, 0], hidden[..., 0] = 1.0, 0.0
+    for at, height in ((17, 90.0), (18, -90.0), (300, 70.0), (301, -70.0), (302, -50.0), (700, 200.0), (999, -300.0)):
+        hidden[0, at, 0] = height
+    if K:
+        args[1][0, ::2, 3] = 9.0
+    valid = torch.arange(1000, device="cuda")[None] % 5 != 2
+    valid[0, 512:768] &= torch.arange(256, device="cuda") < 100
+    hidden = torch.where(valid[..., None], hidden, math.nan)
+    clean = torch.where(valid[..., None], hidden, 0.0)
+    kd = {"temperature": 1.5} if K else {}
+    grads_of = ops.vocab_distillation_grads if K else ops.vocab_cross_entropy_grads
+    bound = torch.where(valid[0], loss_bound(clean, weight, args, 1.5 if K else 1.0), 0.0)
+    for reduction in ("mean", "none"):
+        want = formula(clean, weight, *args, valid=valid, T=1.5 if K else 1.0, reduction=reduction, grad=64.0)
+        loss, gh, gw = grads_of(hidden, weight, *args, valid, 64.0, reduction=reduction, **kd)
+        near(loss, want, "loss"), near(gh, want, "gh"), near(gw, want, "gw")
+        assert bool((gh[~valid] == 0).all())
+        if reduction == "none":
+            assert bool(((loss[0].double() - want["loss"][0]).abs() <= bound).all())
+        # (the column that the heights go through cancels in dH and is made of a few rows in dW)
+        near_in_norm(gh[..., 1:], want["gh"][..., 1:], 2.0 ** -8, 0.0, "gh"), near_in_norm(gw[:, 1:], want["gw"][:, 1:], 2.0 ** -8, 0.0, "gw")
+    args[0][0, 18 if not K else slice(18, 19)] = 30_000  # an id outside, in a row that is made again
+    loss, gh, gw = grads_of(hidden, weight, *args, valid, reduction="none", **kd)
+    assert loss.isnan().nonzero().tolist() == [[0, 18]] and bool(gh[0, 18].isnan().all()) and bool(gw.isnan().all())
+    assert not bool(gh[0, :18].isnan().any()) and not bool(gh[0, 19:].isnan().any())
