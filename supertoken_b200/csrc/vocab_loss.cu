@@ -413,7 +413,7 @@ template <class T>
 __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int slices, unsigned all_blocks) {
     next_may_come();
     before_is_done();
-    __shared__ float tops[8][8], sums[8][8], lse2s[8], refs[8];
+    __shared__ float tops[8][8], sums[8][8], logits[8][8], lse2s[8], means[8], refs[8];
     __shared__ double losses[8];
     __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -422,13 +422,18 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
     const i64 until = p.fixed ? (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS : n;
     const int slice = blockIdx.x % slices;
     for (i64 m0 = (i64)(blockIdx.x / slices) * 8; m0 < until; m0 += (i64)(gridDim.x / slices) * 8) {
-        float top = LOWEST, sum = 0.f;
-        auto add = [&](float m, float x) {
+        float top = LOWEST, sum = 0.f, logit = 0.f;  // of the row's parts, and the sum of the maxima times their sums
+        auto add = [&](float m, float x, float y) {
             const float both = fmaxf(top, m);
-            // (with a fixed reference all parts of a row have it)
-            sum = p.fixed ? sum + x : sum * exp2f(top - both) + x * exp2f(m - both);
+            if (p.fixed) {  // all parts of a row have the same reference
+                sum += x, logit += y;
+            } else {
+                const float f = exp2f(top - both), g = exp2f(m - both);
+                sum = sum * f + x * g, logit = logit * f + y * g;
+            }
             top = both;
         };
+        const float shift = p.keep && !p.fixed ? 14.f : 0.f;  // (MAKE_R: what the maxima are less by)
         // the row of this warp; the sum of its target's logit needs nothing of the parts
         const i64 m = m0 + warp, slot = r0 + m;
         const int row = m < n ? p.row_of[slot] : 0;
@@ -437,18 +442,21 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
         if (m0 + (lane & 7) < n) {
             const float *from_max = p.part_max + m0 + (lane & 7), *from_sum = p.part_sum + m0 + (lane & 7);
 #pragma unroll 4
-            for (int t = warp * 4 + (lane >> 3); t < p.parts; t += 32) add(from_max[t * p.part_stride], from_sum[t * p.part_stride]);
+            for (int t = warp * 4 + (lane >> 3); t < p.parts; t += 32) {
+                const float m = from_max[t * p.part_stride], x = from_sum[t * p.part_stride];
+                add(m, x, x * (m + shift));
+            }
         }
         for (int d = 8; d < 32; d <<= 1) {
-            const float m = __shfl_xor_sync(~0u, top, d), x = __shfl_xor_sync(~0u, sum, d);
-            add(m, x);
+            const float m = __shfl_xor_sync(~0u, top, d), x = __shfl_xor_sync(~0u, sum, d), y = __shfl_xor_sync(~0u, logit, d);
+            add(m, x, y);
         }
         if (refined >= 0) sum_z = entry_logit<T>(p, slot, row, refined, lane);
-        if (lane < 8) tops[warp][lane] = top, sums[warp][lane] = sum;
+        if (lane < 8) tops[warp][lane] = top, sums[warp][lane] = sum, logits[warp][lane] = logit;
         __syncthreads();
         if (threadIdx.x < 8) {
-            top = tops[0][lane], sum = sums[0][lane];
-            for (int w = 1; w < 8; ++w) add(tops[w][lane], sums[w][lane]);
+            top = tops[0][lane], sum = sums[0][lane], logit = logits[0][lane];
+            for (int w = 1; w < 8; ++w) add(tops[w][lane], sums[w][lane], logits[w][lane]);
             float ref = top;
             // a logit of +inf makes the sum NaN about a maximum, and has to about a fixed reference
             if (p.fixed && top == INFINITY) sum = NAN;
@@ -461,12 +469,12 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
                     p.again[(r0 + m0) / TILE_ROWS] = p.meta->again = 1;
                 }
             }
-            refs[lane] = ref, lse2s[lane] = ref + log2f(sum);
+            refs[lane] = ref, lse2s[lane] = ref + log2f(sum), means[lane] = logit / sum;
         }
         __syncthreads();
         T *scaled = (T *)p.scaled + m * p.dim_padded;
         if (m < n) {
-            finish_row<T>(p, m, slot, row, lse2s[warp], refs[warp], refined, sum_z, lane, slice, slices);
+            finish_row<T>(p, m, slot, row, lse2s[warp], means[warp], refs[warp], refined, sum_z, lane, slice, slices);
         } else if (p.fixed && m < until) {  // zeros behind the last row
             for (int d = lane * 8; d < p.dim_padded; d += 256) *(uint4 *)(scaled + d) = make_uint4(0, 0, 0, 0);
         }
