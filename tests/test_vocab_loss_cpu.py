@@ -96,3 +96,74 @@ def test_scoring_many_rows_takes_a_bounded_workspace():
     assert _need(_args(**rows))[1] < (1 << 30) + 2 * inputs
     # a teacher's rows have two bytes for every 256 ids, too
     assert _need(_args(**rows, k=16, logits_type=2))[1] < (1 << 30) + 4 * inputs + (1 << 20) * 1024 * 2
+
+
+def test_calls_run_on_their_tensors_device(monkeypatch):
+    """Another device is current: launches, the gradients' scaling and the question for a capture go to the tensors' own, and the current one stays."""
+    now, seen = [1], []
+
+    class Switch:
+        def __init__(self, device):
+            self.index = device if isinstance(device, int) else device.index
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.index
+
+        def __exit__(self, *_):
+            now[0] = self.before
+
+    class Library:
+        def stbpe_vocab_loss_workspace(self, *_):
+            seen.append(("workspace", now[0]))
+            return L.E_BADARG
+
+        def stbpe_scale_gradients(self, *args):
+            seen.append(("scale", now[0], args[-1]))
+            return L.OK
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", Switch)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: seen.append(("capture", now[0])) or False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index, raising=False)
+    monkeypatch.setattr(L, "load", Library)
+    for index in (0, 1, 2):
+        device = torch.device("cuda", index)
+        with pytest.raises(ValueError):
+            losses._run(_args(), device)
+        by = type("Up", (), {"device": device, "data_ptr": lambda self: 512})()
+        losses._scale(None, None, by)
+        losses._refuse_capture(device)
+        assert seen == [("workspace", index), ("scale", index, 100 + index), ("capture", index)] and now == [1]
+        seen.clear()
+
+
+def test_the_bounds_in_norms_see_a_loss_of_precision():
+    """Mistakes that are planted in the formula: logits in 16 bits, a factor of half a percent, a target's logit that is cut off."""
+    from test_vocab_loss_edges_gpu import loss_bound, near_in_norm
+    g = torch.Generator().manual_seed(0)
+    rows, D, V, u = 256, 1024, 2048, 2.0 ** -8
+    hidden = torch.randn(1, rows, D, generator=g).bfloat16()
+    weight = (torch.randn(V, D, generator=g) / 32).bfloat16()
+    t = torch.randint(0, V, (rows,), generator=g)
+    z = hidden[0].double() @ weight.double().T
+    bound = loss_bound(hidden, weight, (t[None],))
+
+    def results(z, factor=1.0):
+        lse = torch.logsumexp(z, 1)
+        G = (z - lse[:, None]).exp()
+        G[torch.arange(rows), t] -= 1.0
+        G *= factor
+        return lse - z[torch.arange(rows), t], (G @ weight.double()).bfloat16(), (G.T @ hidden[0].double()).bfloat16()
+
+    loss, gh, gw = results(z)
+    want = [x.double() for x in results(z)[1:]]
+    near_in_norm(gh, want[0], u, 0.0, "gh"), near_in_norm(gw, want[1], u, 0.0, "gw")
+    for factor in (1.005, 0.995):
+        for got, right in zip(results(z, factor)[1:], want):
+            with pytest.raises(AssertionError):
+                near_in_norm(got, right, u, 0.0, "")
+    assert bool(((results(z.bfloat16().double())[0] - loss).abs() > bound).any())
+    cut = z.clone()
+    cut[torch.arange(rows), t] *= 1 - 2.0 ** -13
+    assert bool(((results(cut)[0] - loss).abs() > bound).any())
+    assert float((bound / loss).max()) < 2e-5
