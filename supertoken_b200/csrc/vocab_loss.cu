@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
     const i64 until = p.fixed ? (n + TILE_ROWS - 1) / TILE_ROWS * TILE_ROWS : n;
     const int slice = blockIdx.x % slices;
     for (i64 m0 = (i64)(blockIdx.x / slices) * 8; m0 < until; m0 += (i64)(gridDim.x / slices) * 8) {
-        float top = LOWEST, sum = 0.f, logit = 0.f;  // of the row's parts, and the sum of the maxima times their sums
+        float top = LOWEST, sum = 0.f, logit = 0.f;  // of the row's parts: maximum, sum of exp, that times the mean logit
         auto add = [&](float m, float x, float y) {
             const float both = fmaxf(top, m);
             if (p.fixed) {  // all parts of a row have the same reference
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
             }
             top = both;
         };
-        const float shift = p.keep && !p.fixed ? 14.f : 0.f;  // (MAKE_R: what the maxima are less by)
+        const float shift = p.keep && !p.fixed ? 14.f : 0.f, side = 5 + p.group;  // (MAKE_R: what the maxima are less by; 2^6 columns to a part, or 2^7)
         // the row of this warp; the sum of its target's logit needs nothing of the parts
         const i64 m = m0 + warp, slot = r0 + m;
         const int row = m < n ? p.row_of[slot] : 0;
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(256) join_kernel(Plan p, i64 r0, i64 rows, int
 #pragma unroll 4
             for (int t = warp * 4 + (lane >> 3); t < p.parts; t += 32) {
                 const float m = from_max[t * p.part_stride], x = from_sum[t * p.part_stride];
-                add(m, x, x * (m + shift));
+                add(m, x, refines(p) ? x * mean_of_part(m + shift, log2f(x) - (p.fixed ? m : shift), side) : 0.f);
             }
         }
         for (int d = 8; d < 32; d <<= 1) {
@@ -682,7 +682,7 @@ int plan(const stbpe_vocab_loss *a, Plan &p, i64 &bytes, char *err, size_t err_l
         p.g = take(p.chunk_rows * p.g_stride * 2);
         p.split_sums = (float *)take((i64)2 * SMS * 8 * 64 * 2 * 32 * 4);
         p.split_done = (unsigned int *)take(2 * SMS * 8 * 4);
-        if (!p.keep && p.dim > REFINED_DIM) p.refined = (int2 *)take(p.rows_padded * 8);
+        if (!p.keep && refines(p)) p.refined = (int2 *)take(p.rows_padded * 8);
         if (p.fixed) {
             p.reference = (float *)take(p.rows_padded * 4);
             p.out_row = (float *)take(p.rows_padded * 4);

@@ -88,13 +88,14 @@ struct Plan {
 // token (a share about e^-7 below 1 at a width of 4 096 in fp16: dH and dW would be off by 28 % in the 2-norm, and are by 0.1 %).
 // The other logits are as short as they are large, and where they are as large as the target's, as logits with an offset in common are, or
 // those of several likely tokens, the loss would be off by what the target alone was corrected by.  So lse gets for them what the target
-// was short by, of itself, times their mean: each part's largest for all of the part, by its share.  Width 4 096, all logits about 20: mean loss 1.8e-4
-// too small without that, 2.5e-5 too large with it; losses of 0.04 between likely tokens in fp16: 2.5e-4 too small, 2.2e-5.
+// was short by, of itself, times their mean by shares.  Width 4 096, all logits about 20: the mean loss was 1.8e-4 too small without that and is 1.2e-5 too
+// large; losses of 0.04 between likely tokens in fp16: 2.5e-4 too small, 2.2e-5; a target that the row points to, others about 0: 5e-6 too small, 1e-6 too large.
 constexpr int REFINED_DIM = 512;
+__host__ __device__ __forceinline__ bool refines(const Plan &p) { return !p.few && p.dim > REFINED_DIM; }
 
 // which entry of the row that is, -1: none
 __device__ __forceinline__ int refined_entry(const Plan &p, int row, int lane) {
-    if (p.few || p.dim <= REFINED_DIM) return -1;
+    if (!refines(p)) return -1;
     if (!p.k) return p.entries[row].x != INT_MAX ? 0 : -1;
     int found = -1;
     for (int k = lane; k < p.k; k += 32) {
@@ -117,6 +118,14 @@ __device__ __forceinline__ float entry_logit(const Plan &p, i64 slot, int row, i
     }
     for (int d = 16; d; d >>= 1) z += __shfl_xor_sync(~0u, z, d);
     return z;
+}
+
+// The mean of a part's logits by their shares, about: its largest less what shares of 2^side normally distributed logits lie below it on average.  size is
+// the logarithm of the part's sum of exponentials about the largest: 0 where that is alone and side where all are as large, when the mean is the
+// largest, and a parabola between, less than half a power of e off for any deviation where the largest is up to 1.8 off.  All in powers of 2.
+__device__ __forceinline__ float mean_of_part(float top, float size, float side) {
+    const float l = fminf(fmaxf(size, 0.f), side);
+    return top - 0.18f * l * (side - l);
 }
 
 // What follows from a row's lse2 (mean: of its logits, in powers of 2): its loss.  Where E has a fixed reference, the entries in E (from their logits in 32 bits, once
@@ -204,14 +213,15 @@ __device__ __noinline__ void join_again(const Plan &p, i64 r0, i64 m0, i64 n, in
     for (i64 m = m0; m < m0 + TILE_ROWS && m < n; ++m) {
         const i64 slot = r0 + m;
         const int row = p.row_of[slot];
+        const float ref = p.reference[slot];
         float sum = 0.f, logits = 0.f;
         for (int t = lane; t < p.parts; t += 32) {
             const float x = __ldcg(p.part_sum + t * p.part_stride + m);
-            sum += x, logits += x * __ldcg(p.part_max + t * p.part_stride + m);
+            const float y = __ldcg(p.part_max + t * p.part_stride + m);
+            sum += x, logits += x * mean_of_part(y, log2f(x) + ref - y, 5 + p.group);
         }
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d), logits += __shfl_xor_sync(~0u, logits, d);
         if (sum == INFINITY) sum = NAN;  // a logit of +inf: no other is that far from its reference by now
-        const float ref = p.reference[slot];
         const int refined = refined_entry(p, row, lane);
         finish_row<T>(p, m, slot, row, ref + log2f(sum), logits / sum, ref, refined, refined >= 0 ? entry_logit<T>(p, slot, row, refined, lane) : 0.f, lane);
     }
