@@ -138,13 +138,14 @@ __device__ __forceinline__ void finish_row(const Plan &p, i64 m, i64 slot, int r
     const float scale = p.inv_temperature * 1.4426950408889634f;
     const int2 *e = p.entries + (i64)row * entries_of_row;
     const float *z = p.entry_z + slot * entries_of_row;
+    float longer = 1.f;  // what a teacher's other entries are set right by
     if (refined >= 0) {
         const float before = z[refined], share = exp2f(fmaf(before, scale, -lse2));
         // (a logit of -inf has no share, and no difference to itself)
         if (share > 0.f) lse2 += log1pf(share * expm1f((target - before) * p.inv_temperature)) * 1.4426950408889634f;
         // no more than half a step of 32 bits for each of the sum's (a target near 0 does not tell)
         const float cut = fminf(fmaxf((target - before) / before, 0.f), p.dim * (1.f / 16 / 16777216));
-        if (cut > 0.f) lse2 += cut * (mean - share * before * scale);
+        if (cut > 0.f) lse2 += cut * (mean - share * before * scale), longer += cut;
     }
     const int refined_id = refined >= 0 ? e[refined].x : -1;  // (in more than one entry, if a teacher gives it twice)
     float unit = exp2f(lse2 - ref), minus = ref, times = 1.f;  // a share, the logits and a factor in the units of E
@@ -177,7 +178,7 @@ __device__ __forceinline__ void finish_row(const Plan &p, i64 m, i64 slot, int r
     for (int k = lane; k < entries_of_row; k += 32) {
         const int2 it = e[k];
         if (it.x == INT_MAX) break;
-        const float its = it.x == refined_id ? target : z[k];
+        const float its = it.x == refined_id ? target : z[k] * longer;
         pz += __int_as_float(it.y) * its;
         if (p.keep && it.x >= from_j && it.x < to_j && (k == 0 || e[k - 1].x != it.x)) {  // (the same id again: its first entry takes them all)
             float share = __int_as_float(it.y);

@@ -389,17 +389,21 @@ def test_large_steps_with_rows_of_any_height(D, K):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K", [0, 4])
 @pytest.mark.parametrize("D", [1024, 4096])
 @pytest.mark.parametrize("offset", [20.0, -20.0])
-def test_logits_with_an_offset_in_common(offset, D, dtype):
+def test_logits_with_an_offset_in_common(offset, D, K, dtype):
     """The target's logit is not summed once more at the cost of the others'.  Sums of 16 to 32 are cut off by half a step of 2^-19 on average in each of D / 16
-    steps; what the target was cut by, of itself, times a mean of the logits that is too large by at most log 128 (a part's largest for all 128 of it)
-    and as far off as the target's own logit, 1 on average, leaves that by (log 128 + 1) / 20; and the roundings of ``norms``."""
-    hidden, weight, targets = make(1, 500, D, 8000, dtype=dtype)
+    steps; what the target was cut by, of itself, times a mean of normally distributed logits that is off by at most 1 / 2, and by the target's own
+    logit, 1 on average, leaves that by 1.5 / 20; and the roundings of ``norms``.  A teacher's entries but the one with 0.51 of the share are off by
+    as much as the target's own logit is, 1 / 20 of the cut."""
+    hidden, weight, *args = make(1, 500, D, 8000, K, dtype=dtype)
     weight[:, 0], hidden[..., 0] = 1.0, offset
-    want = formula(hidden, weight, targets, reduction="none")
-    left = D / 16 * 2.0 ** -20 * (math.log(128) + 1) / 20
+    if K:
+        args[1][:] = torch.tensor([0.18, 0.51, 0.16, 0.15], device="cuda").log()
+    loss_of, grads_of = (ops.vocab_distillation, ops.vocab_distillation_grads) if K else (ops.vocab_cross_entropy, ops.vocab_cross_entropy_grads)
+    want = formula(hidden, weight, *args, reduction="none")
+    left = D / 16 * 2.0 ** -20 * (1.5 + (0.49 if K else 0.0)) / 20
     off = float(8 * 2.0 ** -24 * (torch.logsumexp(hidden[0].double() @ weight.double().T, 1).abs() / math.log(2) + 1).mean())
-    for loss in (ops.vocab_cross_entropy(hidden, weight, targets, reduction="none"),
-                 ops.vocab_cross_entropy_grads(hidden, weight, targets, reduction="none")[0]):
+    for loss in (loss_of(hidden, weight, *args, reduction="none"), grads_of(hidden, weight, *args, reduction="none")[0]):
         assert abs(float((loss.double() - want["loss"]).mean())) <= left + off
