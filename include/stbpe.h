@@ -327,7 +327,8 @@ int stbpe_rows_count_pairs_noalloc(const int32_t *tokens, const uint8_t *valid, 
  * They have no counterpart in the reference, whose padded batches (tokens, valid) they take.  Rows are outer x inner,
  * every array is reached by its strides (in elements, the last dimension contiguous).  A row does not count where valid is 0, its
  * id is negative (k == 0), or it has no entry with an id of 0 or more and a logit above -inf (k > 0): its loss and its row of
- * grad_hidden are 0 and what it holds is not multiplied.  An id of vocab or more, or a logit of NaN or +inf, gives NaN.
+ * grad_hidden are 0 and what it holds is not multiplied.  An id of vocab or more, or a logit of NaN or +inf, gives NaN;
+ * a target's of -inf a loss of +inf.
  *   STBPE_WANT_LOSS  : loss[rows] (no reduction) or loss[1] (sum, or mean over the rows that count; 0 if none does), and
  *                      lse2[rows] (NULL: not wanted), log2 of the sum, which a later call for the gradients takes
  *   STBPE_WANT_GRADS : grad_hidden[rows][dim] and grad_weight[vocab][dim] in the inputs' type (NULL: not wanted), times

@@ -5,8 +5,8 @@
 //   loss_i = T^2 (lse_i + sum_k p_ik (log p_ik - s z_i,t_ik))
 //   G_ij = g_i T (exp(s z_ij - lse_i) - sum_k p_ik [j = t_ik])       dH = G W        dW = G^T H
 // The N x V logits are never stored.  Two ways to the gradients:
-//   keep    (loss and gradients at once): E_ij = exp2(z_ij s log2 e - c_i) goes to memory in 16 bits, for at most 1 GiB of rows at
-//           a time, and the sums that make lse_i (lse2_i in powers of 2) beside it.  Three products.
+//   keep    (loss and gradients at once): E_ij = exp2(z_ij s log2 e - c_i) goes to memory in 16 bits, for at most 1 GiB of rows (or 2 048
+//           of them) at a time, and the sums that make lse_i (lse2_i in powers of 2) beside it.  Three products.
 //           With each part's own maximum (of 64 or 128 columns, less 14) as c, E has the range that fp16 needs, and becomes G
 //           where it lies once lse_i is known, the entries from z in 32 bits: E is read and written once more (0.2 ms for 4 336 rows of
 //           50 257), and G is rounded twice but for the entries, from which most of the gradients come.
@@ -16,7 +16,8 @@
 //           largest logit lies more than a factor of 2^96 above c_i or 2^80 below gets it as its reference and its tile is made again, which
 //           a largest logit between -55 and 66 never needs.
 //   anew    (gradients after the loss, as fp16 and losses per row need them through autograd): z is made a second time,
-//           and G from it for up to 1 GiB of the vocabulary at a time.  Three products behind the loss's one.
+//           and G from it for up to 1 GiB of the vocabulary (or 2 048 ids) at a time, the target's
+//           from the logit that the loss had.  Three products behind the loss's one: 3.2 ms for 8 188 x 32 256 x 2 048 in fp16, 2.9 at once.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -175,8 +176,9 @@ __device__ __forceinline__ void copy_row(T *to, const T *from, i64 inside, i64 a
 // Then counted rows of `hidden` go one behind another, zeros up to the end of the last tile, a warp to a row: products then do no
 // work for padding, never multiply what a masked row holds (it may be NaN), and may read rows of any stride or alignment.  The
 // rows of dH that do not count get their zeros here.
-// dlogits are held in the inputs' 16-bit type, so they are brought into that type's range: the largest |g_i T| becomes 16376 (fp16
-// keeps shares down to 2^-28 at full precision and its entries stay below 2^15; just below a power of two, a target's
+// dlogits are held in the inputs' 16-bit type, so they are brought into that type's range: the largest |g_i T| becomes 16376 (in the rows where |g_i| is
+// near the largest fp16 keeps shares down to 2^-28 at full precision; a row with 2^-20 of it keeps those down to 2^-8, and 2^-18 coarsely;
+// its entries stay below 2^15; just below a power of two, a target's
 // dlogit, -g T (1 - q), loses half as much to its rounding as just above one), and both gradients are scaled back in 32 bits.
 template <class T>
 __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Plan p) {
 // The losses of up to eight rows, as when text is scored as it is generated: bound by the weight, which is read once (V D 2 bytes), and by
 // launches, so numbering the rows and the product are one kernel.  A warp takes four of the weight's rows at a time, a lane 16 bytes of each per
 // 256 columns, against the rows of `hidden` in shared memory; sums in 32 bits, every block leaves its part as the tiles
-// of a product do.  17 MB of weight in 5 us, 13 us a call where the tensor cores' tiles of 128 rows and a launch more take 18.
+// of a product do.  17 MB of weight in 6 us, 12 to 14 us a captured call where the tensor cores' tiles of 128 rows and a launch more take 18.
 constexpr int FEW_ROWS = 8, FEW_NUMBERS = 16384;  // rows, and rows (rounded up to a power of two) times width
 template <class T, int ROWS>
 __global__ void __launch_bounds__(256) few_kernel(Plan p) {
@@ -578,7 +580,7 @@ int fail(char *err, size_t len, int status, const char *what, const char *why) {
 i64 up_to(i64 x, i64 unit) { return (x + unit - 1) / unit * unit; }
 
 // CTAs to a tile of a product, by what it takes: steps of 64 terms, 0.36 us for 256 x 256 by a pair and 0.28 for 128 x 128 by a single
-// CTA, of which twice as many run at a time (1.4 against 0.95 PFLOP/s).
+// CTA, of which twice as many run at a time: 1.7 against 1.1 PFLOP/s in a launch of few rounds (in long ones 1.5 to 1.6 against 0.93 to 0.98).
 int group_of(i64 rows, i64 cols, i64 rows2, i64 cols2, i64 depth, i64 depth2, bool split, bool split2) {
     double cost[3];
     for (int g = 1; g <= 2; ++g) {

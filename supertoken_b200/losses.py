@@ -10,7 +10,8 @@ their last.  Any strides, but for the last dimension of ``hidden``, ``weight`` a
 A row counts unless ``valid`` is 0 there or its target is negative (the padding of the batches); with a teacher, unless it has
 no entry with an id of 0 or more and a logit above ``-inf``.  Rows that do not count have a loss and a gradient of 0, and
 what ``hidden`` holds there is not looked at.  ``reduction="mean"`` divides by the rows that count (0 if none does).  Nothing is read back, so
-an id of ``V`` or more cannot raise: it makes the loss NaN, as a NaN among the inputs does.  Results are the same at every call with the same
+an id of ``V`` or more cannot raise: it makes the loss NaN, as a NaN among the inputs or a logit of
+``+inf`` does; a target's logit of ``-inf`` makes it ``+inf``.  Results are the same at every call with the same
 inputs; sums are held in 32 bits, those of the losses of rows in 64."""
 from __future__ import annotations
 
@@ -252,7 +253,8 @@ def vocab_cross_entropy_grads(hidden: torch.Tensor, weight: torch.Tensor, target
                               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(loss, grad_hidden, grad_weight)`` in one call without autograd, which can be captured into a graph.  The
     gradients are contiguous, in the inputs' type, and times ``grad_loss``: a number, a float32 tensor of one element (a loss
-    scale), or with ``reduction="none"`` one of the loss's shape."""
+    scale), or with ``reduction="none"`` one of the loss's shape.  In float16 all rows' dlogits are held at one scale, the largest
+    ``|grad_loss|``'s: rows with a millionth of it still have their gradient in full, those with less lose it bit by bit."""
     return _grads(_arguments(hidden, weight, targets, None, valid, 1.0, reduction), hidden, weight, reduction, grad_loss, None)[:3]
 
 

@@ -407,3 +407,21 @@ def test_logits_with_an_offset_in_common(offset, D, K, dtype):
     off = float(8 * 2.0 ** -24 * (torch.logsumexp(hidden[0].double() @ weight.double().T, 1).abs() / math.log(2) + 1).mean())
     for loss in (loss_of(hidden, weight, *args, reduction="none"), grads_of(hidden, weight, *args, reduction="none")[0]):
         assert abs(float((loss.double() - want["loss"]).mean())) <= left + off
+
+
+@pytest.mark.parametrize("down", [1.0, 1e-3, 1e-5, 1e-6])
+def test_rows_of_small_weight_in_half_precision(down):
+    """Without a reduction fp16 dlogits have the scale of the largest |grad_loss|, 16376.  In a row's gradient, of itself: its target's dlogit is off by u at the
+    most, everything else by roundings of u / sqrt(3) in the 2-norm, together less than 2 u; below 2^-14 all dlogits are rounded to 2^-24, that is
+    2^-25 / sqrt(3) each in the 2-norm, and so are the results; a row of them by half as much again at the most."""
+    rows, D, V = 300, 256, 3000
+    hidden, weight, targets = make(1, rows, D, V, dtype=torch.float16)
+    up = torch.full((1, rows), 65536.0 * down, device="cuda")
+    up[0, 0] = 65536.0
+    want = formula(hidden, weight, targets, reduction="none", grad=up)["gh"][0]
+    size, u = want.norm(dim=1), 2.0 ** -11
+    coarse = 2.0 ** -25 / math.sqrt(3) * (65536 / 16376 * float(weight.double().norm()) + math.sqrt(D))
+    h = hidden.clone().requires_grad_(True)
+    auto, = torch.autograd.grad(ops.vocab_cross_entropy(h, weight, targets, reduction="none"), h, up)
+    for gh in (ops.vocab_cross_entropy_grads(hidden, weight, targets, None, up, reduction="none")[1], auto):
+        assert bool(((gh[0].double() - want).norm(dim=1) <= 2 * u * size + 1.5 * coarse).all())
