@@ -425,3 +425,16 @@ def test_rows_of_small_weight_in_half_precision(down):
     auto, = torch.autograd.grad(ops.vocab_cross_entropy(h, weight, targets, reduction="none"), h, up)
     for gh in (ops.vocab_cross_entropy_grads(hidden, weight, targets, None, up, reduction="none")[1], auto):
         assert bool(((gh[0].double() - want).norm(dim=1) <= 2 * u * size + 1.5 * coarse).all())
+
+
+@pytest.mark.parametrize("D", [770, 1024])
+def test_a_targets_dlogit_is_not_rounded_on_large_steps(D):
+    """Cross entropy in bf16 with more than 48 MB of E: the row's factor takes back what its target's entry lost.  Numbers with mantissas that are spread evenly
+    over their logarithm round by 0.425 u in the 2-norm (the root of a third of the mean of 1 / m^2); dH has the result's own rounding, dW that and a H's, and
+    a tenth more is left to the other ids' shares, whose rows of the weight hardly add up."""
+    hidden, weight, targets = make(1, 1000, D, 30_000)
+    want = formula(hidden, weight, targets)
+    _, gh, gw = ops.vocab_cross_entropy_grads(hidden, weight, targets)
+    one = 1.1 * 0.425 * 2.0 ** -8
+    assert float((gh.double() - want["gh"]).norm() / want["gh"].norm()) <= one
+    assert float((gw.double() - want["gw"]).norm() / want["gw"].norm()) <= math.sqrt(2) * one
